@@ -769,6 +769,105 @@ hipError_t rlm_block_statistics(const rlm_tensor* keys, int64_t block_size,
                                 const rlm_tensor* out_mean, const rlm_tensor* out_std,
                                 hipStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * A routed attention layer (no reference counterpart: the reference's routed
+ * path picks one anchor and K partners where these attend)
+ *
+ * Inputs may be strided views with unit stride in their last dim; outputs are
+ * contiguous.  `positions` is 0-d, [Tq] (shared by the batch) or [B,Tq], int32
+ * or int64.
+ * ---------------------------------------------------------------------- */
+
+/*
+ * Rotary positions of query [B,Tq,Hq,D] and key [B,Tq,Hk,D]: pair i of a head
+ * turns by position * frequencies[i] (frequencies [F] f32, 2 F <= D; the angle
+ * is reduced in float64), both features times `scale`:
+ *   (a, b) -> scale * (a cos - b sin, a sin + b cos).
+ * Pair i is the features (i, F + i), or (2 i, 2 i + 1) where `interleaved`;
+ * features from 2 F on pass unchanged.  D <= 1024.
+ * Outputs: out_query, out_key of the inputs' shapes and dtype.
+ */
+hipError_t rlm_rotary_positions(const rlm_tensor* query, const rlm_tensor* key,
+                                const rlm_tensor* positions, const rlm_tensor* frequencies,
+                                int32_t interleaved, double scale, const rlm_tensor* out_query,
+                                const rlm_tensor* out_key, hipStream_t stream);
+
+/*
+ * rlm_rotary_positions of tokens that follow each other -- token i of batch row
+ * b at position[b] + i, `position` 0-d or [B] -- with the rotated key and the
+ * value [B,Tq,Hk,D] written to row position[b] + i of key_cache / value_cache
+ * [B,T,Hk,D] (mutated; any non-overlapping strides) instead of an output.
+ * Positions outside [0, T) and tokens from lengths[b] on (lengths [B] or NULL)
+ * leave the caches as they are.  ring: row (position[b] + i) mod T for any
+ * position >= 0, T a power of two, Tq <= T.
+ */
+hipError_t rlm_rotary_to_caches(const rlm_tensor* query, const rlm_tensor* key,
+                                const rlm_tensor* value, const rlm_tensor* position,
+                                const rlm_tensor* frequencies, const rlm_tensor* key_cache,
+                                const rlm_tensor* value_cache, const rlm_tensor* lengths,
+                                int32_t interleaved, double scale, int32_t ring,
+                                const rlm_tensor* out_query, hipStream_t stream);
+
+/*
+ * The block router by itself: for each query the top_blocks best complete
+ * blocks (strict: complete blocks wholly before the local window), with the
+ * scores and the tie rule of rlm_relation_select_packed: score descending, ties
+ * to the lowest block.
+ *   router_query [B,Tq,S,RD], block_mean/std [B,NB,H,HD] f32 (H*HD == RD <= 1024,
+ *   HD a multiple of 4), gamma [H], bias [H,RB] (H*RB <= 2048), top_blocks in
+ *   [1, 64].  ring: slot j holds the newest block of index j mod NB (NB and
+ *   block_size powers of two); blocks stay absolute.
+ * Outputs: out_blocks int32 [B,Tq,S,TOP], out_scores f32 [B,Tq,S,TOP]; -1 and
+ * -inf where a query has fewer blocks to pick from.  A block whose score is NaN
+ * or at most -1e30 is not picked.
+ */
+hipError_t rlm_block_route(const rlm_tensor* router_query, const rlm_tensor* block_mean,
+                           const rlm_tensor* block_std, const rlm_tensor* gamma,
+                           const rlm_tensor* bias, const rlm_tensor* positions,
+                           int64_t block_size, int64_t local_window, int64_t top_blocks,
+                           int32_t strict_valid, int32_t ring, const rlm_tensor* out_blocks,
+                           const rlm_tensor* out_scores, hipStream_t stream);
+
+/*
+ * Attention of query [B,Tq,Hq,D] over its local window [t - local_window + 1, t]
+ * and, before the window, the blocks picked for it (blocks int32 [B,Tq,TOP], or
+ * [B,Tq,Hk,TOP] with picks per key head; TOP <= 64), as far as the caches
+ * key_cache / value_cache [B,T,Hk,D] hold them:
+ *   out = softmax(scale * q . k) v,  lse = log sum exp(scale * q . k).
+ * Hq a multiple of Hk (query head h reads key head h / (Hq / Hk)); D a multiple
+ * of 8 up to 256; 16-byte aligned, strides multiples of 8 elements.  A position
+ * counts once however often it is named; picks outside the cache (-1) name
+ * nothing.  A query that sees no position gives 0 and lse -inf; what the caches
+ * hold in rows that a query does not see does not reach it.
+ * ring: position p in row p mod T, positions (t - T, t] held; T a power of two
+ * and a multiple of block_size.
+ * Outputs: out [B,Tq,Hq,D] in query's dtype, out_lse f32 [B,Tq,Hq].
+ */
+hipError_t rlm_routed_attention(const rlm_tensor* query, const rlm_tensor* key_cache,
+                                const rlm_tensor* value_cache, const rlm_tensor* blocks,
+                                const rlm_tensor* positions, int64_t block_size,
+                                int64_t local_window, double scale, int32_t ring,
+                                const rlm_tensor* out, const rlm_tensor* out_lse,
+                                hipStream_t stream);
+
+/*
+ * What stands between two blocks of a stack, in one pass:
+ *   out_hidden     = residual_scale * residual + sigmoid(gate) * post(branch)
+ *   out_normalized = norm(out_hidden before its rounding)
+ * with norm(x) = (x - mean) / sqrt(var + norm_eps) * norm_weight + norm_bias, or,
+ * where `rms`, x / sqrt(mean x^2 + norm_eps) * norm_weight + norm_bias; post the
+ * same with post_weight / post_bias / post_eps, or nothing where post_weight is
+ * NULL.  branch, residual [N,D] (row-strided), D <= 8192; gate 0-d, [D] or [N,D];
+ * biases may be NULL; the vectors [D] of any float dtype.
+ */
+hipError_t rlm_gated_residual_norm(const rlm_tensor* branch, const rlm_tensor* residual,
+                                   const rlm_tensor* gate, const rlm_tensor* norm_weight,
+                                   const rlm_tensor* norm_bias, double norm_eps,
+                                   const rlm_tensor* post_weight, const rlm_tensor* post_bias,
+                                   double post_eps, double residual_scale, int32_t rms,
+                                   const rlm_tensor* out_hidden,
+                                   const rlm_tensor* out_normalized, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -511,9 +512,20 @@ inline int64_t dtype_size(int d) { return (d == RLM_F32 || d == RLM_I32) ? 4 : (
 
 // Checks that `t` is a non-null, contiguous tensor of the given rank.
 bool check_tensor(const rlm_tensor* t, const char* name, int ndim);
+// check_tensor that takes a tensor without elements whatever its strides.
+bool check_dense(const rlm_tensor* t, const char* name, int ndim);
 // Checks that `t` is a non-null 2-d tensor of unit column stride whose row
 // stride is at least its width (row-strided views such as cache[:, t]).
 bool check_rows(const rlm_tensor* t, const char* name);
+// Checks that `t` is a non-null tensor of the given rank and of unit stride in its last
+// dim; the other strides are as they come (0 for a broadcast input).
+bool check_strided(const rlm_tensor* t, const char* name, int ndim);
+// Checks that no two elements of a strided tensor share memory (tensors that are written).
+bool check_no_overlap(const rlm_tensor* t, const char* name);
+// Checks the queries' positions: 0-d (one for all), contiguous [Tq] (shared by the batch) or
+// [B,Tq]; gives their strides.
+bool check_positions(const rlm_tensor* t, const char* name, int64_t B, int64_t Tq,
+                     int64_t* stride_b, int64_t* stride_q);
 // Checks t->shape[dim] == value.
 bool check_dim(const rlm_tensor* t, const char* name, int dim, int64_t value);
 bool check_dtype_float(const rlm_tensor* t, const char* name);

@@ -60,6 +60,16 @@ bool check_tensor(const rlm_tensor* t, const char* name, int ndim) {
   return true;
 }
 
+bool check_dense(const rlm_tensor* t, const char* name, int ndim) {
+  bool empty = false;
+  if (t != nullptr && t->ndim == ndim)
+    for (int i = 0; i < ndim; ++i) {
+      if (t->shape[i] < 0) return check_tensor(t, name, ndim);
+      empty = empty || t->shape[i] == 0;
+    }
+  return empty || check_tensor(t, name, ndim);
+}
+
 bool check_rows(const rlm_tensor* t, const char* name) {
   if (t == nullptr) {
     set_error("%s: missing tensor", name);
@@ -87,6 +97,78 @@ bool check_rows(const rlm_tensor* t, const char* name) {
     return false;
   }
   return true;
+}
+
+bool check_strided(const rlm_tensor* t, const char* name, int ndim) {
+  if (t == nullptr) {
+    set_error("%s: missing tensor", name);
+    return false;
+  }
+  if (t->ndim != ndim) {
+    set_error("%s: expected a %d-d tensor, got %d-d", name, ndim, t->ndim);
+    return false;
+  }
+  int64_t numel = 1;
+  for (int i = 0; i < ndim; ++i) {
+    if (t->shape[i] < 0) {
+      set_error("%s: negative size in dim %d", name, i);
+      return false;
+    }
+    if (t->stride[i] < 0) {
+      set_error("%s: negative stride in dim %d", name, i);
+      return false;
+    }
+    numel *= t->shape[i];
+  }
+  if (numel > 0 && t->data == nullptr) {
+    set_error("%s: null data pointer", name);
+    return false;
+  }
+  if (t->shape[ndim - 1] > 1 && t->stride[ndim - 1] != 1) {
+    set_error("%s: the last dim must be unit-stride (got stride %lld)", name,
+              (long long)t->stride[ndim - 1]);
+    return false;
+  }
+  return true;
+}
+
+bool check_no_overlap(const rlm_tensor* t, const char* name) {
+  // Dims by rising stride: each must step over everything that the smaller ones span.
+  bool used[RLM_MAX_DIMS] = {};
+  int64_t span = 1;
+  for (int n = 0; n < t->ndim; ++n) {
+    int best = -1;
+    for (int i = 0; i < t->ndim; ++i)
+      if (!used[i] && (best < 0 || t->stride[i] < t->stride[best])) best = i;
+    used[best] = true;
+    if (t->shape[best] <= 1) continue;
+    if (t->stride[best] < span) {
+      set_error("%s: rows overlap in memory (dim %d has stride %lld)", name, best,
+                (long long)t->stride[best]);
+      return false;
+    }
+    span = t->stride[best] * (t->shape[best] - 1) + span;
+  }
+  return true;
+}
+
+bool check_positions(const rlm_tensor* t, const char* name, int64_t B, int64_t Tq,
+                     int64_t* stride_b, int64_t* stride_q) {
+  if (t == nullptr || !is_index_dtype(t->dtype)) {
+    set_error("%s: expected an int32/int64 tensor", name);
+    return false;
+  }
+  if (t->ndim == 0) {
+    *stride_b = *stride_q = 0;
+    return check_dense(t, name, 0);
+  }
+  *stride_q = 1;
+  if (t->ndim == 1) {
+    *stride_b = 0;
+    return check_dense(t, name, 1) && check_dim(t, name, 0, Tq);
+  }
+  *stride_b = Tq;
+  return check_dense(t, name, 2) && check_dim(t, name, 0, B) && check_dim(t, name, 1, Tq);
 }
 
 bool check_dim(const rlm_tensor* t, const char* name, int dim, int64_t value) {

@@ -1,7 +1,7 @@
 """Loads the HIP operator library and registers fake (meta) kernels.
 
-Importing this module makes ``torch.ops.relation_lm.*`` and
-``torch.ops.relationlex.*`` available.  There is no fallback: when the built
+Importing this module makes ``torch.ops.relation_lm.*``,
+``torch.ops.relationlex.*`` and ``torch.ops.rlm.*`` available.  There is no fallback: when the built
 library is missing the import fails with instructions to build it, and calling
 an op with CPU tensors raises (only the ROCm-device implementation exists) --
 except ``packed_sparse_cache_projection``, whose CPU tensors take ``at::linear``
@@ -202,6 +202,34 @@ def _register_fakes() -> None:
         shape = (keys.shape[0], keys.shape[1] // block_size, keys.shape[2])
         return (keys.new_empty(shape, dtype=torch.float32),
                 keys.new_empty(shape, dtype=torch.float32))
+
+    @torch.library.register_fake("rlm::rotary_positions")
+    def _(query, key, *rest, **options):
+        return query.new_empty(query.shape), key.new_empty(key.shape)
+
+    @torch.library.register_fake("rlm::rotary_to_caches")
+    def _(query, *rest, **options):
+        return query.new_empty(query.shape)
+
+    def fake_route(router_query, block_mean, block_std, gamma, bias, position, block_size,
+                   local_window, top_blocks, strict_valid, ring=False):
+        shape = tuple(router_query.shape[:-1]) + (top_blocks,)
+        return (router_query.new_empty(shape, dtype=torch.int32),
+                router_query.new_empty(shape, dtype=torch.float32))
+
+    torch.library.register_fake("rlm::block_route")(fake_route)
+    torch.library.register_fake("rlm::block_route_seq")(fake_route)
+
+    def fake_attention(query, *rest, **options):
+        return (query.new_empty(query.shape),
+                query.new_empty(query.shape[:-1], dtype=torch.float32))
+
+    torch.library.register_fake("rlm::routed_attention")(fake_attention)
+    torch.library.register_fake("rlm::routed_attention_seq")(fake_attention)
+
+    @torch.library.register_fake("rlm::gated_residual_norm")
+    def _(branch, *rest, **options):
+        return branch.new_empty(branch.shape), branch.new_empty(branch.shape)
 
 
 load()
