@@ -5,45 +5,12 @@
 // that the cache holds (linear: p < T; ring: p > t - T, position p in row p mod T):
 //   out = sum_p softmax_p(scale q . k_p) v_p,   lse = log sum_p exp(scale q . k_p).
 // A position counts once whichever way it is named; a query that sees none gives 0 and -inf.
-#include "rlm_common.hpp"
-#include "rlm_fastdiv.hpp"
+#include "rlm_attention.hpp"
 
 namespace rlm {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-constexpr int kMaxTop = 64;
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.69314718055994530942f;
-
-struct AttentionParams {
-  const void *q, *k, *v;   // [B,Tq,Hq,D], [B,T,Hk,D] twice; unit stride in D
-  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
-  const int32_t* blocks;   // [B,Tq,(Hk),TOP]
-  int64_t blk_sb, blk_st, blk_sh;
-  const void* pos;
-  int pos_dtype;
-  int64_t pos_sb, pos_sq;
-  void* out;               // [B,Tq,Hq,D]
-  float* lse;              // [B,Tq,Hq]
-  int64_t T, BS, local_window;
-  float scale_log2;        // scale * log2(e): scores are kept in powers of two
-  int B, Tq, Hq, Hk, G, D, TOP;
-  int head_chunks;         // of at most 16 query heads
-  int waves_per_item;
-  uint32_t items;          // B * Tq * Hk * head_chunks
-  FastDiv by_chunks, by_kv, by_queries, by_block_tiles;
-  bool ring;
-};
-
-__device__ __forceinline__ float rows_max(float v) {
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float rows_sum(float v) { return swap32_sum(swap16_sum(v)); }
+using namespace attention;
 
 // ---------------------------------------------------------------------------
 // Up to 16 heads of one query to a wave, fp32 products
@@ -57,7 +24,7 @@ __device__ __forceinline__ float rows_sum(float v) { return swap32_sum(swap16_su
 // (one wide load).  One query's heads share its keys, so a masked key is masked for the whole
 // wave; a lane of a masked key reads a key of the same run that is not.
 template <typename T, int DT>
-__global__ __launch_bounds__(512) void attend_query_kernel(AttentionParams p) {
+__global__ __launch_bounds__(512) void attend_query_kernel(Params p) {
   extern __shared__ __align__(16) float merge[];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int r = lane & 15, quad = lane >> 4;
@@ -210,7 +177,7 @@ __global__ __launch_bounds__(512) void attend_query_kernel(AttentionParams p) {
 }
 
 template <typename T, int DT>
-hipError_t launch_query(AttentionParams& p, hipStream_t stream) {
+hipError_t launch_query(Params& p, hipStream_t stream) {
   // Waves of an item: one where the items alone fill the chip.
   const int64_t seen = p.local_window + static_cast<int64_t>(p.TOP) * p.BS;
   const int64_t tiles = (seen + 15) / 16;
@@ -225,7 +192,7 @@ hipError_t launch_query(AttentionParams& p, hipStream_t stream) {
 }
 
 template <typename T>
-hipError_t launch_type(AttentionParams& p, hipStream_t stream) {
+hipError_t launch_type(Params& p, hipStream_t stream) {
   if (p.D <= 32) return launch_query<T, 2>(p, stream);
   if (p.D <= 64) return launch_query<T, 4>(p, stream);
   if (p.D <= 96) return launch_query<T, 6>(p, stream);
@@ -283,7 +250,7 @@ extern "C" hipError_t rlm_routed_attention(
   if (blocks->ndim == 4) RLM_TRY(check_dim(blocks, "blocks", 2, Hk));
   const int64_t TOP = blocks->shape[blocks->ndim - 1];
   RLM_REQUIRE(TOP <= kMaxTop, "blocks: at most %d picks, got %lld", kMaxTop, (long long)TOP);
-  AttentionParams p{};
+  Params p{};
   RLM_TRY(check_positions(positions, "positions", B, Tq, &p.pos_sb, &p.pos_sq));
   RLM_TRY(check_dense(out, "out", 4));
   RLM_TRY(check_same_dtype(out, "out", query, "query"));
@@ -333,6 +300,7 @@ extern "C" hipError_t rlm_routed_attention(
   p.by_kv = FastDiv(static_cast<uint32_t>(Hk));
   p.by_queries = FastDiv(static_cast<uint32_t>(Tq));
   p.by_block_tiles = FastDiv(static_cast<uint32_t>((block_size + 15) / 16));
+  if (tile_fits(p, query->dtype)) return tile_launch(p, query->dtype, stream);
   switch (query->dtype) {
     case RLM_F32: return launch_type<float>(p, stream);
     case RLM_BF16: return launch_type<bf16>(p, stream);

@@ -1,0 +1,536 @@
+// Attention over a window and picked blocks for many queries of 16-bit types: key tiles shared
+// by the rows of a workgroup.
+//
+// A workgroup holds 4 waves of RG x 16 rows, a row being one query head of one query; the rows
+// of a wave are whole queries with the heads of one key head, consecutive positions of the
+// sequence.  It walks the 64-key tiles that any of its queries sees -- its windows' and its
+// picked blocks' union, found from the picks in LDS -- and every wave takes part in those that
+// its own queries see.  Neighbouring queries share their windows and much of their picks, so a
+// tile is read once for all of them; a query's own picks decide only which of its scores count.
+//
+// Tiles come by DMA (buffer_load ... lds), the next one in flight while one is worked on.  With
+// keys as rows and query rows as columns of v_mfma_f32_16x16x32:
+//   S^T[key, row]: lane (row = l % 16, keys 16 kt + 4 (l / 16) + i) -- scores of one row, so
+//     the softmax needs two lane exchanges for its maximum and none for its weights;
+//   O^T[dim, row] += V^T P^T over 32 keys whose order is free: a lane's eight weights of two
+//     16-key groups are its operand as they stand, and V^T's operand is two transposing reads
+//     (ds_read_b64_tr_b16) of four keys each from the row-major tile.
+// LDS rows are swizzled in 16-byte pieces, so that both reads spread over all banks.
+//
+// The weights are rounded to the 16-bit type for the second product (half a step, relative to
+// each weight); scores, maxima, sums and outputs stay fp32.
+//
+// A masked key's weight is 0, which is no protection from what its value row holds if that is
+// an infinity or NaN (0 x inf): a row whose sums are not finite at the end is computed again,
+// position by position, from the rows that it sees alone.
+#include "rlm_attention.hpp"
+
+namespace rlm {
+namespace {
+
+using namespace attention;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kKeys = 64;           // keys of a tile
+constexpr int kWindowTiles = 256;   // tiles (and blocks) looked at at once
+// A wave's running maximum is raised only when a row's scores pass it by this many powers of
+// two (fp16 weights then reach 2^6, far inside the type): the outputs' rescaling is rare.
+constexpr float kSlack = 6.0f;
+
+struct TileParams {
+  Params p;
+  int hg;                // heads of a wave's query (a chunk of the group)
+  int chunks;            // chunks of a group
+  int nqw;               // queries of a wave
+  uint32_t pairs;        // (batch row, key head, chunk)
+  uint32_t tiles;        // workgroups along the sequence
+  FastDiv by_pairs, by_chunks, by_kv, by_heads, by_block;
+  float c;               // |scale| log2(e), above 0
+  bool negate;
+};
+
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, f16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bf16) { return pack_bf16x2(lo, hi); }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, f16) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  const f32x2_t v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+}
+
+// 16-byte pieces of an LDS row: rows of 8 pieces alternate between the halves of the 16 piece
+// columns that the banks form, so their swizzle goes by pairs of rows.
+template <int PITCH>
+__device__ __forceinline__ int swizzle(int row) {
+  return PITCH == 8 ? (row >> 1) & 7 : row & 15;
+}
+
+// One row from the positions that it sees alone, a position at a time: lanes hold features.
+template <typename T>
+__device__ void attend_row_alone(const Params& p, int64_t b, int64_t step, int64_t hk, int64_t head,
+                                 float scale_log2) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const T* q = static_cast<const T*>(p.q) + b * p.q_sb + step * p.q_st + head * p.q_sh;
+  const T* kbase = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vbase = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  const int32_t* picks = p.blocks + b * p.blk_sb + step * p.blk_st + hk * p.blk_sh;
+  const int32_t mine = lane < p.TOP ? picks[lane] : -1;
+  const int64_t t = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_sq);
+  const int64_t high = t + 1 < p.T ? t + 1 : p.T;
+  int64_t start = t - p.local_window + 1;
+  start = start > 0 ? start : 0;
+  float qf[4], acc[4] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d = lane + kWave * i;
+    qf[i] = d < p.D ? to_f32(q[d]) : 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+  for (int run = -1; run < p.TOP; ++run) {
+    int64_t first = start, end = high;
+    if (run >= 0) {
+      const int32_t block = __builtin_amdgcn_readlane(mine, run);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(mine == block);
+      if (block < 0 || (same & ((uint64_t(1) << run) - 1)) != 0) continue;
+      first = block * p.BS;
+      end = first + p.BS < start ? first + p.BS : start;
+      end = end < high ? end : high;
+    }
+    for (int64_t at = first; at < end; ++at) {
+      float s = 0.0f, v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = lane + kWave * i;
+        v[i] = d < p.D ? to_f32(vbase[at * p.v_st + d]) : 0.0f;
+        if (d < p.D) s = fmaf(qf[i], to_f32(kbase[at * p.k_st + d]), s);
+      }
+      s = wave_sum_f32(s) * scale_log2;
+      const float top = fmaxf(m, s), base = top == -INFINITY ? 0.0f : top;
+      const float fade = __builtin_amdgcn_exp2f(m - base);
+      const float w = __builtin_amdgcn_exp2f(s - base);
+      m = top;
+      l = fmaf(l, fade, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(acc[i], fade, w * v[i]);
+    }
+  }
+  const int64_t row = (b * p.Tq + step) * p.Hq + head;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = static_cast<T*>(p.out) + row * p.D;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d = lane + kWave * i;
+    if (d < p.D) out[d] = from_f32<T>(acc[i] * inv);
+  }
+  if (lane == 0)
+    p.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// DC: head dim in 32s, RG: row groups of a wave.
+template <typename T, int DC, int RG>
+__global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(TileParams tp) {
+  constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;  // 16-byte pieces of an LDS row
+  constexpr int kRow = 16 * kPitch;                        // bytes
+  constexpr int kTile = kKeys * kRow;                      // bytes of a key (or value) tile
+  constexpr int kDma = kPitch * kKeys / kThreads;          // DMA instructions of a wave per tile
+  constexpr int DT = 2 * DC;                               // head dim in 16s
+  extern __shared__ __align__(16) char lds[];              // [2][key tile, value tile]
+  __shared__ uint32_t sel[(kWindowTiles + 2) * kWaves];    // [block][wave]: its queries' picks
+  __shared__ __align__(16) uint32_t act[kWindowTiles * kWaves];          // [tile][wave]: its queries that see it
+  __shared__ int32_t s_high[kWaves * 32], s_start[kWaves * 32];
+  __shared__ uint16_t list[kWindowTiles];
+  __shared__ int32_t s_count, s_last;
+
+  const Params& p = tp.p;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 15, quad = lane >> 4;
+  // The longest sequences' ends first; a (batch row, key head)'s workgroups stay on one XCD
+  // (or a few) where their number and the XCDs' divide each other.
+  uint32_t pair, chunk, hk;
+  const uint32_t tile = tp.tiles - 1 - tp.by_pairs.div(blockIdx.x, pair);
+  const int64_t b = tp.by_kv.div(tp.by_chunks.div(pair, chunk), hk);
+  const int queries = kWaves * tp.nqw;
+  const int q0 = static_cast<int>(tile) * queries;
+
+  const T* kbase = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vbase = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+
+  // Positions: query i of the workgroup sees [.., high) and its window starts at `start`.
+  if (threadIdx.x == 0) s_last = 0;
+  __syncthreads();
+  if (threadIdx.x < queries) {
+    const int q = q0 + threadIdx.x;
+    int32_t high = 0, start = 0;
+    if (q < p.Tq) {
+      const int64_t t = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + q * p.pos_sq);
+      int64_t s = t - p.local_window + 1;
+      s = s > 0 ? s : 0;
+      high = static_cast<int32_t>(t < 0 ? 0 : t + 1 < p.T ? t + 1 : p.T);
+      start = static_cast<int32_t>(s < high ? s : high);
+    }
+    s_high[threadIdx.x] = high;
+    s_start[threadIdx.x] = start;
+    atomicMax(&s_last, high);
+  }
+
+  // This lane's rows.
+  int32_t high[RG], start[RG];
+  int bit[RG];
+  s16x8 qf[RG][DC];
+  bool row_ok[RG];
+  int head[RG], step[RG];
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    uint32_t in_query;
+    const uint32_t mine = tp.by_heads.div(16 * g + r, in_query);
+    const int q = q0 + wave * tp.nqw + static_cast<int>(mine);
+    const int h = static_cast<int>(chunk) * tp.hg + static_cast<int>(in_query);
+    row_ok[g] = mine < static_cast<uint32_t>(tp.nqw) && q < p.Tq && h < p.G;
+    head[g] = static_cast<int>(hk) * p.G + (row_ok[g] ? h : 0);
+    step[g] = row_ok[g] ? q : 0;
+    bit[g] = row_ok[g] ? static_cast<int>(mine) : 0;
+    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + step[g] * p.q_st + head[g] * p.q_sh;
+#pragma unroll
+    for (int j = 0; j < DC; ++j) {
+      const int d = 32 * j + 8 * quad;
+      uint4 x = *reinterpret_cast<const uint4*>(src + (d < p.D ? d : 0));
+      const uint32_t flip = tp.negate ? 0x80008000u : 0u;
+      x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+      if (!(d < p.D && row_ok[g])) x = make_uint4(0, 0, 0, 0);
+      qf[g][j] = __builtin_bit_cast(s16x8, x);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    high[g] = row_ok[g] ? s_high[wave * tp.nqw + bit[g]] : 0;
+    start[g] = row_ok[g] ? s_start[wave * tp.nqw + bit[g]] : 0;
+  }
+  const int32_t last = __builtin_amdgcn_readfirstlane(s_last);
+
+  f32x4 acc[RG][DT];
+  float m[RG], l[RG];
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < DT; ++j) acc[g][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // This lane's pieces of a tile: row and byte in the row, which the swizzle permutes.
+  int dma_row[kDma];
+  uint32_t dma_byte[kDma];
+#pragma unroll
+  for (int k = 0; k < kDma; ++k) {
+    const int piece = (wave * kDma + k) * kWave + lane;
+    dma_row[k] = piece / kPitch;
+    const int from = (piece % kPitch) ^ swizzle<kPitch>(dma_row[k]);
+    dma_byte[k] = 8 * from < p.D ? 16u * from : kNoOffset;
+  }
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const uint32_t k_bytes = static_cast<uint32_t>(p.k_st) * 2u;
+  const uint32_t v_bytes = static_cast<uint32_t>(p.v_st) * 2u;
+  auto issue = [&](int buffer, int64_t first) {
+    // Rows past the last that a query of the workgroup sees (their keys are masked, and they may
+    // hold anything) read that one.
+    const int rows = min(last - 1 - static_cast<int>(first), kKeys - 1);
+    const rsrc_t kr = make_rsrc(kbase + first * p.k_st, 0x7ffffff0u);
+    const rsrc_t vr = make_rsrc(vbase + first * p.v_st, 0x7ffffff0u);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kTile + wave * kDma * 1024);
+#pragma unroll
+    for (int k = 0; k < kDma; ++k) {
+      const uint32_t row = min(dma_row[k], rows);
+      lds_dma16(kr, to + 1024u * k, dma_byte[k] == kNoOffset ? kNoOffset : row * k_bytes + dma_byte[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kDma; ++k) {
+      const uint32_t row = min(dma_row[k], rows);
+      lds_dma16(vr, to + kTile + 1024u * k,
+                dma_byte[k] == kNoOffset ? kNoOffset : row * v_bytes + dma_byte[k]);
+    }
+  };
+
+  // Windows of the cache: as many keys as kWindowTiles tiles or blocks hold.
+  const int32_t span = kKeys * static_cast<int32_t>(
+      min(static_cast<int64_t>(kWindowTiles), max(static_cast<int64_t>(1), kWindowTiles * p.BS / kKeys)));
+  for (int32_t w0 = 0; w0 < last; w0 += span) {
+    const int32_t w1 = min(w0 + span, last);
+    const int32_t block0 = static_cast<int32_t>(tp.by_block.div(w0));
+    const int window_tiles = (w1 - w0 + kKeys - 1) / kKeys;
+    // What the queries see in this window.
+    for (int i = threadIdx.x; i < (kWindowTiles + 2) * kWaves; i += kThreads) sel[i] = 0;
+    for (int i = threadIdx.x; i < window_tiles * kWaves; i += kThreads) act[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < queries * (p.TOP + 1); i += kThreads) {
+      const int q = i / (p.TOP + 1), k = i % (p.TOP + 1) - 1;
+      if (q0 + q >= p.Tq) continue;
+      const int w = q / tp.nqw;
+      const uint32_t mine = 1u << (q - w * tp.nqw);
+      int32_t first = s_start[q], end = s_high[q];
+      if (k >= 0) {
+        const int32_t block =
+            p.blocks[b * p.blk_sb + static_cast<int64_t>(q0 + q) * p.blk_st + hk * p.blk_sh + k];
+        const int64_t at = static_cast<int64_t>(block) * p.BS;
+        if (block < 0 || at >= min(s_start[q], w1) || at + p.BS <= w0) continue;
+        atomicOr(&sel[(block - block0) * kWaves + w], mine);
+        first = static_cast<int32_t>(at);
+        end = static_cast<int32_t>(min(at + p.BS, static_cast<int64_t>(s_start[q])));
+      }
+      first = max(first, w0);
+      end = min(end, w1);
+      for (int32_t t = (first - w0) / kKeys; w0 + t * kKeys < end; ++t)
+        if (first < end) atomicOr(&act[t * kWaves + w], mine);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      int count = 0;
+      for (int i = 0; i < window_tiles; i += kWave) {
+        const int t = i + lane;
+        bool any = false;
+        if (t < window_tiles) {
+          const uint4 a = *reinterpret_cast<const uint4*>(&act[t * kWaves]);
+          any = (a.x | a.y | a.z | a.w) != 0;
+        }
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(any);
+        if (any) list[count + __builtin_popcountll(mask & ((uint64_t(1) << lane) - 1))] = t;
+        count += __builtin_popcountll(mask);
+      }
+      if (lane == 0) s_count = count;
+    }
+    __syncthreads();
+    const int count = __builtin_amdgcn_readfirstlane(s_count);
+    if (count == 0) continue;
+    issue(0, w0 + kKeys * __builtin_amdgcn_readfirstlane(list[0]));
+    for (int n = 0; n < count; ++n) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      __syncthreads();  // tile n is in LDS, tile n - 1 has been read
+      if (n + 1 < count)
+        issue((n + 1) & 1, w0 + kKeys * __builtin_amdgcn_readfirstlane(list[n + 1]));
+      const int t = __builtin_amdgcn_readfirstlane(list[n]);
+      const uint32_t see = __builtin_amdgcn_readfirstlane(act[t * kWaves + wave]);
+      if (see == 0) continue;
+      const int32_t p0 = w0 + t * kKeys;
+      const char* ktile = lds + (n & 1) * 2 * kTile;
+      const char* vtile = ktile + kTile;
+
+      // Row groups with a row that sees the tile, and those whose rows see all of it.
+      bool use[RG], whole[RG];
+      uint32_t picked[4];  // by 16-key group: the wave's queries that picked its block
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+        picked[kt] = sel[(tp.by_block.div(p0 + 16 * kt + 4 * quad) - block0) * kWaves + wave];
+#pragma unroll
+      for (int g = 0; g < RG; ++g) {
+        const bool mine = row_ok[g] && ((see >> bit[g]) & 1) != 0;
+        use[g] = __builtin_amdgcn_ballot_w64(mine) != 0;
+        bool all = mine && p0 + kKeys <= high[g];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+          all = all && (((picked[kt] >> bit[g]) & 1) != 0 || p0 + 16 * kt + 4 * quad >= start[g]);
+        whole[g] = __builtin_amdgcn_ballot_w64(!all && row_ok[g]) == 0;
+      }
+
+      // S^T = K Q^T.
+      f32x4 s[RG][4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        s16x8 kf[DC];
+#pragma unroll
+        for (int j = 0; j < DC; ++j) {
+          const int row = 16 * kt + r;
+          kf[j] = *reinterpret_cast<const s16x8*>(
+              ktile + row * kRow + (((4 * j + quad) ^ swizzle<kPitch>(row)) << 4));
+        }
+#pragma unroll
+        for (int g = 0; g < RG; ++g) {
+          if (!use[g]) continue;
+          s[g][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < DC; ++j) s[g][kt] = mfma(kf[j], qf[g][j], s[g][kt], T{});
+        }
+      }
+
+      // The weights, as the second product's operand: two 16-key groups to each.
+      uint4 weights[RG][2];
+#pragma unroll
+      for (int g = 0; g < RG; ++g) {
+        if (!use[g]) continue;
+        if (!whole[g]) {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt) {
+            const int32_t at = p0 + 16 * kt + 4 * quad;
+            const int32_t from = ((picked[kt] >> bit[g]) & 1) != 0 ? 0 : start[g] - at;
+            const int32_t to = high[g] - at;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[g][kt][i] = i >= from && i < to ? s[g][kt][i] : -INFINITY;
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+          top = fmaxf(top, fmaxf(fmaxf(s[g][kt][0], s[g][kt][1]), fmaxf(s[g][kt][2], s[g][kt][3])));
+        top = rows_max(top) * tp.c;
+        if (__builtin_amdgcn_ballot_w64(top > m[g] + kSlack) != 0) {
+          const float raised = fmaxf(m[g], top);
+          const float fade = __builtin_amdgcn_exp2f(m[g] - (raised == -INFINITY ? 0.0f : raised));
+          m[g] = raised;
+          l[g] *= fade;
+#pragma unroll
+          for (int j = 0; j < DT; ++j) acc[g][j] *= fade;
+        }
+        const float base = m[g] == -INFINITY ? 0.0f : m[g];
+        uint32_t word[8];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(fmaf(s[g][kt][i], tp.c, -base));
+            l[g] += w[i];
+          }
+          word[2 * kt] = pack2(w[0], w[1], T{});
+          word[2 * kt + 1] = pack2(w[2], w[3], T{});
+        }
+        weights[g][0] = make_uint4(word[0], word[1], word[2], word[3]);
+        weights[g][1] = make_uint4(word[4], word[5], word[6], word[7]);
+      }
+
+      // O^T += V^T P^T.
+#pragma unroll
+      for (int j = 0; j < DT; ++j) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // Lane l reads four values of key 4 quad + l % 16 / 4 and gets four keys of value
+          // feature l % 16.
+          const int key = 32 * half + 4 * quad + (r >> 2);
+          const int piece = 2 * j + ((r & 3) >> 1), rest = (r & 1) * 8;
+          typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(
+              vtile + key * kRow + ((piece ^ swizzle<kPitch>(key)) << 4) + rest));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(
+              vtile + (key + 16) * kRow + ((piece ^ swizzle<kPitch>(key + 16)) << 4) + rest));
+          const s16x8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+          for (int g = 0; g < RG; ++g)
+            if (use[g])
+              acc[g][j] = mfma(vf, __builtin_bit_cast(s16x8, weights[g][half]), acc[g][j], T{});
+        }
+      }
+    }
+    __syncthreads();  // the lists and tiles have been read
+  }
+
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    const float total = rows_sum(l[g]);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    bool fine = fabsf(total) < INFINITY;
+#pragma unroll
+    for (int j = 0; j < DT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fine = fine && fabsf(acc[g][j][i]) < INFINITY;
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(!fine && row_ok[g]);
+    if (row_ok[g]) {
+      const int64_t row = (b * p.Tq + step[g]) * p.Hq + head[g];
+      T* out = static_cast<T*>(p.out) + row * p.D;
+#pragma unroll
+      for (int j = 0; j < DT; ++j) {
+        const int d = 16 * j + 4 * quad;
+        if (d < p.D)
+          put4<T>(out + d, acc[g][j][0] * inv, acc[g][j][1] * inv, acc[g][j][2] * inv,
+                  acc[g][j][3] * inv);
+      }
+      if (quad == 0)
+        p.lse[row] = total == 0.0f ? -INFINITY : (m[g] + __builtin_amdgcn_logf(total)) * kLn2;
+    }
+    if (bad != 0) {
+      uint32_t rows = static_cast<uint32_t>(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xffffu;
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the stores above, which these replace
+      while (rows != 0) {
+        const int from = __builtin_ctz(rows);
+        rows &= rows - 1;
+        attend_row_alone<T>(p, b, __builtin_amdgcn_readlane(step[g], from), hk,
+                            __builtin_amdgcn_readlane(head[g], from),
+                            tp.negate ? -tp.c : tp.c);
+      }
+    }
+  }
+}
+
+template <typename T, int DC, int RG>
+hipError_t launch(TileParams& tp, hipStream_t stream) {
+  const Params& p = tp.p;
+  // Rows of a wave: whole queries, the heads of one key head each.
+  constexpr int kRows = 16 * RG;
+  tp.chunks = (p.G + kRows - 1) / kRows;
+  tp.hg = (p.G + tp.chunks - 1) / tp.chunks;
+  tp.nqw = kRows / tp.hg;
+  tp.pairs = static_cast<uint32_t>(p.B * p.Hk * tp.chunks);
+  tp.tiles = static_cast<uint32_t>((p.Tq + kWaves * tp.nqw - 1) / (kWaves * tp.nqw));
+  tp.by_pairs = FastDiv(tp.pairs);
+  tp.by_chunks = FastDiv(static_cast<uint32_t>(tp.chunks));
+  tp.by_kv = FastDiv(static_cast<uint32_t>(p.Hk));
+  tp.by_heads = FastDiv(static_cast<uint32_t>(tp.hg));
+  tp.by_block = FastDiv(static_cast<uint32_t>(p.BS));
+  constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;
+  const size_t lds = 4 * kKeys * 16 * kPitch;
+  if (lds > 48 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(
+        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, RG>),
+        hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+    RLM_REQUIRE(e == hipSuccess, "routed_attention: %zu bytes of LDS refused: %s", lds,
+                hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL((attend_tile_kernel<T, DC, RG>), dim3(tp.pairs * tp.tiles), dim3(kThreads),
+                     lds, stream, tp);
+  return launch_status("routed_attention");
+}
+
+template <typename T>
+hipError_t launch_type(TileParams& tp, hipStream_t stream) {
+  const int dc = (tp.p.D + 31) / 32;
+  if (dc <= 1) return launch<T, 1, 2>(tp, stream);
+  if (dc <= 2) return launch<T, 2, 2>(tp, stream);
+  if (dc <= 3) return launch<T, 3, 2>(tp, stream);
+  if (dc <= 4) return launch<T, 4, 2>(tp, stream);
+  return launch<T, 8, 1>(tp, stream);
+}
+
+}  // namespace
+
+namespace attention {
+
+bool tile_fits(const Params& p, int dtype) {
+  const int64_t limit = (int64_t(1) << 31) / (2 * kKeys) - 1;  // bytes of a tile's rows
+  return (dtype == RLM_BF16 || dtype == RLM_F16) && !p.ring && p.Tq > 1 && p.T >= 1 &&
+         p.BS % 4 == 0 && p.k_st < limit && p.v_st < limit &&
+         static_cast<int64_t>(p.B) * p.Hk * ((p.G + 15) / 16) * p.Tq < (int64_t(1) << 31);
+}
+
+hipError_t tile_launch(Params& p, int dtype, hipStream_t stream) {
+  TileParams tp{};
+  tp.p = p;
+  tp.negate = p.scale_log2 < 0.0f;
+  // A scale of 0 as the smallest number: scores of 0 for the keys, -inf for the masked.
+  tp.c = std::max(std::fabs(p.scale_log2), 1e-37f);
+  return dtype == RLM_BF16 ? launch_type<bf16>(tp, stream) : launch_type<f16>(tp, stream);
+}
+
+}  // namespace attention
+}  // namespace rlm
