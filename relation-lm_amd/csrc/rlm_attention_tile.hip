@@ -23,6 +23,8 @@
 // A masked key's weight is 0, which is no protection from what its value row holds if that is
 // an infinity or NaN (0 x inf): a row whose sums are not finite at the end is computed again,
 // position by position, from the rows that it sees alone.
+#include <type_traits>
+
 #include "rlm_attention.hpp"
 
 namespace rlm {
@@ -35,13 +37,16 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+typedef const __attribute__((address_space(3))) s16x8* lds_s16x8;
+
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kKeys = 64;           // keys of a tile
 constexpr int kWindowTiles = 256;   // tiles (and blocks) looked at at once
-// A wave's running maximum is raised only when a row's scores pass it by this many powers of
-// two (fp16 weights then reach 2^6, far inside the type): the outputs' rescaling is rare.
-constexpr float kSlack = 6.0f;
+// Sum of a lane's weights of a row in one tile beyond which its base is raised: fp16 weights stay far
+// inside the type, and the outputs' rescaling is rare.
+constexpr float kLimit = 4096.0f;
 
 struct TileParams {
   Params p;
@@ -139,15 +144,15 @@ __device__ void attend_row_alone(const Params& p, int64_t b, int64_t step, int64
     p.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// DC: head dim in 32s, RG: row groups of a wave.
-template <typename T, int DC, int RG>
-__global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(TileParams tp) {
+// DC: head dim in 32s, RG: row groups of a wave, WHOLE: a tile lies within one block.
+template <typename T, int DC, int RG, bool WHOLE, int MINW = DC <= 2 ? 3 : 2>
+__global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams tp) {
   constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;  // 16-byte pieces of an LDS row
   constexpr int kRow = 16 * kPitch;                        // bytes
   constexpr int kTile = kKeys * kRow;                      // bytes of a key (or value) tile
   constexpr int kDma = kPitch * kKeys / kThreads;          // DMA instructions of a wave per tile
   constexpr int DT = 2 * DC;                               // head dim in 16s
-  extern __shared__ __align__(16) char lds[];              // [2][key tile, value tile]
+  extern __shared__ __align__(1024) char lds[];            // [2][key tile, value tile]
   __shared__ uint32_t sel[(kWindowTiles + 2) * kWaves];    // [block][wave]: its queries' picks
   __shared__ __align__(16) uint32_t act[kWindowTiles * kWaves];          // [tile][wave]: its queries that see it
   __shared__ int32_t s_high[kWaves * 32], s_start[kWaves * 32];
@@ -221,6 +226,14 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(TileParams tp)
     start[g] = row_ok[g] ? s_start[wave * tp.nqw + bit[g]] : 0;
   }
   const int32_t last = __builtin_amdgcn_readfirstlane(s_last);
+  // Tiles that end at `remote` or before lie before every window of the wave's rows: their keys
+  // are seen by the picks alone, whole blocks at a time.
+  int32_t remote = 0x7fffffff;
+#pragma unroll
+  for (int g = 0; g < RG; ++g) remote = high[g] > 0 ? min(remote, start[g]) : remote;
+#pragma unroll
+  for (int off = 1; off < 16; off <<= 1) remote = min(remote, __shfl_xor(remote, off, kWave));
+  remote = __builtin_amdgcn_readfirstlane(remote);
 
   f32x4 acc[RG][DT];
   float m[RG], l[RG];
@@ -232,36 +245,41 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(TileParams tp)
     for (int j = 0; j < DT; ++j) acc[g][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // This lane's pieces of a tile: row and byte in the row, which the swizzle permutes.
-  int dma_row[kDma];
-  uint32_t dma_byte[kDma];
+  // This lane's pieces of a tile: row and byte in the row, which the swizzle permutes; pieces
+  // past the head dim come as zeros.
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const uint32_t k_bytes = static_cast<uint32_t>(p.k_st) * 2u;
+  const uint32_t v_bytes = static_cast<uint32_t>(p.v_st) * 2u;
+  uint32_t dma_row[kDma], k_off[kDma], v_off[kDma];
 #pragma unroll
   for (int k = 0; k < kDma; ++k) {
     const int piece = (wave * kDma + k) * kWave + lane;
     dma_row[k] = piece / kPitch;
     const int from = (piece % kPitch) ^ swizzle<kPitch>(dma_row[k]);
-    dma_byte[k] = 8 * from < p.D ? 16u * from : kNoOffset;
+    const bool ok = 8 * from < p.D;
+    k_off[k] = ok ? dma_row[k] * k_bytes + 16u * from : kNoOffset;
+    v_off[k] = ok ? dma_row[k] * v_bytes + 16u * from : kNoOffset;
   }
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
-  const uint32_t k_bytes = static_cast<uint32_t>(p.k_st) * 2u;
-  const uint32_t v_bytes = static_cast<uint32_t>(p.v_st) * 2u;
-  auto issue = [&](int buffer, int64_t first) {
-    // Rows past the last that a query of the workgroup sees (their keys are masked, and they may
-    // hold anything) read that one.
-    const int rows = min(last - 1 - static_cast<int>(first), kKeys - 1);
+  auto issue = [&](int buffer, int32_t first) {
     const rsrc_t kr = make_rsrc(kbase + first * p.k_st, 0x7ffffff0u);
     const rsrc_t vr = make_rsrc(vbase + first * p.v_st, 0x7ffffff0u);
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kTile + wave * kDma * 1024);
+    // Rows past the last that a query of the workgroup sees (their keys are masked, and they may
+    // hold anything) read that one.
+    const uint32_t rows = static_cast<uint32_t>(last - 1 - first);
+    if (rows >= kKeys - 1) {
 #pragma unroll
-    for (int k = 0; k < kDma; ++k) {
-      const uint32_t row = min(dma_row[k], rows);
-      lds_dma16(kr, to + 1024u * k, dma_byte[k] == kNoOffset ? kNoOffset : row * k_bytes + dma_byte[k]);
-    }
+      for (int k = 0; k < kDma; ++k) lds_dma16(kr, to + 1024u * k, k_off[k]);
 #pragma unroll
-    for (int k = 0; k < kDma; ++k) {
-      const uint32_t row = min(dma_row[k], rows);
-      lds_dma16(vr, to + kTile + 1024u * k,
-                dma_byte[k] == kNoOffset ? kNoOffset : row * v_bytes + dma_byte[k]);
+      for (int k = 0; k < kDma; ++k) lds_dma16(vr, to + kTile + 1024u * k, v_off[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kDma; ++k) {
+        const uint32_t over = dma_row[k] > rows ? dma_row[k] - rows : 0;
+        const uint32_t ko = k_off[k] - over * k_bytes, vo = v_off[k] - over * v_bytes;
+        lds_dma16(kr, to + 1024u * k, k_off[k] == kNoOffset ? kNoOffset : ko);
+        lds_dma16(vr, to + kTile + 1024u * k, v_off[k] == kNoOffset ? kNoOffset : vo);
+      }
     }
   };
 
@@ -287,14 +305,17 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(TileParams tp)
             p.blocks[b * p.blk_sb + static_cast<int64_t>(q0 + q) * p.blk_st + hk * p.blk_sh + k];
         const int64_t at = static_cast<int64_t>(block) * p.BS;
         if (block < 0 || at >= min(s_start[q], w1) || at + p.BS <= w0) continue;
-        atomicOr(&sel[(block - block0) * kWaves + w], mine);
+        if (!WHOLE) atomicOr(&sel[(block - block0) * kWaves + w], mine);
         first = static_cast<int32_t>(at);
         end = static_cast<int32_t>(min(at + p.BS, static_cast<int64_t>(s_start[q])));
       }
       first = max(first, w0);
       end = min(end, w1);
       for (int32_t t = (first - w0) / kKeys; w0 + t * kKeys < end; ++t)
-        if (first < end) atomicOr(&act[t * kWaves + w], mine);
+        if (first < end) {
+          atomicOr(&act[t * kWaves + w], mine);
+          if (WHOLE && k >= 0) atomicOr(&sel[t * kWaves + w], mine);
+        }
     }
     __syncthreads();
     if (wave == 0) {
@@ -315,123 +336,160 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(TileParams tp)
     __syncthreads();
     const int count = __builtin_amdgcn_readfirstlane(s_count);
     if (count == 0) continue;
-    issue(0, w0 + kKeys * __builtin_amdgcn_readfirstlane(list[0]));
+    // Lane i holds the list's entry i of the current 64, and what the wave's queries see of it.
+    int entry = list[min(lane, count - 1)];
+    uint32_t seen = act[entry * kWaves + wave];
+    int next = __builtin_amdgcn_readlane(entry, 0);
+    uint32_t next_see = __builtin_amdgcn_readlane(seen, 0);
+    issue(0, w0 + kKeys * next);
     for (int n = 0; n < count; ++n) {
+      const int t = next;
+      const uint32_t see = next_see;
+      if (n + 1 < count) {
+        if (((n + 1) & (kWave - 1)) == 0) {
+          entry = list[min(n + 1 + lane, count - 1)];
+          seen = act[entry * kWaves + wave];
+        }
+        next = __builtin_amdgcn_readlane(entry, (n + 1) & (kWave - 1));
+        next_see = __builtin_amdgcn_readlane(seen, (n + 1) & (kWave - 1));
+      }
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
       __syncthreads();  // tile n is in LDS, tile n - 1 has been read
-      if (n + 1 < count)
-        issue((n + 1) & 1, w0 + kKeys * __builtin_amdgcn_readfirstlane(list[n + 1]));
-      const int t = __builtin_amdgcn_readfirstlane(list[n]);
-      const uint32_t see = __builtin_amdgcn_readfirstlane(act[t * kWaves + wave]);
+      if (n + 1 < count) issue((n + 1) & 1, w0 + kKeys * next);
       if (see == 0) continue;
       const int32_t p0 = w0 + t * kKeys;
-      const char* ktile = lds + (n & 1) * 2 * kTile;
-      const char* vtile = ktile + kTile;
+      const bool near = p0 + kKeys > remote;
+      // A lane's first piece of the key and of the value rows that it reads; the swizzle makes
+      // later ones an exclusive or away (pieces 4 j + quad of the keys, 2 j + (0 or 1) of the
+      // values).
+      const uint32_t tile0 = lds0 + (n & 1) * 2 * kTile;
+      const uint32_t key0 = tile0 + r * kRow + ((quad ^ swizzle<kPitch>(r)) << 4);
+      const int vrow = 4 * quad + (r >> 2);
+      const uint32_t value0 = tile0 + kTile + vrow * kRow +
+                              ((((r & 3) >> 1) ^ swizzle<kPitch>(vrow)) << 4) + (r & 1) * 8;
+      // The wave's queries that picked the block of a lane's four keys of 16-key group kt.
+      constexpr int kPicked = WHOLE ? 1 : 4;
+      uint32_t picked[kPicked];
+#pragma unroll
+      for (int kt = 0; kt < kPicked; ++kt)
+        picked[kt] = WHOLE ? sel[t * kWaves + wave]
+                           : sel[(tp.by_block.div(p0 + 16 * kt + 4 * quad) - block0) * kWaves + wave];
+      uint32_t groups = 0;
+#pragma unroll
+      for (int g = 0; g < RG; ++g)
+        if (__builtin_amdgcn_ballot_w64(row_ok[g] & (((see >> bit[g]) & 1) != 0)) != 0)
+          groups |= 1u << g;
+      groups = __builtin_amdgcn_readfirstlane(groups);
 
-      // Row groups with a row that sees the tile, and those whose rows see all of it.
-      bool use[RG], whole[RG];
-      uint32_t picked[4];  // by 16-key group: the wave's queries that picked its block
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-        picked[kt] = sel[(tp.by_block.div(p0 + 16 * kt + 4 * quad) - block0) * kWaves + wave];
-#pragma unroll
-      for (int g = 0; g < RG; ++g) {
-        const bool mine = row_ok[g] && ((see >> bit[g]) & 1) != 0;
-        use[g] = __builtin_amdgcn_ballot_w64(mine) != 0;
-        bool all = mine && p0 + kKeys <= high[g];
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-          all = all && (((picked[kt] >> bit[g]) & 1) != 0 || p0 + 16 * kt + 4 * quad >= start[g]);
-        whole[g] = __builtin_amdgcn_ballot_w64(!all && row_ok[g]) == 0;
-      }
-
-      // S^T = K Q^T.
-      f32x4 s[RG][4];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        s16x8 kf[DC];
-#pragma unroll
-        for (int j = 0; j < DC; ++j) {
-          const int row = 16 * kt + r;
-          kf[j] = *reinterpret_cast<const s16x8*>(
-              ktile + row * kRow + (((4 * j + quad) ^ swizzle<kPitch>(row)) << 4));
-        }
-#pragma unroll
-        for (int g = 0; g < RG; ++g) {
-          if (!use[g]) continue;
-          s[g][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int j = 0; j < DC; ++j) s[g][kt] = mfma(kf[j], qf[g][j], s[g][kt], T{});
-        }
-      }
-
-      // The weights, as the second product's operand: two 16-key groups to each.
-      uint4 weights[RG][2];
-#pragma unroll
-      for (int g = 0; g < RG; ++g) {
-        if (!use[g]) continue;
-        if (!whole[g]) {
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt) {
-            const int32_t at = p0 + 16 * kt + 4 * quad;
-            const int32_t from = ((picked[kt] >> bit[g]) & 1) != 0 ? 0 : start[g] - at;
-            const int32_t to = high[g] - at;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              s[g][kt][i] = i >= from && i < to ? s[g][kt][i] : -INFINITY;
-          }
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-          top = fmaxf(top, fmaxf(fmaxf(s[g][kt][0], s[g][kt][1]), fmaxf(s[g][kt][2], s[g][kt][3])));
-        top = rows_max(top) * tp.c;
-        if (__builtin_amdgcn_ballot_w64(top > m[g] + kSlack) != 0) {
-          const float raised = fmaxf(m[g], top);
-          const float fade = __builtin_amdgcn_exp2f(m[g] - (raised == -INFINITY ? 0.0f : raised));
-          m[g] = raised;
-          l[g] *= fade;
-#pragma unroll
-          for (int j = 0; j < DT; ++j) acc[g][j] *= fade;
-        }
-        const float base = m[g] == -INFINITY ? 0.0f : m[g];
-        uint32_t word[8];
+      // The tile for the row groups of MASK.
+      auto work = [&](auto mask) {
+        constexpr int MASK = decltype(mask)::value;
+        // S^T = K Q^T.
+        f32x4 s[RG][4];
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-          float w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(fmaf(s[g][kt][i], tp.c, -base));
-            l[g] += w[i];
+          for (int j = 0; j < DC; ++j) {
+            const s16x8 kf = *(lds_s16x8)((key0 ^ (64u * j)) + 16 * kt * kRow);
+#pragma unroll
+            for (int g = 0; g < RG; ++g) {
+              if (!(MASK >> g & 1)) continue;
+              if (j == 0) s[g][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+              s[g][kt] = mfma(kf, qf[g][j], s[g][kt], T{});
+            }
           }
-          word[2 * kt] = pack2(w[0], w[1], T{});
-          word[2 * kt + 1] = pack2(w[2], w[3], T{});
         }
-        weights[g][0] = make_uint4(word[0], word[1], word[2], word[3]);
-        weights[g][1] = make_uint4(word[4], word[5], word[6], word[7]);
-      }
-
-      // O^T += V^T P^T.
+        // The weights, as the second product's operand: two 16-key groups to each.
+        uint4 weights[RG][2];
 #pragma unroll
-      for (int j = 0; j < DT; ++j) {
+        for (int g = 0; g < RG; ++g) {
+          if (!(MASK >> g & 1)) continue;
+          bool pick[kPicked];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          // Lane l reads four values of key 4 quad + l % 16 / 4 and gets four keys of value
-          // feature l % 16.
-          const int key = 32 * half + 4 * quad + (r >> 2);
-          const int piece = 2 * j + ((r & 3) >> 1), rest = (r & 1) * 8;
-          typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(
-              vtile + key * kRow + ((piece ^ swizzle<kPitch>(key)) << 4) + rest));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(
-              vtile + (key + 16) * kRow + ((piece ^ swizzle<kPitch>(key + 16)) << 4) + rest));
-          const s16x8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          for (int kt = 0; kt < kPicked; ++kt) pick[kt] = ((picked[kt] >> bit[g]) & 1) != 0;
+          if (near) {
 #pragma unroll
-          for (int g = 0; g < RG; ++g)
-            if (use[g])
-              acc[g][j] = mfma(vf, __builtin_bit_cast(s16x8, weights[g][half]), acc[g][j], T{});
+            for (int kt = 0; kt < 4; ++kt) {
+              const int32_t at = p0 + 16 * kt + 4 * quad;
+              const int32_t from = pick[WHOLE ? 0 : kt] ? 0 : start[g] - at;
+              const int32_t to = high[g] - at;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                s[g][kt][i] = ((i >= from) & (i < to)) ? s[g][kt][i] : -INFINITY;
+            }
+          }
+          // A row's base m is the maximum of its first tile; past the limit it is raised to a
+          // later tile's, where the weights give a lane at most 16.
+          bool up = __builtin_amdgcn_ballot_w64((m[g] == -INFINITY) &
+                                                (((see >> bit[g]) & 1) != 0) & row_ok[g]) != 0;
+          bool raised = false;
+          float fade = 1.0f;
+          for (int pass = 0;; ++pass) {
+            if (up) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int kt = 0; kt < 4; ++kt) {
+                const float x =
+                    fmaxf(fmaxf(s[g][kt][0], s[g][kt][1]), fmaxf(s[g][kt][2], s[g][kt][3]));
+                top = (near | pick[WHOLE ? 0 : kt]) ? fmaxf(top, x) : top;
+              }
+              const float more = fmaxf(m[g], rows_max(top) * tp.c);
+              const float f = __builtin_amdgcn_exp2f(m[g] - (more == -INFINITY ? 0.0f : more));
+              m[g] = more;
+              l[g] *= f;
+              fade *= f;
+              raised = true;
+            }
+            const float base = m[g] == -INFINITY ? 0.0f : -m[g];
+            uint32_t word[8];
+            float sum[4];
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+              const float shift = (near | pick[WHOLE ? 0 : kt]) ? base : -INFINITY;
+              float w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(s[g][kt][i], tp.c, shift));
+                sum[i] = kt == 0 ? w[i] : sum[i] + w[i];
+              }
+              word[2 * kt] = pack2(w[0], w[1], T{});
+              word[2 * kt + 1] = pack2(w[2], w[3], T{});
+            }
+            weights[g][0] = make_uint4(word[0], word[1], word[2], word[3]);
+            weights[g][1] = make_uint4(word[4], word[5], word[6], word[7]);
+            const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            up = pass == 0 && __builtin_amdgcn_ballot_w64(total > kLimit) != 0;
+            if (!up) {
+              l[g] += total;
+              break;
+            }
+          }
+          if (raised) {
+#pragma unroll
+            for (int j = 0; j < DT; ++j) acc[g][j] *= fade;
+          }
         }
-      }
+        // O^T += V^T P^T.
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // Lane l reads four values of key 4 quad + l % 16 / 4 and gets four keys of value
+            // feature l % 16.
+            const uint32_t at = (value0 ^ (32u * j)) + 32 * half * kRow;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 16 * kRow));
+            const s16x8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int g = 0; g < RG; ++g)
+              if (MASK >> g & 1)
+                acc[g][j] = mfma(vf, __builtin_bit_cast(s16x8, weights[g][half]), acc[g][j], T{});
+          }
+        }
+      };
+      if (RG == 1 || groups == 1) work(std::integral_constant<int, 1>{});
+      else if (groups == 2) work(std::integral_constant<int, RG == 1 ? 1 : 2>{});
+      else work(std::integral_constant<int, RG == 1 ? 1 : 3>{});
     }
     __syncthreads();  // the lists and tiles have been read
   }
@@ -473,7 +531,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(TileParams tp)
   }
 }
 
-template <typename T, int DC, int RG>
+template <typename T, int DC, int RG, bool WHOLE>
 hipError_t launch(TileParams& tp, hipStream_t stream) {
   const Params& p = tp.p;
   // Rows of a wave: whole queries, the heads of one key head each.
@@ -492,24 +550,24 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
   const size_t lds = 4 * kKeys * 16 * kPitch;
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, RG>),
+        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, RG, WHOLE>),
         hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     RLM_REQUIRE(e == hipSuccess, "routed_attention: %zu bytes of LDS refused: %s", lds,
                 hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((attend_tile_kernel<T, DC, RG>), dim3(tp.pairs * tp.tiles), dim3(kThreads),
+  hipLaunchKernelGGL((attend_tile_kernel<T, DC, RG, WHOLE>), dim3(tp.pairs * tp.tiles), dim3(kThreads),
                      lds, stream, tp);
   return launch_status("routed_attention");
 }
 
-template <typename T>
+template <typename T, bool WHOLE>
 hipError_t launch_type(TileParams& tp, hipStream_t stream) {
   const int dc = (tp.p.D + 31) / 32;
-  if (dc <= 1) return launch<T, 1, 2>(tp, stream);
-  if (dc <= 2) return launch<T, 2, 2>(tp, stream);
-  if (dc <= 3) return launch<T, 3, 2>(tp, stream);
-  if (dc <= 4) return launch<T, 4, 2>(tp, stream);
-  return launch<T, 8, 1>(tp, stream);
+  if (dc <= 1) return launch<T, 1, 2, WHOLE>(tp, stream);
+  if (dc <= 2) return launch<T, 2, 2, WHOLE>(tp, stream);
+  if (dc <= 3) return launch<T, 3, 2, WHOLE>(tp, stream);
+  if (dc <= 4) return launch<T, 4, 2, WHOLE>(tp, stream);
+  return launch<T, 8, 1, WHOLE>(tp, stream);
 }
 
 }  // namespace
@@ -529,7 +587,11 @@ hipError_t tile_launch(Params& p, int dtype, hipStream_t stream) {
   tp.negate = p.scale_log2 < 0.0f;
   // A scale of 0 as the smallest number: scores of 0 for the keys, -inf for the masked.
   tp.c = std::max(std::fabs(p.scale_log2), 1e-37f);
-  return dtype == RLM_BF16 ? launch_type<bf16>(tp, stream) : launch_type<f16>(tp, stream);
+  if (p.BS % kKeys == 0)
+    return dtype == RLM_BF16 ? launch_type<bf16, true>(tp, stream)
+                             : launch_type<f16, true>(tp, stream);
+  return dtype == RLM_BF16 ? launch_type<bf16, false>(tp, stream)
+                           : launch_type<f16, false>(tp, stream);
 }
 
 }  // namespace attention
