@@ -1,9 +1,8 @@
 // Attention over a window and picked blocks for many queries of 16-bit types: key tiles shared
 // by the rows of a workgroup.
 //
-// A workgroup holds 4 waves of RG x 16 rows, a row being one query head of one query; the rows
-// of a wave are whole queries with the heads of one key head, consecutive positions of the
-// sequence.  It walks the 64-key tiles that any of its queries sees -- its windows' and its
+// A workgroup holds 8 waves of 16 rows, a row being one query head of one query; the rows of a
+// wave are whole queries with the heads of one key head, consecutive positions of the sequence.  It walks the 64-key tiles that any of its queries sees -- its windows' and its
 // picked blocks' union, found from the picks in LDS -- and every wave takes part in those that
 // its own queries see.  Neighbouring queries share their windows and much of their picks, so a
 // tile is read once for all of them; a query's own picks decide only which of its scores count.
@@ -40,7 +39,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 typedef const __attribute__((address_space(3))) s16x8* lds_s16x8;
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
+constexpr int kRows = 16;            // rows of a wave
 constexpr int kThreads = kWaves * kWave;
 constexpr int kKeys = 64;           // keys of a tile
 constexpr int kWindowTiles = 256;   // tiles (and blocks) looked at at once
@@ -55,7 +55,7 @@ struct TileParams {
   int nqw;               // queries of a wave
   uint32_t pairs;        // (batch row, key head, chunk)
   uint32_t tiles;        // workgroups along the sequence
-  FastDiv by_pairs, by_chunks, by_kv, by_heads, by_block;
+  FastDiv by_pairs, by_chunks, by_kv, by_heads, by_block, by_picks, by_wave_queries;
   float c;               // |scale| log2(e), above 0
   bool negate;
 };
@@ -81,6 +81,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, f16) {
 template <int PITCH>
 __device__ __forceinline__ int swizzle(int row) {
   return PITCH == 8 ? (row >> 1) & 7 : row & 15;
+}
+
+// Lane l reads four values of key l / 16 * 4 + l % 16 / 4 at `at` and gets four keys of value
+// feature l % 16; eight keys, of the two 16-key groups `apart` bytes from each other.
+__device__ __forceinline__ s16x8 read_values(uint32_t at, uint32_t apart) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + apart));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // One row from the positions that it sees alone, a position at a time: lanes hold features.
@@ -144,18 +152,19 @@ __device__ void attend_row_alone(const Params& p, int64_t b, int64_t step, int64
     p.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// DC: head dim in 32s, RG: row groups of a wave, WHOLE: a tile lies within one block.
-template <typename T, int DC, int RG, bool WHOLE, int MINW = DC <= 2 ? 3 : 2>
-__global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams tp) {
+// DC: head dim in 32s, WHOLE: a tile lies within one block.
+template <typename T, int DC, bool WHOLE>
+__global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(TileParams tp) {
   constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;  // 16-byte pieces of an LDS row
   constexpr int kRow = 16 * kPitch;                        // bytes
   constexpr int kTile = kKeys * kRow;                      // bytes of a key (or value) tile
   constexpr int kDma = kPitch * kKeys / kThreads;          // DMA instructions of a wave per tile
   constexpr int DT = 2 * DC;                               // head dim in 16s
+  constexpr int kWords = kWaves / 2;                       // 16 queries of a wave: half a word
   extern __shared__ __align__(1024) char lds[];            // [2][key tile, value tile]
-  __shared__ uint32_t sel[(kWindowTiles + 2) * kWaves];    // [block][wave]: its queries' picks
-  __shared__ __align__(16) uint32_t act[kWindowTiles * kWaves];          // [tile][wave]: its queries that see it
-  __shared__ int32_t s_high[kWaves * 32], s_start[kWaves * 32];
+  __shared__ __align__(16) uint32_t sel[(kWindowTiles + 2) * kWords];  // [block]: who picked it
+  __shared__ __align__(16) uint32_t act[kWindowTiles * kWords];        // [tile]: who sees it
+  __shared__ int32_t s_high[kWaves * kRows], s_start[kWaves * kRows];
   __shared__ uint16_t list[kWindowTiles];
   __shared__ int32_t s_count, s_last;
 
@@ -192,73 +201,60 @@ __global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams 
     atomicMax(&s_last, high);
   }
 
-  // This lane's rows.
-  int32_t high[RG], start[RG];
-  int bit[RG];
-  s16x8 qf[RG][DC];
-  bool row_ok[RG];
-  int head[RG], step[RG];
-#pragma unroll
-  for (int g = 0; g < RG; ++g) {
-    uint32_t in_query;
-    const uint32_t mine = tp.by_heads.div(16 * g + r, in_query);
-    const int q = q0 + wave * tp.nqw + static_cast<int>(mine);
-    const int h = static_cast<int>(chunk) * tp.hg + static_cast<int>(in_query);
-    row_ok[g] = mine < static_cast<uint32_t>(tp.nqw) && q < p.Tq && h < p.G;
-    head[g] = static_cast<int>(hk) * p.G + (row_ok[g] ? h : 0);
-    step[g] = row_ok[g] ? q : 0;
-    bit[g] = row_ok[g] ? static_cast<int>(mine) : 0;
-    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + step[g] * p.q_st + head[g] * p.q_sh;
+  // This lane's row.
+  uint32_t in_query;
+  const uint32_t in_wave = tp.by_heads.div(r, in_query);
+  const int q = q0 + wave * tp.nqw + static_cast<int>(in_wave);
+  const int h = static_cast<int>(chunk) * tp.hg + static_cast<int>(in_query);
+  const bool row_ok = in_wave < static_cast<uint32_t>(tp.nqw) && q < p.Tq && h < p.G;
+  const int head = static_cast<int>(hk) * p.G + (row_ok ? h : 0);
+  const int step = row_ok ? q : 0;
+  const int bit = (row_ok ? static_cast<int>(in_wave) : 0) + 16 * (wave & 1);
+  s16x8 qf[DC];
+  {
+    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + step * p.q_st + head * p.q_sh;
+    const uint32_t flip = tp.negate ? 0x80008000u : 0u;
 #pragma unroll
     for (int j = 0; j < DC; ++j) {
       const int d = 32 * j + 8 * quad;
       uint4 x = *reinterpret_cast<const uint4*>(src + (d < p.D ? d : 0));
-      const uint32_t flip = tp.negate ? 0x80008000u : 0u;
       x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-      if (!(d < p.D && row_ok[g])) x = make_uint4(0, 0, 0, 0);
-      qf[g][j] = __builtin_bit_cast(s16x8, x);
+      if (!(d < p.D && row_ok)) x = make_uint4(0, 0, 0, 0);
+      qf[j] = __builtin_bit_cast(s16x8, x);
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int g = 0; g < RG; ++g) {
-    high[g] = row_ok[g] ? s_high[wave * tp.nqw + bit[g]] : 0;
-    start[g] = row_ok[g] ? s_start[wave * tp.nqw + bit[g]] : 0;
-  }
+  const int32_t high = row_ok ? s_high[wave * tp.nqw + (bit & 15)] : 0;
+  const int32_t start = row_ok ? s_start[wave * tp.nqw + (bit & 15)] : 0;
   const int32_t last = __builtin_amdgcn_readfirstlane(s_last);
   // Tiles that end at `remote` or before lie before every window of the wave's rows: their keys
   // are seen by the picks alone, whole blocks at a time.
-  int32_t remote = 0x7fffffff;
-#pragma unroll
-  for (int g = 0; g < RG; ++g) remote = high[g] > 0 ? min(remote, start[g]) : remote;
+  int32_t remote = high > 0 ? start : 0x7fffffff;
 #pragma unroll
   for (int off = 1; off < 16; off <<= 1) remote = min(remote, __shfl_xor(remote, off, kWave));
   remote = __builtin_amdgcn_readfirstlane(remote);
 
-  f32x4 acc[RG][DT];
-  float m[RG], l[RG];
+  f32x4 acc[DT];
+  float m = -INFINITY, l = 0.0f;
 #pragma unroll
-  for (int g = 0; g < RG; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < DT; ++j) acc[g][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int j = 0; j < DT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   // This lane's pieces of a tile: row and byte in the row, which the swizzle permutes; pieces
   // past the head dim come as zeros.
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   const uint32_t k_bytes = static_cast<uint32_t>(p.k_st) * 2u;
   const uint32_t v_bytes = static_cast<uint32_t>(p.v_st) * 2u;
-  uint32_t dma_row[kDma], k_off[kDma], v_off[kDma];
+  uint32_t k_off[kDma], v_off[kDma];
+  auto dma_row = [&](int k) {
+    return static_cast<uint32_t>(((wave * kDma + k) * kWave + lane) / kPitch);
+  };
 #pragma unroll
   for (int k = 0; k < kDma; ++k) {
-    const int piece = (wave * kDma + k) * kWave + lane;
-    dma_row[k] = piece / kPitch;
-    const int from = (piece % kPitch) ^ swizzle<kPitch>(dma_row[k]);
+    const uint32_t row = dma_row(k);
+    const int from = (lane % kPitch) ^ swizzle<kPitch>(row);
     const bool ok = 8 * from < p.D;
-    k_off[k] = ok ? dma_row[k] * k_bytes + 16u * from : kNoOffset;
-    v_off[k] = ok ? dma_row[k] * v_bytes + 16u * from : kNoOffset;
+    k_off[k] = ok ? row * k_bytes + 16u * from : kNoOffset;
+    v_off[k] = ok ? row * v_bytes + 16u * from : kNoOffset;
   }
   auto issue = [&](int buffer, int32_t first) {
     const rsrc_t kr = make_rsrc(kbase + first * p.k_st, 0x7ffffff0u);
@@ -275,7 +271,7 @@ __global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams 
     } else {
 #pragma unroll
       for (int k = 0; k < kDma; ++k) {
-        const uint32_t over = dma_row[k] > rows ? dma_row[k] - rows : 0;
+        const uint32_t row = dma_row(k), over = row > rows ? row - rows : 0;
         const uint32_t ko = k_off[k] - over * k_bytes, vo = v_off[k] - over * v_bytes;
         lds_dma16(kr, to + 1024u * k, k_off[k] == kNoOffset ? kNoOffset : ko);
         lds_dma16(vr, to + kTile + 1024u * k, v_off[k] == kNoOffset ? kNoOffset : vo);
@@ -291,31 +287,35 @@ __global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams 
     const int32_t block0 = static_cast<int32_t>(tp.by_block.div(w0));
     const int window_tiles = (w1 - w0 + kKeys - 1) / kKeys;
     // What the queries see in this window.
-    for (int i = threadIdx.x; i < (kWindowTiles + 2) * kWaves; i += kThreads) sel[i] = 0;
-    for (int i = threadIdx.x; i < window_tiles * kWaves; i += kThreads) act[i] = 0;
+    for (int i = threadIdx.x; i < (kWindowTiles + 2) * kWords; i += kThreads) sel[i] = 0;
+    for (int i = threadIdx.x; i < window_tiles * kWords; i += kThreads) act[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < queries * (p.TOP + 1); i += kThreads) {
-      const int q = i / (p.TOP + 1), k = i % (p.TOP + 1) - 1;
-      if (q0 + q >= p.Tq) continue;
-      const int w = q / tp.nqw;
-      const uint32_t mine = 1u << (q - w * tp.nqw);
-      int32_t first = s_start[q], end = s_high[q];
-      if (k >= 0) {
-        const int32_t block =
-            p.blocks[b * p.blk_sb + static_cast<int64_t>(q0 + q) * p.blk_st + hk * p.blk_sh + k];
+      uint32_t pick;
+      const int query = static_cast<int>(tp.by_picks.div(i, pick));
+      if (q0 + query >= p.Tq) continue;
+      uint32_t place;
+      const uint32_t of = tp.by_wave_queries.div(query, place);
+      const uint32_t mine = 1u << (place + 16 * (of & 1));
+      int32_t first = s_start[query], end = s_high[query];
+      const bool window = pick == static_cast<uint32_t>(p.TOP);
+      if (!window) {
+        const int32_t block = p.blocks[b * p.blk_sb + static_cast<int64_t>(q0 + query) * p.blk_st +
+                                       hk * p.blk_sh + pick];
         const int64_t at = static_cast<int64_t>(block) * p.BS;
-        if (block < 0 || at >= min(s_start[q], w1) || at + p.BS <= w0) continue;
-        if (!WHOLE) atomicOr(&sel[(block - block0) * kWaves + w], mine);
+        if (block < 0 || at >= min(first, w1) || at + p.BS <= w0) continue;
+        if (!WHOLE) atomicOr(&sel[(block - block0) * kWords + of / 2], mine);
+        end = static_cast<int32_t>(min(at + p.BS, static_cast<int64_t>(first)));
         first = static_cast<int32_t>(at);
-        end = static_cast<int32_t>(min(at + p.BS, static_cast<int64_t>(s_start[q])));
       }
       first = max(first, w0);
       end = min(end, w1);
-      for (int32_t t = (first - w0) / kKeys; w0 + t * kKeys < end; ++t)
+      for (int32_t t = (first - w0) / kKeys; w0 + t * kKeys < end; ++t) {
         if (first < end) {
-          atomicOr(&act[t * kWaves + w], mine);
-          if (WHOLE && k >= 0) atomicOr(&sel[t * kWaves + w], mine);
+          atomicOr(&act[t * kWords + of / 2], mine);
+          if (WHOLE && !window) atomicOr(&sel[t * kWords + of / 2], mine);
         }
+      }
     }
     __syncthreads();
     if (wave == 0) {
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams 
         const int t = i + lane;
         bool any = false;
         if (t < window_tiles) {
-          const uint4 a = *reinterpret_cast<const uint4*>(&act[t * kWaves]);
+          const uint4 a = *reinterpret_cast<const uint4*>(&act[t * kWords]);
           any = (a.x | a.y | a.z | a.w) != 0;
         }
         const uint64_t mask = __builtin_amdgcn_ballot_w64(any);
@@ -337,8 +337,10 @@ __global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams 
     const int count = __builtin_amdgcn_readfirstlane(s_count);
     if (count == 0) continue;
     // Lane i holds the list's entry i of the current 64, and what the wave's queries see of it.
+    const int word = wave / 2;
+    const uint32_t own = 0xffffu << (16 * (wave & 1));
     int entry = list[min(lane, count - 1)];
-    uint32_t seen = act[entry * kWaves + wave];
+    uint32_t seen = act[entry * kWords + word] & own;
     int next = __builtin_amdgcn_readlane(entry, 0);
     uint32_t next_see = __builtin_amdgcn_readlane(seen, 0);
     issue(0, w0 + kKeys * next);
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams 
       if (n + 1 < count) {
         if (((n + 1) & (kWave - 1)) == 0) {
           entry = list[min(n + 1 + lane, count - 1)];
-          seen = act[entry * kWaves + wave];
+          seen = act[entry * kWords + word] & own;
         }
         next = __builtin_amdgcn_readlane(entry, (n + 1) & (kWave - 1));
         next_see = __builtin_amdgcn_readlane(seen, (n + 1) & (kWave - 1));
@@ -367,175 +369,140 @@ __global__ __launch_bounds__(kThreads, MINW) void attend_tile_kernel(TileParams 
       const int vrow = 4 * quad + (r >> 2);
       const uint32_t value0 = tile0 + kTile + vrow * kRow +
                               ((((r & 3) >> 1) ^ swizzle<kPitch>(vrow)) << 4) + (r & 1) * 8;
-      // The wave's queries that picked the block of a lane's four keys of 16-key group kt.
+      // Whether the row picked the block of this lane's four keys of 16-key group kt.
       constexpr int kPicked = WHOLE ? 1 : 4;
-      uint32_t picked[kPicked];
+      bool pick[kPicked];
 #pragma unroll
-      for (int kt = 0; kt < kPicked; ++kt)
-        picked[kt] = WHOLE ? sel[t * kWaves + wave]
-                           : sel[(tp.by_block.div(p0 + 16 * kt + 4 * quad) - block0) * kWaves + wave];
-      uint32_t groups = 0;
-#pragma unroll
-      for (int g = 0; g < RG; ++g)
-        if (__builtin_amdgcn_ballot_w64(row_ok[g] & (((see >> bit[g]) & 1) != 0)) != 0)
-          groups |= 1u << g;
-      groups = __builtin_amdgcn_readfirstlane(groups);
+      for (int kt = 0; kt < kPicked; ++kt) {
+        const uint32_t who =
+            WHOLE ? sel[t * kWords + word]
+                  : sel[(tp.by_block.div(p0 + 16 * kt + 4 * quad) - block0) * kWords + word];
+        pick[kt] = row_ok & (((who >> bit) & 1) != 0);
+      }
 
-      // The tile for the row groups of MASK.
-      auto work = [&](auto mask) {
-        constexpr int MASK = decltype(mask)::value;
-        // S^T = K Q^T.
-        f32x4 s[RG][4];
+      // S^T = K Q^T.
+      f32x4 s[4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        s[kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < DC; ++j)
+          s[kt] = mfma(*(lds_s16x8)((key0 ^ (64u * j)) + 16 * kt * kRow), qf[j], s[kt], T{});
+      }
+      // The first values of the second product, on their way while the weights are computed:
+      // step i is 32-key half i / DT and feature group i % DT.
+      constexpr int kAhead = 4;
+      auto values = [&](int i) {
+        return read_values((value0 ^ (32u * (i % DT))) + i / DT * 32 * kRow, 16 * kRow);
+      };
+      s16x8 vf[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) vf[i] = values(i);
+      __builtin_amdgcn_sched_barrier(0);
+
+      // The weights, as the second product's operand: two 16-key groups to each.
+      if (near) {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
+          const int32_t at = p0 + 16 * kt + 4 * quad;
+          const int32_t from = pick[WHOLE ? 0 : kt] ? 0 : start - at;
+          const int32_t to = high - at;
 #pragma unroll
-          for (int j = 0; j < DC; ++j) {
-            const s16x8 kf = *(lds_s16x8)((key0 ^ (64u * j)) + 16 * kt * kRow);
-#pragma unroll
-            for (int g = 0; g < RG; ++g) {
-              if (!(MASK >> g & 1)) continue;
-              if (j == 0) s[g][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-              s[g][kt] = mfma(kf, qf[g][j], s[g][kt], T{});
-            }
-          }
+          for (int i = 0; i < 4; ++i) s[kt][i] = ((i >= from) & (i < to)) ? s[kt][i] : -INFINITY;
         }
-        // The weights, as the second product's operand: two 16-key groups to each.
-        uint4 weights[RG][2];
+      }
+      // A row's base m is the maximum of its first tile; past the limit it is raised to a later
+      // tile's, where the weights give a lane at most 16.
+      bool up = __builtin_amdgcn_ballot_w64((m == -INFINITY) & (((see >> bit) & 1) != 0) &
+                                            row_ok) != 0;
+      uint4 weights[2];
+      for (int pass = 0;; ++pass) {
+        if (up) {
+          float top = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < RG; ++g) {
-          if (!(MASK >> g & 1)) continue;
-          bool pick[kPicked];
-#pragma unroll
-          for (int kt = 0; kt < kPicked; ++kt) pick[kt] = ((picked[kt] >> bit[g]) & 1) != 0;
-          if (near) {
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-              const int32_t at = p0 + 16 * kt + 4 * quad;
-              const int32_t from = pick[WHOLE ? 0 : kt] ? 0 : start[g] - at;
-              const int32_t to = high[g] - at;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                s[g][kt][i] = ((i >= from) & (i < to)) ? s[g][kt][i] : -INFINITY;
-            }
+          for (int kt = 0; kt < 4; ++kt) {
+            const float x = fmaxf(fmaxf(s[kt][0], s[kt][1]), fmaxf(s[kt][2], s[kt][3]));
+            top = (near | pick[WHOLE ? 0 : kt]) ? fmaxf(top, x) : top;
           }
-          // A row's base m is the maximum of its first tile; past the limit it is raised to a
-          // later tile's, where the weights give a lane at most 16.
-          bool up = __builtin_amdgcn_ballot_w64((m[g] == -INFINITY) &
-                                                (((see >> bit[g]) & 1) != 0) & row_ok[g]) != 0;
-          bool raised = false;
-          float fade = 1.0f;
-          for (int pass = 0;; ++pass) {
-            if (up) {
-              float top = -INFINITY;
+          const float more = fmaxf(m, rows_max(top) * tp.c);
+          const float fade = __builtin_amdgcn_exp2f(m - (more == -INFINITY ? 0.0f : more));
+          m = more;
+          l *= fade;
 #pragma unroll
-              for (int kt = 0; kt < 4; ++kt) {
-                const float x =
-                    fmaxf(fmaxf(s[g][kt][0], s[g][kt][1]), fmaxf(s[g][kt][2], s[g][kt][3]));
-                top = (near | pick[WHOLE ? 0 : kt]) ? fmaxf(top, x) : top;
-              }
-              const float more = fmaxf(m[g], rows_max(top) * tp.c);
-              const float f = __builtin_amdgcn_exp2f(m[g] - (more == -INFINITY ? 0.0f : more));
-              m[g] = more;
-              l[g] *= f;
-              fade *= f;
-              raised = true;
-            }
-            const float base = m[g] == -INFINITY ? 0.0f : -m[g];
-            uint32_t word[8];
-            float sum[4];
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-              const float shift = (near | pick[WHOLE ? 0 : kt]) ? base : -INFINITY;
-              float w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(fmaf(s[g][kt][i], tp.c, shift));
-                sum[i] = kt == 0 ? w[i] : sum[i] + w[i];
-              }
-              word[2 * kt] = pack2(w[0], w[1], T{});
-              word[2 * kt + 1] = pack2(w[2], w[3], T{});
-            }
-            weights[g][0] = make_uint4(word[0], word[1], word[2], word[3]);
-            weights[g][1] = make_uint4(word[4], word[5], word[6], word[7]);
-            const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            up = pass == 0 && __builtin_amdgcn_ballot_w64(total > kLimit) != 0;
-            if (!up) {
-              l[g] += total;
-              break;
-            }
-          }
-          if (raised) {
-#pragma unroll
-            for (int j = 0; j < DT; ++j) acc[g][j] *= fade;
-          }
+          for (int j = 0; j < DT; ++j) acc[j] *= fade;
         }
-        // O^T += V^T P^T.
+        const float base = m == -INFINITY ? 0.0f : -m;
+        uint32_t half[8];
+        float sum[4];
 #pragma unroll
-        for (int j = 0; j < DT; ++j) {
+        for (int kt = 0; kt < 4; ++kt) {
+          const float shift = (near | pick[WHOLE ? 0 : kt]) ? base : -INFINITY;
+          float w[4];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            // Lane l reads four values of key 4 quad + l % 16 / 4 and gets four keys of value
-            // feature l % 16.
-            const uint32_t at = (value0 ^ (32u * j)) + 32 * half * kRow;
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 16 * kRow));
-            const s16x8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-            for (int g = 0; g < RG; ++g)
-              if (MASK >> g & 1)
-                acc[g][j] = mfma(vf, __builtin_bit_cast(s16x8, weights[g][half]), acc[g][j], T{});
+          for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], tp.c, shift));
+            sum[i] = kt == 0 ? w[i] : sum[i] + w[i];
           }
+          half[2 * kt] = pack2(w[0], w[1], T{});
+          half[2 * kt + 1] = pack2(w[2], w[3], T{});
         }
-      };
-      if (RG == 1 || groups == 1) work(std::integral_constant<int, 1>{});
-      else if (groups == 2) work(std::integral_constant<int, RG == 1 ? 1 : 2>{});
-      else work(std::integral_constant<int, RG == 1 ? 1 : 3>{});
+        weights[0] = make_uint4(half[0], half[1], half[2], half[3]);
+        weights[1] = make_uint4(half[4], half[5], half[6], half[7]);
+        const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        up = pass == 0 && __builtin_amdgcn_ballot_w64(total > kLimit) != 0;
+        if (!up) {
+          l += total;
+          break;
+        }
+      }
+
+      // O^T += V^T P^T.
+#pragma unroll
+      for (int i = 0; i < 2 * DT; ++i) {
+        acc[i % DT] = mfma(vf[i % kAhead], __builtin_bit_cast(s16x8, weights[i / DT]), acc[i % DT],
+                           T{});
+        if (i + kAhead < 2 * DT) vf[i % kAhead] = values(i + kAhead);
+      }
     }
     __syncthreads();  // the lists and tiles have been read
   }
 
+  const float total = rows_sum(l);
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  bool fine = fabsf(total) < INFINITY;
 #pragma unroll
-  for (int g = 0; g < RG; ++g) {
-    const float total = rows_sum(l[g]);
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    bool fine = fabsf(total) < INFINITY;
+  for (int j = 0; j < DT; ++j)
 #pragma unroll
-    for (int j = 0; j < DT; ++j)
+    for (int i = 0; i < 4; ++i) fine = fine & (fabsf(acc[j][i]) < INFINITY);
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(!fine && row_ok);
+  if (row_ok) {
+    const int64_t row = (b * p.Tq + step) * p.Hq + head;
+    T* out = static_cast<T*>(p.out) + row * p.D;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) fine = fine && fabsf(acc[g][j][i]) < INFINITY;
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(!fine && row_ok[g]);
-    if (row_ok[g]) {
-      const int64_t row = (b * p.Tq + step[g]) * p.Hq + head[g];
-      T* out = static_cast<T*>(p.out) + row * p.D;
-#pragma unroll
-      for (int j = 0; j < DT; ++j) {
-        const int d = 16 * j + 4 * quad;
-        if (d < p.D)
-          put4<T>(out + d, acc[g][j][0] * inv, acc[g][j][1] * inv, acc[g][j][2] * inv,
-                  acc[g][j][3] * inv);
-      }
-      if (quad == 0)
-        p.lse[row] = total == 0.0f ? -INFINITY : (m[g] + __builtin_amdgcn_logf(total)) * kLn2;
+    for (int j = 0; j < DT; ++j) {
+      const int d = 16 * j + 4 * quad;
+      if (d < p.D)
+        put4<T>(out + d, acc[j][0] * inv, acc[j][1] * inv, acc[j][2] * inv, acc[j][3] * inv);
     }
-    if (bad != 0) {
-      uint32_t rows = static_cast<uint32_t>(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xffffu;
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the stores above, which these replace
-      while (rows != 0) {
-        const int from = __builtin_ctz(rows);
-        rows &= rows - 1;
-        attend_row_alone<T>(p, b, __builtin_amdgcn_readlane(step[g], from), hk,
-                            __builtin_amdgcn_readlane(head[g], from),
-                            tp.negate ? -tp.c : tp.c);
-      }
+    if (quad == 0)
+      p.lse[row] = total == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(total)) * kLn2;
+  }
+  if (bad != 0) {
+    uint32_t rows = static_cast<uint32_t>(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xffffu;
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the stores above, which these replace
+    while (rows != 0) {
+      const int from = __builtin_ctz(rows);
+      rows &= rows - 1;
+      attend_row_alone<T>(p, b, __builtin_amdgcn_readlane(step, from), hk,
+                          __builtin_amdgcn_readlane(head, from), tp.negate ? -tp.c : tp.c);
     }
   }
 }
 
-template <typename T, int DC, int RG, bool WHOLE>
+template <typename T, int DC, bool WHOLE>
 hipError_t launch(TileParams& tp, hipStream_t stream) {
   const Params& p = tp.p;
   // Rows of a wave: whole queries, the heads of one key head each.
-  constexpr int kRows = 16 * RG;
   tp.chunks = (p.G + kRows - 1) / kRows;
   tp.hg = (p.G + tp.chunks - 1) / tp.chunks;
   tp.nqw = kRows / tp.hg;
@@ -545,17 +512,19 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
   tp.by_chunks = FastDiv(static_cast<uint32_t>(tp.chunks));
   tp.by_kv = FastDiv(static_cast<uint32_t>(p.Hk));
   tp.by_heads = FastDiv(static_cast<uint32_t>(tp.hg));
+  tp.by_picks = FastDiv(static_cast<uint32_t>(p.TOP + 1));
+  tp.by_wave_queries = FastDiv(static_cast<uint32_t>(tp.nqw));
   tp.by_block = FastDiv(static_cast<uint32_t>(p.BS));
   constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;
   const size_t lds = 4 * kKeys * 16 * kPitch;
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, RG, WHOLE>),
+        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, WHOLE>),
         hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     RLM_REQUIRE(e == hipSuccess, "routed_attention: %zu bytes of LDS refused: %s", lds,
                 hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((attend_tile_kernel<T, DC, RG, WHOLE>), dim3(tp.pairs * tp.tiles), dim3(kThreads),
+  hipLaunchKernelGGL((attend_tile_kernel<T, DC, WHOLE>), dim3(tp.pairs * tp.tiles), dim3(kThreads),
                      lds, stream, tp);
   return launch_status("routed_attention");
 }
@@ -563,11 +532,11 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
 template <typename T, bool WHOLE>
 hipError_t launch_type(TileParams& tp, hipStream_t stream) {
   const int dc = (tp.p.D + 31) / 32;
-  if (dc <= 1) return launch<T, 1, 2, WHOLE>(tp, stream);
-  if (dc <= 2) return launch<T, 2, 2, WHOLE>(tp, stream);
-  if (dc <= 3) return launch<T, 3, 2, WHOLE>(tp, stream);
-  if (dc <= 4) return launch<T, 4, 2, WHOLE>(tp, stream);
-  return launch<T, 8, 1, WHOLE>(tp, stream);
+  if (dc <= 1) return launch<T, 1, WHOLE>(tp, stream);
+  if (dc <= 2) return launch<T, 2, WHOLE>(tp, stream);
+  if (dc <= 3) return launch<T, 3, WHOLE>(tp, stream);
+  if (dc <= 4) return launch<T, 4, WHOLE>(tp, stream);
+  return launch<T, 8, WHOLE>(tp, stream);
 }
 
 }  // namespace
