@@ -1,7 +1,7 @@
 // Attention over a window and picked blocks for many queries of 16-bit types: key tiles shared
 // by the rows of a workgroup.
 //
-// A workgroup holds 8 waves of 16 rows, a row being one query head of one query; the rows of a
+// A workgroup holds 4 waves of 16 rows, a row being one query head of one query; the rows of a
 // wave are whole queries with the heads of one key head, consecutive positions of the sequence.  It walks the 64-key tiles that any of its queries sees -- its windows' and its
 // picked blocks' union, found from the picks in LDS -- and every wave takes part in those that
 // its own queries see.  Neighbouring queries share their windows and much of their picks, so a
@@ -39,10 +39,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 typedef const __attribute__((address_space(3))) s16x8* lds_s16x8;
 
-constexpr int kWaves = 8;
-constexpr int kRows = 16;            // rows of a wave
-constexpr int kThreads = kWaves * kWave;
-constexpr int kKeys = 64;           // keys of a tile
+constexpr int kRows = 16;           // rows of a wave
+constexpr int kMostKeys = 64;       // keys of the largest tile
 constexpr int kWindowTiles = 256;   // tiles (and blocks) looked at at once
 // Sum of a lane's weights of a row in one tile beyond which its base is raised: fp16 weights stay far
 // inside the type, and the outputs' rescaling is rare.
@@ -58,6 +56,7 @@ struct TileParams {
   FastDiv by_pairs, by_chunks, by_kv, by_heads, by_block, by_picks, by_wave_queries;
   float c;               // |scale| log2(e), above 0
   bool negate;
+  bool far;              // rows of a key head reach over 2 GiB: offsets from each tile's first
 };
 
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, bf16) {
@@ -74,6 +73,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, f16) {
   typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
   const f32x2_t v = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+}
+
+// A workgroup barrier that orders LDS reads and leaves loads into LDS outstanding.
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // 16-byte pieces of an LDS row: rows of 8 pieces alternate between the halves of the 16 piece
@@ -152,16 +158,19 @@ __device__ void attend_row_alone(const Params& p, int64_t b, int64_t step, int64
     p.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// DC: head dim in 32s, WHOLE: a tile lies within one block.
-template <typename T, int DC, bool WHOLE>
-__global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(TileParams tp) {
+// DC: head dim in 32s, WHOLE: a tile lies within one block; tiles of kKeys keys for kWaves waves,
+// kStages of them in LDS.
+template <typename T, int DC, bool WHOLE, int kKeys, int kWaves, int kStages>
+__global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_kernel(TileParams tp) {
+  constexpr int kThreads = kWaves * kWave;
+  constexpr int KT = kKeys / 16;                           // 16-key groups of a tile
   constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;  // 16-byte pieces of an LDS row
   constexpr int kRow = 16 * kPitch;                        // bytes
   constexpr int kTile = kKeys * kRow;                      // bytes of a key (or value) tile
   constexpr int kDma = kPitch * kKeys / kThreads;          // DMA instructions of a wave per tile
   constexpr int DT = 2 * DC;                               // head dim in 16s
   constexpr int kWords = kWaves / 2;                       // 16 queries of a wave: half a word
-  extern __shared__ __align__(1024) char lds[];            // [2][key tile, value tile]
+  extern __shared__ __align__(1024) char lds[];            // [stage][key tile, value tile]
   __shared__ __align__(16) uint32_t sel[(kWindowTiles + 2) * kWords];  // [block]: who picked it
   __shared__ __align__(16) uint32_t act[kWindowTiles * kWords];        // [tile]: who sees it
   __shared__ int32_t s_high[kWaves * kRows], s_start[kWaves * kRows];
@@ -256,19 +265,21 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
     k_off[k] = ok ? row * k_bytes + 16u * from : kNoOffset;
     v_off[k] = ok ? row * v_bytes + 16u * from : kNoOffset;
   }
+  const rsrc_t k_rows = make_rsrc(kbase, 0x7ffffff0u), v_rows = make_rsrc(vbase, 0x7ffffff0u);
   auto issue = [&](int buffer, int32_t first) {
-    const rsrc_t kr = make_rsrc(kbase + first * p.k_st, 0x7ffffff0u);
-    const rsrc_t vr = make_rsrc(vbase + first * p.v_st, 0x7ffffff0u);
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kTile + wave * kDma * 1024);
     // Rows past the last that a query of the workgroup sees (their keys are masked, and they may
     // hold anything) read that one.
     const uint32_t rows = static_cast<uint32_t>(last - 1 - first);
-    if (rows >= kKeys - 1) {
+    if (!tp.far && rows >= kKeys - 1) {
+      const uint32_t ks = first * k_bytes, vs = first * v_bytes;
 #pragma unroll
-      for (int k = 0; k < kDma; ++k) lds_dma16(kr, to + 1024u * k, k_off[k]);
+      for (int k = 0; k < kDma; ++k) lds_dma16(k_rows, to + 1024u * k, k_off[k], ks);
 #pragma unroll
-      for (int k = 0; k < kDma; ++k) lds_dma16(vr, to + kTile + 1024u * k, v_off[k]);
+      for (int k = 0; k < kDma; ++k) lds_dma16(v_rows, to + kTile + 1024u * k, v_off[k], vs);
     } else {
+      const rsrc_t kr = make_rsrc(kbase + first * p.k_st, 0x7ffffff0u);
+      const rsrc_t vr = make_rsrc(vbase + first * p.v_st, 0x7ffffff0u);
 #pragma unroll
       for (int k = 0; k < kDma; ++k) {
         const uint32_t row = dma_row(k), over = row > rows ? row - rows : 0;
@@ -324,8 +335,10 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
         const int t = i + lane;
         bool any = false;
         if (t < window_tiles) {
-          const uint4 a = *reinterpret_cast<const uint4*>(&act[t * kWords]);
-          any = (a.x | a.y | a.z | a.w) != 0;
+          uint32_t a = 0;
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) a |= act[t * kWords + w];
+          any = a != 0;
         }
         const uint64_t mask = __builtin_amdgcn_ballot_w64(any);
         if (any) list[count + __builtin_popcountll(mask & ((uint64_t(1) << lane) - 1))] = t;
@@ -341,36 +354,63 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
     const uint32_t own = 0xffffu << (16 * (wave & 1));
     int entry = list[min(lane, count - 1)];
     uint32_t seen = act[entry * kWords + word] & own;
-    int next = __builtin_amdgcn_readlane(entry, 0);
-    uint32_t next_see = __builtin_amdgcn_readlane(seen, 0);
-    issue(0, w0 + kKeys * next);
-    for (int n = 0; n < count; ++n) {
-      const int t = next;
-      const uint32_t see = next_see;
-      if (n + 1 < count) {
-        if (((n + 1) & (kWave - 1)) == 0) {
-          entry = list[min(n + 1 + lane, count - 1)];
-          seen = act[entry * kWords + word] & own;
-        }
-        next = __builtin_amdgcn_readlane(entry, (n + 1) & (kWave - 1));
-        next_see = __builtin_amdgcn_readlane(seen, (n + 1) & (kWave - 1));
+    // Tile i of the list goes to stage i mod kStages; kStages - 1 of them are on their way while
+    // one is worked on.
+    constexpr int kQueue = kStages - 1;
+    auto tile_of = [&](int i) {
+      if ((i & (kWave - 1)) == 0 && i != 0) {
+        entry = list[min(i + lane, count - 1)];
+        seen = act[entry * kWords + word] & own;
       }
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-      __syncthreads();  // tile n is in LDS, tile n - 1 has been read
-      if (n + 1 < count) issue((n + 1) & 1, w0 + kKeys * next);
+      return __builtin_amdgcn_readlane(entry, i & (kWave - 1));
+    };
+    int ahead = 0, stage = 0;
+    int tiles_ahead[kQueue];
+    uint32_t see_ahead[kQueue];
+#pragma unroll
+    for (int i = 0; i < kQueue; ++i) {
+      tiles_ahead[i] = see_ahead[i] = 0;
+      if (i < count) {
+        tiles_ahead[i] = tile_of(i);
+        see_ahead[i] = __builtin_amdgcn_readlane(seen, i & (kWave - 1));
+        issue(i, w0 + kKeys * tiles_ahead[i]);
+        ++ahead;
+      }
+    }
+    for (int n = 0; n < count; ++n) {
+      const int t = tiles_ahead[0];
+      const uint32_t see = see_ahead[0];
+#pragma unroll
+      for (int i = 0; i + 1 < kQueue; ++i) {
+        tiles_ahead[i] = tiles_ahead[i + 1];
+        see_ahead[i] = see_ahead[i + 1];
+      }
+      // Tile n has arrived when at most the loads of the tiles after it are outstanding.
+      if (kStages > 2 && n + kStages - 2 < count)
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((kQueue - 1) * 2 * kDma));
+      else
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      barrier();  // tile n is in LDS for every wave, tile n - 1 has been read by every wave
+      if (ahead < count) {
+        tiles_ahead[kQueue - 1] = tile_of(ahead);
+        see_ahead[kQueue - 1] = __builtin_amdgcn_readlane(seen, ahead & (kWave - 1));
+        issue(stage == 0 ? kStages - 1 : stage - 1, w0 + kKeys * tiles_ahead[kQueue - 1]);
+        ++ahead;
+      }
+      const uint32_t tile0 = lds0 + stage * 2 * kTile;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
       if (see == 0) continue;
       const int32_t p0 = w0 + t * kKeys;
       const bool near = p0 + kKeys > remote;
       // A lane's first piece of the key and of the value rows that it reads; the swizzle makes
       // later ones an exclusive or away (pieces 4 j + quad of the keys, 2 j + (0 or 1) of the
       // values).
-      const uint32_t tile0 = lds0 + (n & 1) * 2 * kTile;
       const uint32_t key0 = tile0 + r * kRow + ((quad ^ swizzle<kPitch>(r)) << 4);
       const int vrow = 4 * quad + (r >> 2);
       const uint32_t value0 = tile0 + kTile + vrow * kRow +
                               ((((r & 3) >> 1) ^ swizzle<kPitch>(vrow)) << 4) + (r & 1) * 8;
       // Whether the row picked the block of this lane's four keys of 16-key group kt.
-      constexpr int kPicked = WHOLE ? 1 : 4;
+      constexpr int kPicked = WHOLE ? 1 : KT;
       bool pick[kPicked];
 #pragma unroll
       for (int kt = 0; kt < kPicked; ++kt) {
@@ -381,9 +421,9 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
       }
 
       // S^T = K Q^T.
-      f32x4 s[4];
+      f32x4 s[KT];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
+      for (int kt = 0; kt < KT; ++kt) {
         s[kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < DC; ++j)
@@ -391,19 +431,20 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
       }
       // The first values of the second product, on their way while the weights are computed:
       // step i is 32-key half i / DT and feature group i % DT.
-      constexpr int kAhead = 4;
+      constexpr int kAhead = 4, kSteps = DT * KT / 2;
       auto values = [&](int i) {
         return read_values((value0 ^ (32u * (i % DT))) + i / DT * 32 * kRow, 16 * kRow);
       };
       s16x8 vf[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) vf[i] = values(i);
+      for (int i = 0; i < kAhead; ++i)
+        if (i < kSteps) vf[i] = values(i);
       __builtin_amdgcn_sched_barrier(0);
 
       // The weights, as the second product's operand: two 16-key groups to each.
       if (near) {
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
+        for (int kt = 0; kt < KT; ++kt) {
           const int32_t at = p0 + 16 * kt + 4 * quad;
           const int32_t from = pick[WHOLE ? 0 : kt] ? 0 : start - at;
           const int32_t to = high - at;
@@ -415,13 +456,14 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
       // tile's, where the weights give a lane at most 16.
       bool up = __builtin_amdgcn_ballot_w64((m == -INFINITY) & (((see >> bit) & 1) != 0) &
                                             row_ok) != 0;
-      uint4 weights[2];
+      uint4 weights[KT / 2];
       for (int pass = 0;; ++pass) {
         if (up) {
           float top = -INFINITY;
 #pragma unroll
-          for (int kt = 0; kt < 4; ++kt) {
-            const float x = fmaxf(fmaxf(s[kt][0], s[kt][1]), fmaxf(s[kt][2], s[kt][3]));
+          for (int kt = 0; kt < KT; ++kt) {
+            float x = fmaxf(fmaxf(s[kt][0], s[kt][1]), fmaxf(s[kt][2], s[kt][3]));
+            asm("" : "+v"(x));  // keeps these maxima in this rare branch
             top = (near | pick[WHOLE ? 0 : kt]) ? fmaxf(top, x) : top;
           }
           const float more = fmaxf(m, rows_max(top) * tp.c);
@@ -432,10 +474,10 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
           for (int j = 0; j < DT; ++j) acc[j] *= fade;
         }
         const float base = m == -INFINITY ? 0.0f : -m;
-        uint32_t half[8];
+        uint32_t half[2 * KT];
         float sum[4];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
+        for (int kt = 0; kt < KT; ++kt) {
           const float shift = (near | pick[WHOLE ? 0 : kt]) ? base : -INFINITY;
           float w[4];
 #pragma unroll
@@ -446,8 +488,9 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
           half[2 * kt] = pack2(w[0], w[1], T{});
           half[2 * kt + 1] = pack2(w[2], w[3], T{});
         }
-        weights[0] = make_uint4(half[0], half[1], half[2], half[3]);
-        weights[1] = make_uint4(half[4], half[5], half[6], half[7]);
+#pragma unroll
+        for (int i = 0; i < KT / 2; ++i)
+          weights[i] = make_uint4(half[4 * i], half[4 * i + 1], half[4 * i + 2], half[4 * i + 3]);
         const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         up = pass == 0 && __builtin_amdgcn_ballot_w64(total > kLimit) != 0;
         if (!up) {
@@ -458,10 +501,10 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
 
       // O^T += V^T P^T.
 #pragma unroll
-      for (int i = 0; i < 2 * DT; ++i) {
+      for (int i = 0; i < kSteps; ++i) {
         acc[i % DT] = mfma(vf[i % kAhead], __builtin_bit_cast(s16x8, weights[i / DT]), acc[i % DT],
                            T{});
-        if (i + kAhead < 2 * DT) vf[i % kAhead] = values(i + kAhead);
+        if (i + kAhead < kSteps) vf[i % kAhead] = values(i + kAhead);
       }
     }
     __syncthreads();  // the lists and tiles have been read
@@ -499,7 +542,7 @@ __global__ __launch_bounds__(kThreads, DC <= 4 ? 4 : 2) void attend_tile_kernel(
   }
 }
 
-template <typename T, int DC, bool WHOLE>
+template <typename T, int DC, bool WHOLE, int kKeys, int kWaves, int kStages>
 hipError_t launch(TileParams& tp, hipStream_t stream) {
   const Params& p = tp.p;
   // Rows of a wave: whole queries, the heads of one key head each.
@@ -516,27 +559,34 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
   tp.by_wave_queries = FastDiv(static_cast<uint32_t>(tp.nqw));
   tp.by_block = FastDiv(static_cast<uint32_t>(p.BS));
   constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;
-  const size_t lds = 4 * kKeys * 16 * kPitch;
+  const size_t lds = kStages * 2 * kKeys * 16 * kPitch;
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, WHOLE>),
+        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, WHOLE, kKeys, kWaves, kStages>),
         hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     RLM_REQUIRE(e == hipSuccess, "routed_attention: %zu bytes of LDS refused: %s", lds,
                 hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((attend_tile_kernel<T, DC, WHOLE>), dim3(tp.pairs * tp.tiles), dim3(kThreads),
-                     lds, stream, tp);
+  hipLaunchKernelGGL((attend_tile_kernel<T, DC, WHOLE, kKeys, kWaves, kStages>), dim3(tp.pairs * tp.tiles),
+                     dim3(kWaves * kWave), lds, stream, tp);
   return launch_status("routed_attention");
 }
 
+// Tiles and waves of a workgroup, by what was measured (us, 4 x 4096 queries of 12 heads on 4 of 64
+// features / 8192 of 16 on 2 of 128; two tiles in LDS, with 128 registers to a lane):
+//   keys x waves   64 x 8: 135 / 153   64 x 4: 115 / 277 (two workgroups per CU only)
+//                  32 x 8:   - / 161   32 x 4: 124 / 131   32 x 2: 126 / 173
+// Fewer waves share a tile's loads with fewer queries but wait for fewer of them: what counts is
+// the number of workgroups on a CU (four).  One tile in LDS (seven fit) 120 / 144: registers
+// still allow only four.  Three in LDS (two or three workgroups) 179 / 207.
 template <typename T, bool WHOLE>
 hipError_t launch_type(TileParams& tp, hipStream_t stream) {
   const int dc = (tp.p.D + 31) / 32;
-  if (dc <= 1) return launch<T, 1, WHOLE>(tp, stream);
-  if (dc <= 2) return launch<T, 2, WHOLE>(tp, stream);
-  if (dc <= 3) return launch<T, 3, WHOLE>(tp, stream);
-  if (dc <= 4) return launch<T, 4, WHOLE>(tp, stream);
-  return launch<T, 8, WHOLE>(tp, stream);
+  if (dc <= 1) return launch<T, 1, WHOLE, 64, 4, 2>(tp, stream);
+  if (dc <= 2) return launch<T, 2, WHOLE, 64, 4, 2>(tp, stream);
+  if (dc <= 3) return launch<T, 3, WHOLE, 32, 4, 2>(tp, stream);
+  if (dc <= 4) return launch<T, 4, WHOLE, 32, 4, 2>(tp, stream);
+  return launch<T, 8, WHOLE, 32, 4, 2>(tp, stream);
 }
 
 }  // namespace
@@ -544,7 +594,7 @@ hipError_t launch_type(TileParams& tp, hipStream_t stream) {
 namespace attention {
 
 bool tile_fits(const Params& p, int dtype) {
-  const int64_t limit = (int64_t(1) << 31) / (2 * kKeys) - 1;  // bytes of a tile's rows
+  const int64_t limit = (int64_t(1) << 31) / (2 * kMostKeys) - 1;  // a tile below 2 GiB
   return (dtype == RLM_BF16 || dtype == RLM_F16) && !p.ring && p.Tq > 1 && p.T >= 1 &&
          p.BS % 4 == 0 && p.k_st < limit && p.v_st < limit &&
          static_cast<int64_t>(p.B) * p.Hk * ((p.G + 15) / 16) * p.Tq < (int64_t(1) << 31);
@@ -554,9 +604,10 @@ hipError_t tile_launch(Params& p, int dtype, hipStream_t stream) {
   TileParams tp{};
   tp.p = p;
   tp.negate = p.scale_log2 < 0.0f;
+  tp.far = 2 * p.T * std::max(p.k_st, p.v_st) >= (int64_t(1) << 31) - 4096;
   // A scale of 0 as the smallest number: scores of 0 for the keys, -inf for the masked.
   tp.c = std::max(std::fabs(p.scale_log2), 1e-37f);
-  if (p.BS % kKeys == 0)
+  if (p.BS % kMostKeys == 0)
     return dtype == RLM_BF16 ? launch_type<bf16, true>(tp, stream)
                              : launch_type<f16, true>(tp, stream);
   return dtype == RLM_BF16 ? launch_type<bf16, false>(tp, stream)
