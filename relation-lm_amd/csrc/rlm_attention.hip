@@ -7,203 +7,8 @@
 // A position counts once whichever way it is named; a query that sees none gives 0 and -inf.
 #include "rlm_attention.hpp"
 
-namespace rlm {
-namespace {
-
-using namespace attention;
-
-// ---------------------------------------------------------------------------
-// Up to 16 heads of one query to a wave, fp32 products
-// ---------------------------------------------------------------------------
-//
-// v_mfma_f32_16x16x4_f32 with the keys as rows and the heads as columns, so a lane holds four
-// keys' scores of one head, which are the second product's operand as they stand:
-//   S^T[key, head]  : lane (head = l % 16, keys 4 (l / 16) + i)
-//   O^T[dim, head] += V^T[dim, key] P^T[key, head], four keys (one of each lane group) a step.
-// The features are summed in an order that gives a lane four neighbouring ones of a key's row
-// (one wide load).  One query's heads share its keys, so a masked key is masked for the whole
-// wave; a lane of a masked key reads a key of the same run that is not.
-template <typename T, int DT>
-__global__ __launch_bounds__(512) void attend_query_kernel(Params p) {
-  extern __shared__ __align__(16) float merge[];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int r = lane & 15, quad = lane >> 4;
-  const int W = p.waves_per_item;
-  const uint32_t item = W == 1 ? blockIdx.x * (blockDim.x / kWave) + wave : blockIdx.x;
-  const int share = W == 1 ? 0 : wave;
-  if (item >= p.items) return;  // W == 1 alone: no barrier follows
-  uint32_t chunk, hk, step;
-  const uint32_t b = p.by_queries.div(p.by_kv.div(p.by_chunks.div(item, chunk), hk), step);
-  const int head_in_group = static_cast<int>(chunk) * 16 + r;
-  const bool head_ok = head_in_group < p.G;
-  const int head = static_cast<int>(hk) * p.G + (head_ok ? head_in_group : 0);
-  const int D = p.D;
-
-  float qf[DT][4];
-  {
-    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + step * p.q_st + head * p.q_sh;
-#pragma unroll
-    for (int j = 0; j < DT; ++j) {
-      const int d = 16 * j + 4 * quad;
-      const float4 x = load4(src + (d < D ? d : 0));
-      const bool ok = d < D && head_ok;
-      qf[j][0] = ok ? x.x : 0.0f;
-      qf[j][1] = ok ? x.y : 0.0f;
-      qf[j][2] = ok ? x.z : 0.0f;
-      qf[j][3] = ok ? x.w : 0.0f;
-    }
-  }
-  const int64_t t = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_sq);
-  const int32_t* picks = p.blocks + b * p.blk_sb + step * p.blk_st + hk * p.blk_sh;
-  const int32_t mine = lane < p.TOP ? picks[lane] : -1;
-  // Positions seen: [low, high), of which [start, high) are the window's.
-  const int64_t high = p.ring ? t + 1 : (t + 1 < p.T ? t + 1 : p.T);
-  const int64_t low = p.ring && t + 1 > p.T ? t + 1 - p.T : 0;
-  int64_t start = t - p.local_window + 1;
-  start = start > low ? start : low;
-  const int64_t near = high > start ? high - start : 0;
-  const uint32_t near_tiles = static_cast<uint32_t>((near + 15) / 16);
-  const uint32_t tiles = near_tiles + p.TOP * p.by_block_tiles.d;
-
-  const T* kbase = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
-  const T* vbase = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
-  f32x4 acc[DT] = {};
-  float m = -INFINITY, l = 0.0f;
-
-  for (uint32_t tile = share; tile < tiles; tile += W) {
-    int64_t first, end;  // this tile's positions [first, end), at most 16
-    if (tile < near_tiles) {
-      first = start + 16 * static_cast<int64_t>(tile);
-      end = first + 16 < high ? first + 16 : high;
-    } else {
-      uint32_t part;
-      const int pick = static_cast<int>(p.by_block_tiles.div(tile - near_tiles, part));
-      const int32_t block = __builtin_amdgcn_readlane(mine, pick);
-      const uint64_t same = __builtin_amdgcn_ballot_w64(mine == block);
-      if (block < 0 || (same & ((uint64_t(1) << pick) - 1)) != 0) continue;
-      first = block * p.BS;
-      end = first + p.BS < start ? first + p.BS : start;
-      end = end < high ? end : high;
-      first += 16 * static_cast<int64_t>(part);
-      end = first + 16 < end ? first + 16 : end;
-      first = first > low ? first : low;
-    }
-    if (first >= end) continue;
-    const int count = static_cast<int>(end - first);
-    const int64_t row0 = p.ring ? (first & (p.T - 1)) : first;
-    auto row_of = [&](int i) {
-      const int64_t row = row0 + (i < count ? i : 0);
-      return p.ring && row >= p.T ? row - p.T : row;
-    };
-    const T* krow = kbase + row_of(r) * p.k_st;
-    f32x4 s = {};
-#pragma unroll
-    for (int j = 0; j < DT; ++j) {
-      const int d = 16 * j + 4 * quad;
-      const float4 x = load4(krow + (d < D ? d : 0));  // past D: the query's features are 0 ...
-      const bool ok = d < D;                           // ... and so is the key's, whatever it holds
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(ok ? x.x : 0.0f, qf[j][0], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(ok ? x.y : 0.0f, qf[j][1], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(ok ? x.z : 0.0f, qf[j][2], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(ok ? x.w : 0.0f, qf[j][3], s, 0, 0, 0);
-    }
-    float x[4], top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = 4 * quad + i < count ? s[i] * p.scale_log2 : -INFINITY;
-      top = fmaxf(top, x[i]);
-    }
-    top = fmaxf(m, rows_max(top));
-    const float base = top == -INFINITY ? 0.0f : top;
-    const float fade = __builtin_amdgcn_exp2f(m - base);
-    m = top;
-    l *= fade;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = __builtin_amdgcn_exp2f(x[i] - base);
-      l += x[i];
-    }
-#pragma unroll
-    for (int j = 0; j < DT; ++j) {
-      acc[j] *= fade;
-      const int d = 16 * j + r;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v = to_f32(vbase[row_of(4 * quad + i) * p.v_st + (d < D ? d : 0)]);
-        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[i], acc[j], 0, 0, 0);
-      }
-    }
-  }
-  l = rows_sum(l);
-
-  if (W > 1) {
-    // The waves' sums into the first wave's, in the waves' order.
-    constexpr int kFloats = 4 * DT + 2;
-    if (wave != 0) {
-      float* to = merge + (wave - 1) * kFloats * kWave + lane;
-#pragma unroll
-      for (int j = 0; j < DT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to[(4 * j + i) * kWave] = acc[j][i];
-      to[4 * DT * kWave] = m;
-      to[(4 * DT + 1) * kWave] = l;
-    }
-    __syncthreads();
-    if (wave != 0) return;
-    for (int w = 1; w < W; ++w) {
-      const float* from = merge + (w - 1) * kFloats * kWave + lane;
-      const float mw = from[4 * DT * kWave], lw = from[(4 * DT + 1) * kWave];
-      const float top = fmaxf(m, mw), base = top == -INFINITY ? 0.0f : top;
-      const float a = __builtin_amdgcn_exp2f(m - base), c = __builtin_amdgcn_exp2f(mw - base);
-      m = top;
-      l = l * a + lw * c;
-#pragma unroll
-      for (int j = 0; j < DT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          acc[j][i] = acc[j][i] * a + from[(4 * j + i) * kWave] * c;
-    }
-  }
-  if (!head_ok) return;
-  const int64_t row = (static_cast<int64_t>(b) * p.Tq + step) * p.Hq + head;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(p.out) + row * D;
-#pragma unroll
-  for (int j = 0; j < DT; ++j) {
-    const int d = 16 * j + 4 * quad;
-    if (d < D) put4<T>(out + d, acc[j][0] * inv, acc[j][1] * inv, acc[j][2] * inv, acc[j][3] * inv);
-  }
-  if (quad == 0) p.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
-}
-
-template <typename T, int DT>
-hipError_t launch_query(Params& p, hipStream_t stream) {
-  // Waves of an item: one where the items alone fill the chip.
-  const int64_t seen = p.local_window + static_cast<int64_t>(p.TOP) * p.BS;
-  const int64_t tiles = (seen + 15) / 16;
-  int waves = p.items >= 4096 ? 1 : p.items >= 1024 ? 4 : 8;
-  if (waves > tiles) waves = static_cast<int>(tiles > 4 ? 4 : 1);
-  p.waves_per_item = waves;
-  const size_t lds = waves > 1 ? sizeof(float) * (waves - 1) * (4 * DT + 2) * kWave : 0;
-  const unsigned grid = waves > 1 ? p.items : (p.items + 3) / 4;
-  hipLaunchKernelGGL((attend_query_kernel<T, DT>), dim3(grid),
-                     dim3(kWave * (waves > 1 ? waves : 4)), lds, stream, p);
-  return launch_status("routed_attention");
-}
-
-template <typename T>
-hipError_t launch_type(Params& p, hipStream_t stream) {
-  if (p.D <= 32) return launch_query<T, 2>(p, stream);
-  if (p.D <= 64) return launch_query<T, 4>(p, stream);
-  if (p.D <= 96) return launch_query<T, 6>(p, stream);
-  if (p.D <= 128) return launch_query<T, 8>(p, stream);
-  return launch_query<T, 16>(p, stream);
-}
-
-}  // namespace
-}  // namespace rlm
-
 using namespace rlm;
+using namespace rlm::attention;
 
 extern "C" hipError_t rlm_routed_attention(
     const rlm_tensor* query, const rlm_tensor* key_cache, const rlm_tensor* value_cache,
@@ -290,6 +95,7 @@ extern "C" hipError_t rlm_routed_attention(
   p.TOP = static_cast<int>(TOP);
   p.ring = ring != 0;
   p.head_chunks = (p.G + 15) / 16;
+  p.heads_per_chunk = (p.G + p.head_chunks - 1) / p.head_chunks;
   RLM_REQUIRE(B * Tq * Hk * p.head_chunks < (int64_t(1) << 31),
               "at most 2^31 - 1 (query, key head, 16 query heads) items");
   p.items = static_cast<uint32_t>(B * Tq * Hk * p.head_chunks);
@@ -299,11 +105,7 @@ extern "C" hipError_t rlm_routed_attention(
   p.by_chunks = FastDiv(static_cast<uint32_t>(p.head_chunks));
   p.by_kv = FastDiv(static_cast<uint32_t>(Hk));
   p.by_queries = FastDiv(static_cast<uint32_t>(Tq));
-  p.by_block_tiles = FastDiv(static_cast<uint32_t>((block_size + 15) / 16));
-  if (tile_fits(p, query->dtype)) return tile_launch(p, query->dtype, stream);
-  switch (query->dtype) {
-    case RLM_F32: return launch_type<float>(p, stream);
-    case RLM_BF16: return launch_type<bf16>(p, stream);
-    default: return launch_type<f16>(p, stream);
-  }
+  p.by_block = FastDiv(static_cast<uint32_t>(block_size));
+  return tile_fits(p, query->dtype) ? tile_launch(p, query->dtype, stream)
+                                    : query_launch(p, query->dtype, stream);
 }

@@ -27,10 +27,10 @@ struct Params {
   int64_t T, BS, local_window;
   float scale_log2;        // scale * log2(e): scores are kept in powers of two
   int B, Tq, Hq, Hk, G, D, TOP;
-  int head_chunks;         // of at most 16 query heads
-  int waves_per_item;
+  int head_chunks;         // of a key head's query heads, at most 16 each
+  int heads_per_chunk;
   uint32_t items;          // B * Tq * Hk * head_chunks
-  FastDiv by_chunks, by_kv, by_queries, by_block_tiles;
+  FastDiv by_chunks, by_kv, by_queries, by_block;
   bool ring;
 };
 
@@ -42,6 +42,8 @@ __device__ __forceinline__ float rows_max(float v) {
 }
 __device__ __forceinline__ float rows_sum(float v) { return swap32_sum(swap16_sum(v)); }
 
+// One query to a workgroup (rlm_attention_query.hip).
+hipError_t query_launch(const Params& p, int dtype, hipStream_t stream);
 // Kernels of 64-key tiles shared by up to 128 rows (16-bit types; rlm_attention_tile.hip).
 bool tile_fits(const Params& p, int dtype);
 hipError_t tile_launch(Params& p, int dtype, hipStream_t stream);

@@ -25,19 +25,12 @@
 #include <type_traits>
 
 #include "rlm_attention.hpp"
+#include "rlm_attention_mfma.hpp"
 
 namespace rlm {
 namespace {
 
 using namespace attention;
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-typedef const __attribute__((address_space(3))) s16x8* lds_s16x8;
 
 constexpr int kRows = 16;           // rows of a wave
 constexpr int kMostKeys = 64;       // keys of the largest tile
@@ -59,42 +52,11 @@ struct TileParams {
   bool far;              // rows of a key head reach over 2 GiB: offsets from each tile's first
 };
 
-__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, bf16) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, f16) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
-                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, bf16) { return pack_bf16x2(lo, hi); }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, f16) {
-  typedef float f32x2_t __attribute__((ext_vector_type(2)));
-  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-  const f32x2_t v = {lo, hi};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
-}
-
 // A workgroup barrier that orders LDS reads and leaves loads into LDS outstanding.
 __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
-// 16-byte pieces of an LDS row: rows of 8 pieces alternate between the halves of the 16 piece
-// columns that the banks form, so their swizzle goes by pairs of rows.
-template <int PITCH>
-__device__ __forceinline__ int swizzle(int row) {
-  return PITCH == 8 ? (row >> 1) & 7 : row & 15;
-}
-
-// Lane l reads four values of key l / 16 * 4 + l % 16 / 4 at `at` and gets four keys of value
-// feature l % 16; eight keys, of the two 16-key groups `apart` bytes from each other.
-__device__ __forceinline__ s16x8 read_values(uint32_t at, uint32_t apart) {
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + apart));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // One row from the positions that it sees alone, a position at a time: lanes hold features.
@@ -427,7 +389,7 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
         s[kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < DC; ++j)
-          s[kt] = mfma(*(lds_s16x8)((key0 ^ (64u * j)) + 16 * kt * kRow), qf[j], s[kt], T{});
+          s[kt] = product(*(lds_s16x8)static_cast<uintptr_t>((key0 ^ (64u * j)) + 16 * kt * kRow), qf[j], s[kt], T{});
       }
       // The first values of the second product, on their way while the weights are computed:
       // step i is 32-key half i / DT and feature group i % DT.
@@ -502,7 +464,7 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
       // O^T += V^T P^T.
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        acc[i % DT] = mfma(vf[i % kAhead], __builtin_bit_cast(s16x8, weights[i / DT]), acc[i % DT],
+        acc[i % DT] = product(vf[i % kAhead], __builtin_bit_cast(s16x8, weights[i / DT]), acc[i % DT],
                            T{});
         if (i + kAhead < kSteps) vf[i % kAhead] = values(i + kAhead);
       }
