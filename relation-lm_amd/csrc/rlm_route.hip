@@ -73,8 +73,60 @@ __device__ __forceinline__ void insert_keys(uint64_t& list, uint64_t key, int to
   }
 }
 
+// exp(x) for x <= 0 to 1e-11, NaN for NaN: x = k ln 2 + r with |r| <= ln 2 / 2, the Taylor
+// polynomial of degree 9 in r (its remainder is r^10 / 10! < 7e-12).  A score is rounded to fp32
+// (6e-8) once; two blocks with equal inputs run the same steps and tie.
+__device__ __forceinline__ double exp_down(double x) {
+  x = x < -700.0 ? -700.0 : x;  // 1e-304: nothing beside a sum of at least 1
+  const double k = rint(x * 1.44269504088896340736);
+  double r = fma(k, -6.93147180369123816490e-01, x);  // ln 2: 33 bits, and the rest
+  r = fma(k, -1.90821492927058770002e-10, r);
+  double y = 1.0 / 362880.0;
+  y = fma(y, r, 1.0 / 40320.0);
+  y = fma(y, r, 1.0 / 5040.0);
+  y = fma(y, r, 1.0 / 720.0);
+  y = fma(y, r, 1.0 / 120.0);
+  y = fma(y, r, 1.0 / 24.0);
+  y = fma(y, r, 1.0 / 6.0);
+  y = fma(y, r, 0.5);
+  y = fma(y, r, 1.0);
+  y = fma(y, r, 1.0);
+  return ldexp(y, static_cast<int>(k));
+}
+// log(s) for s >= 1: the fp32 logarithm y, corrected by log(s exp(-y)) = z - z^2 / 2 + O(z^3),
+// |z| <= 1e-6.
+__device__ __forceinline__ double log_up(double s) {
+  const double y = static_cast<double>(__builtin_amdgcn_logf(static_cast<float>(s)) * 0.69314718055994530942f);
+  const double z = fma(s, exp_down(-y), -1.0);
+  return y + fma(z * z, -0.5, z);
+}
+
+// Maximum over the lanes whose number leaves the same remainder by 4 (P = 4), or over all of
+// the wave (P = 1), in each of them.
+template <int P>
+__device__ __forceinline__ uint64_t part_max(uint64_t v) {
+  if constexpr (P == 1) {
+    v = umax64(v, dpp_u64<kDppXor1>(v));
+    v = umax64(v, dpp_u64<kDppXor2>(v));
+  }
+  v = umax64(v, dpp_u64<0x124>(v));  // row_ror:4, row_ror:8
+  v = umax64(v, dpp_u64<0x128>(v));
+  auto lo = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(v), static_cast<uint32_t>(v),
+                                             false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(v >> 32),
+                                             static_cast<uint32_t>(v >> 32), false, false);
+  v = umax64(static_cast<uint64_t>(lo[0]) | (static_cast<uint64_t>(hi[0]) << 32),
+             static_cast<uint64_t>(lo[1]) | (static_cast<uint64_t>(hi[1]) << 32));
+  lo = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(v), static_cast<uint32_t>(v), false,
+                                        false);
+  hi = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(v >> 32),
+                                        static_cast<uint32_t>(v >> 32), false, false);
+  return umax64(static_cast<uint64_t>(lo[0]) | (static_cast<uint64_t>(hi[0]) << 32),
+                static_cast<uint64_t>(lo[1]) | (static_cast<uint64_t>(hi[1]) << 32));
+}
+
 template <typename TQ, int P, int Q, bool SPLIT>
-__global__ __launch_bounds__(SPLIT ? 1024 : 256) void route_kernel(RouteParams p) {
+__global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParams p) {
   extern __shared__ __align__(16) double lds[];
   constexpr int kPer = (Q + P - 1) / P;  // queries whose exponentials a lane carries on
   constexpr int kBlocks = kWave / P;
@@ -91,6 +143,9 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256) void route_kernel(RouteParams p
   if (!live) group = p.groups - 1;
   uint32_t in_batch;
   const uint32_t b = p.by_groups.div(group, in_batch);
+  // Later positions have more blocks: every other batch row runs from the end, so that a CU's
+  // workgroups (whole rounds of the grid apart) are not all long ones.
+  if (!SPLIT && (b & 1)) in_batch = p.groups_per_batch - 1 - in_batch;
   const uint32_t row0 = in_batch * Q;
 
   for (int i = threadIdx.x; i < p.H; i += blockDim.x)
@@ -138,11 +193,41 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256) void route_kernel(RouteParams p
   const int slots = static_cast<int>(complete < p.NB ? complete : p.NB);
   const bool short_list = p.TOP <= 16;
   uint64_t list[Q] = {};
+  // Four queries, four lanes to a block: the first 64 blocks' keys wait in registers (a lane has
+  // its own query's), and the lists start from their TOP largest, found for the four queries
+  // at once.  Blocks after those enter one by one where they pass the list's last.
+  constexpr bool kFirst = Q == 4 && P == 4;
+  uint64_t waiting[kFirst ? P : 1] = {};
+  auto start_lists = [&]() {
+    if constexpr (kFirst) {
+      for (int rank = 0; rank < p.TOP; ++rank) {
+        const uint64_t best = part_max<P>(
+            umax64(umax64(waiting[0], waiting[1]), umax64(waiting[2], waiting[3])));
+#pragma unroll
+        for (int i = 0; i < P; ++i) waiting[i] = waiting[i] == best ? 0 : waiting[i];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          const uint64_t x = lane_u64(best, i);
+          list[i] = lane == rank ? x : list[i];
+        }
+      }
+    }
+  };
 
+  // This lane's statistics of the block that it has in the pass from j0 on (the last block's
+  // past the end).
+  auto block_at = [&](int j0) {
+    return (static_cast<int64_t>(b) * p.NB + min(j0 + in_wave, p.NB - 1)) * RD + 4 * part;
+  };
+  float4 m, s4;
+  {
+    const int64_t at = block_at((SPLIT ? wave : 0) * kBlocks);
+    m = *reinterpret_cast<const float4*>(p.mean + at);
+    s4 = *reinterpret_cast<const float4*>(p.std + at);
+  }
   for (int j0 = (SPLIT ? wave : 0) * kBlocks; j0 < slots; j0 += (SPLIT ? waves : 1) * kBlocks) {
     const int j = j0 + in_wave;
-    const int64_t at = (static_cast<int64_t>(b) * p.NB + min(j, p.NB - 1)) * RD + 4 * part;
-    const float *mean = p.mean + at, *std = p.std + at;
+    const int64_t at = block_at(j0), next_at = block_at(j0 + (SPLIT ? waves : 1) * kBlocks);
     int64_t block[kPer];
     int bucket[kPer];
     bool ok[kPer];
@@ -156,15 +241,17 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256) void route_kernel(RouteParams p
       const int64_t away = mine[k] > end ? mine[k] - end : 0;
       const int log2 = 63 - __builtin_clzll(static_cast<uint64_t>(away + 1));
       bucket[k] = log2 < p.RB ? log2 : p.RB - 1;
-      most[k] = -INFINITY;
-      sum[k] = 0.0;
+      most[k] = sum[k] = 0.0;
     }
     for (int h = 0; h < p.H; ++h) {
       double like[Q] = {}, wide[Q] = {};
       for (int d = 0; d < p.HD; d += 4 * P) {
-        const float4 m = *reinterpret_cast<const float4*>(mean + h * p.HD + d);
-        const float4 s = *reinterpret_cast<const float4*>(std + h * p.HD + d);
-        const double md[4] = {m.x, m.y, m.z, m.w}, sd[4] = {s.x, s.y, s.z, s.w};
+        const double md[4] = {m.x, m.y, m.z, m.w}, sd[4] = {s4.x, s4.y, s4.z, s4.w};
+        // The next features of this block, or the first of the next.
+        const int after = h * p.HD + d + 4 * P;
+        const int64_t load = after < RD ? at + after : next_at;
+        m = *reinterpret_cast<const float4*>(p.mean + load);
+        s4 = *reinterpret_cast<const float4*>(p.std + load);
         const double* qd = q + h * p.HD + d + 4 * part;
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
@@ -187,22 +274,34 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256) void route_kernel(RouteParams p
         for (int i = 0; i < Q; ++i)
           if (i == k * P + part) x = s[i];
         x += bias[h * p.RB + bucket[k]];
-        const double e = exp(-fabs(x - most[k]));
-        sum[k] = x > most[k] ? fma(sum[k], e, 1.0) : sum[k] + e;
-        most[k] = x > most[k] ? x : most[k];
+        if (h == 0) {
+          most[k] = x;
+          sum[k] = 1.0;
+        } else {
+          const double e = exp_down(-fabs(x - most[k]));
+          sum[k] = x > most[k] ? fma(sum[k], e, 1.0) : sum[k] + e;
+          most[k] = x > most[k] ? x : most[k];
+        }
       }
     }
     uint64_t key[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const float score = static_cast<float>(most[k] + log(sum[k]));
+      const float score = static_cast<float>(most[k] + log_up(sum[k]));
       key[k] = ok[k] && score > -1.0e30f
                    ? select_key(score, static_cast<uint32_t>(block[k] - lowest[k]))
                    : 0;
     }
+    if (kFirst && j0 < kWave) {
 #pragma unroll
-    for (int i = 0; i < Q; ++i)
-      insert_keys(list[i], part == i % P ? key[i / P] : 0, p.TOP, short_list);
+      for (int i = 0; i < P; ++i)
+        if (j0 == i * kBlocks) waiting[kFirst ? i : 0] = key[0];
+      if (j0 + kBlocks >= slots || j0 + kBlocks == kWave) start_lists();
+    } else {
+#pragma unroll
+      for (int i = 0; i < Q; ++i)
+        insert_keys(list[i], part == i % P ? key[i / P] : 0, p.TOP, short_list);
+    }
   }
 
   if constexpr (SPLIT) {
