@@ -15,6 +15,14 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 typedef const __attribute__((address_space(3))) s16x8* lds_s16x8;
+typedef const __attribute__((address_space(3))) float* lds_f32;
+
+// 16-byte pieces of an LDS row of at most 32 DC features: a power of two, 8 at least.
+template <typename T, int DC>
+constexpr int pitch() {
+  constexpr int pieces = DC * 32 * static_cast<int>(sizeof(T)) / 16;
+  return pieces <= 8 ? 8 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : 64;
+}
 
 // c + a b over 32 (16-bit types) or 16 (fp32: four steps of four) features or keys.
 __device__ __forceinline__ f32x4 product(s16x8 a, s16x8 b, f32x4 c, bf16) {

@@ -33,7 +33,7 @@ constexpr bool kIs32 = sizeof(T) == 4;
 template <typename T, int DC, int MAXW>
 __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
   constexpr int DT = 2 * DC;                               // head dim in 16s
-  constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;  // 16-byte pieces of an LDS row
+  constexpr int kPitch = pitch<T, DC>();                   // 16-byte pieces of an LDS row
   constexpr int kRow = 16 * kPitch;
   extern __shared__ __align__(1024) char lds[];
   const int lane = threadIdx.x & (kWave - 1);
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
 template <typename T, int DC, int MAXW>
 hipError_t launch(const Params& p, hipStream_t stream) {
   constexpr int DT = 2 * DC;
-  constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;
+  constexpr int kPitch = pitch<T, DC>();
   // Waves of a query: enough to fill the chip, and one tile each at least.
   const int64_t tiles = (p.local_window + p.TOP * p.BS + kKeys - 1) / kKeys;
   int waves = 1;

@@ -1,5 +1,5 @@
-// Attention over a window and picked blocks for many queries of 16-bit types: key tiles shared
-// by the rows of a workgroup.
+// Attention over a window and picked blocks for many queries: key tiles shared by the rows of a
+// workgroup.
 //
 // A workgroup holds 4 waves of 16 rows, a row being one query head of one query; the rows of a
 // wave are whole queries with the heads of one key head, consecutive positions of the sequence.  It walks the 64-key tiles that any of its queries sees -- its windows' and its
@@ -126,7 +126,8 @@ template <typename T, int DC, bool WHOLE, int kKeys, int kWaves, int kStages>
 __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_kernel(TileParams tp) {
   constexpr int kThreads = kWaves * kWave;
   constexpr int KT = kKeys / 16;                           // 16-key groups of a tile
-  constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;  // 16-byte pieces of an LDS row
+  constexpr bool k32 = sizeof(T) == 4;
+  constexpr int kPitch = pitch<T, DC>();                   // 16-byte pieces of an LDS row
   constexpr int kRow = 16 * kPitch;                        // bytes
   constexpr int kTile = kKeys * kRow;                      // bytes of a key (or value) tile
   constexpr int kDma = kPitch * kKeys / kThreads;          // DMA instructions of a wave per tile
@@ -181,17 +182,20 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
   const int head = static_cast<int>(hk) * p.G + (row_ok ? h : 0);
   const int step = row_ok ? q : 0;
   const int bit = (row_ok ? static_cast<int>(in_wave) : 0) + 16 * (wave & 1);
-  s16x8 qf[DC];
+  typedef typename std::conditional<k32, float4, s16x8>::type frag_t;
+  constexpr int kFrags = k32 ? DT : DC;     // 16-byte pieces of a row that a lane has,
+  constexpr int kFeatures = k32 ? 4 : 8;    // of so many features: pieces 4 j + quad
+  frag_t qf[kFrags];
   {
     const T* src = static_cast<const T*>(p.q) + b * p.q_sb + step * p.q_st + head * p.q_sh;
-    const uint32_t flip = tp.negate ? 0x80008000u : 0u;
+    const uint32_t flip = !tp.negate ? 0u : k32 ? 0x80000000u : 0x80008000u;
 #pragma unroll
-    for (int j = 0; j < DC; ++j) {
-      const int d = 32 * j + 8 * quad;
+    for (int j = 0; j < kFrags; ++j) {
+      const int d = kFeatures * (4 * j + quad);
       uint4 x = *reinterpret_cast<const uint4*>(src + (d < p.D ? d : 0));
       x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
       if (!(d < p.D && row_ok)) x = make_uint4(0, 0, 0, 0);
-      qf[j] = __builtin_bit_cast(s16x8, x);
+      qf[j] = __builtin_bit_cast(frag_t, x);
     }
   }
   __syncthreads();
@@ -213,8 +217,8 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
   // This lane's pieces of a tile: row and byte in the row, which the swizzle permutes; pieces
   // past the head dim come as zeros.
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
-  const uint32_t k_bytes = static_cast<uint32_t>(p.k_st) * 2u;
-  const uint32_t v_bytes = static_cast<uint32_t>(p.v_st) * 2u;
+  const uint32_t k_bytes = static_cast<uint32_t>(p.k_st * sizeof(T));
+  const uint32_t v_bytes = static_cast<uint32_t>(p.v_st * sizeof(T));
   uint32_t k_off[kDma], v_off[kDma];
   auto dma_row = [&](int k) {
     return static_cast<uint32_t>(((wave * kDma + k) * kWave + lane) / kPitch);
@@ -223,7 +227,7 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
   for (int k = 0; k < kDma; ++k) {
     const uint32_t row = dma_row(k);
     const int from = (lane % kPitch) ^ swizzle<kPitch>(row);
-    const bool ok = 8 * from < p.D;
+    const bool ok = kFeatures * from < p.D;
     k_off[k] = ok ? row * k_bytes + 16u * from : kNoOffset;
     v_off[k] = ok ? row * v_bytes + 16u * from : kNoOffset;
   }
@@ -368,9 +372,6 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
       // later ones an exclusive or away (pieces 4 j + quad of the keys, 2 j + (0 or 1) of the
       // values).
       const uint32_t key0 = tile0 + r * kRow + ((quad ^ swizzle<kPitch>(r)) << 4);
-      const int vrow = 4 * quad + (r >> 2);
-      const uint32_t value0 = tile0 + kTile + vrow * kRow +
-                              ((((r & 3) >> 1) ^ swizzle<kPitch>(vrow)) << 4) + (r & 1) * 8;
       // Whether the row picked the block of this lane's four keys of 16-key group kt.
       constexpr int kPicked = WHOLE ? 1 : KT;
       bool pick[kPicked];
@@ -388,19 +389,26 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
       for (int kt = 0; kt < KT; ++kt) {
         s[kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < DC; ++j)
-          s[kt] = product(*(lds_s16x8)static_cast<uintptr_t>((key0 ^ (64u * j)) + 16 * kt * kRow), qf[j], s[kt], T{});
+        for (int j = 0; j < kFrags; ++j) {
+          const s16x8 kf = *(lds_s16x8)static_cast<uintptr_t>((key0 ^ (64u * j)) + 16 * kt * kRow);
+          s[kt] = product(__builtin_bit_cast(frag_t, kf), qf[j], s[kt], T{});
+        }
       }
-      // The first values of the second product, on their way while the weights are computed:
-      // step i is 32-key half i / DT and feature group i % DT.
+      // 16-bit values: step i of the second product is 32-key half i / DT and feature group
+      // i % DT; the first steps' operands come while the weights are computed.
       constexpr int kAhead = 4, kSteps = DT * KT / 2;
+      const int vrow = 4 * quad + (r >> 2);
+      const uint32_t value0 = tile0 + kTile + vrow * kRow +
+                              ((((r & 3) >> 1) ^ swizzle<kPitch>(vrow)) << 4) + (r & 1) * 8;
       auto values = [&](int i) {
         return read_values((value0 ^ (32u * (i % DT))) + i / DT * 32 * kRow, 16 * kRow);
       };
       s16x8 vf[kAhead];
+      if constexpr (!k32) {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (i < kSteps) vf[i] = values(i);
+        for (int i = 0; i < kAhead; ++i)
+          if (i < kSteps) vf[i] = values(i);
+      }
       __builtin_amdgcn_sched_barrier(0);
 
       // The weights, as the second product's operand: two 16-key groups to each.
@@ -419,6 +427,7 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
       bool up = __builtin_amdgcn_ballot_w64((m == -INFINITY) & (((see >> bit) & 1) != 0) &
                                             row_ok) != 0;
       uint4 weights[KT / 2];
+      float w32[k32 ? KT : 1][4];
       for (int pass = 0;; ++pass) {
         if (up) {
           float top = -INFINITY;
@@ -446,13 +455,18 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
           for (int i = 0; i < 4; ++i) {
             w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], tp.c, shift));
             sum[i] = kt == 0 ? w[i] : sum[i] + w[i];
+            if constexpr (k32) w32[kt][i] = w[i];
           }
-          half[2 * kt] = pack2(w[0], w[1], T{});
-          half[2 * kt + 1] = pack2(w[2], w[3], T{});
+          if constexpr (!k32) {
+            half[2 * kt] = pack2(w[0], w[1], T{});
+            half[2 * kt + 1] = pack2(w[2], w[3], T{});
+          }
         }
+        if constexpr (!k32) {
 #pragma unroll
-        for (int i = 0; i < KT / 2; ++i)
-          weights[i] = make_uint4(half[4 * i], half[4 * i + 1], half[4 * i + 2], half[4 * i + 3]);
+          for (int i = 0; i < KT / 2; ++i)
+            weights[i] = make_uint4(half[4 * i], half[4 * i + 1], half[4 * i + 2], half[4 * i + 3]);
+        }
         const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         up = pass == 0 && __builtin_amdgcn_ballot_w64(total > kLimit) != 0;
         if (!up) {
@@ -462,11 +476,27 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
       }
 
       // O^T += V^T P^T.
+      if constexpr (k32) {
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        acc[i % DT] = product(vf[i % kAhead], __builtin_bit_cast(s16x8, weights[i / DT]), acc[i % DT],
-                           T{});
-        if (i + kAhead < kSteps) vf[i % kAhead] = values(i + kAhead);
+        for (int i = 0; i < 4; ++i) {
+          const int key = 4 * quad + i;  // of each 16-key group; feature 16 j + r
+          const uint32_t at = tile0 + kTile + key * kRow + (((r >> 2) ^ swizzle<kPitch>(key)) << 4) +
+                              (r & 3) * 4;
+#pragma unroll
+          for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              const float v = *(lds_f32)static_cast<uintptr_t>((at ^ (64u * j)) + 16 * kt * kRow);
+              acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, w32[kt][i], acc[j], 0, 0, 0);
+            }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          acc[i % DT] = product(vf[i % kAhead], __builtin_bit_cast(s16x8, weights[i / DT]),
+                                acc[i % DT], T{});
+          if (i + kAhead < kSteps) vf[i % kAhead] = values(i + kAhead);
+        }
       }
     }
     __syncthreads();  // the lists and tiles have been read
@@ -520,8 +550,7 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
   tp.by_picks = FastDiv(static_cast<uint32_t>(p.TOP + 1));
   tp.by_wave_queries = FastDiv(static_cast<uint32_t>(tp.nqw));
   tp.by_block = FastDiv(static_cast<uint32_t>(p.BS));
-  constexpr int kPitch = DC <= 2 ? 8 : DC <= 4 ? 16 : 32;
-  const size_t lds = kStages * 2 * kKeys * 16 * kPitch;
+  const size_t lds = kStages * 2 * kKeys * 16 * pitch<T, DC>();
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
         reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, WHOLE, kKeys, kWaves, kStages>),
@@ -543,9 +572,10 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
 // still allow only four.  Three in LDS (two or three workgroups) 179 / 207.
 template <typename T, bool WHOLE>
 hipError_t launch_type(TileParams& tp, hipStream_t stream) {
+  constexpr int kSmall = sizeof(T) == 4 ? 32 : 64;
   const int dc = (tp.p.D + 31) / 32;
   if (dc <= 1) return launch<T, 1, WHOLE, 64, 4, 2>(tp, stream);
-  if (dc <= 2) return launch<T, 2, WHOLE, 64, 4, 2>(tp, stream);
+  if (dc <= 2) return launch<T, 2, WHOLE, kSmall, 4, 2>(tp, stream);
   if (dc <= 3) return launch<T, 3, WHOLE, 32, 4, 2>(tp, stream);
   if (dc <= 4) return launch<T, 4, WHOLE, 32, 4, 2>(tp, stream);
   return launch<T, 8, WHOLE, 32, 4, 2>(tp, stream);
@@ -556,9 +586,9 @@ hipError_t launch_type(TileParams& tp, hipStream_t stream) {
 namespace attention {
 
 bool tile_fits(const Params& p, int dtype) {
-  const int64_t limit = (int64_t(1) << 31) / (2 * kMostKeys) - 1;  // a tile below 2 GiB
-  return (dtype == RLM_BF16 || dtype == RLM_F16) && !p.ring && p.Tq > 1 && p.T >= 1 &&
-         p.BS % 4 == 0 && p.k_st < limit && p.v_st < limit &&
+  const int64_t limit =
+      (int64_t(1) << 31) / (dtype_size(dtype) * kMostKeys) - 1;  // a tile below 2 GiB
+  return !p.ring && p.Tq > 1 && p.T >= 1 && p.BS % 4 == 0 && p.k_st < limit && p.v_st < limit &&
          static_cast<int64_t>(p.B) * p.Hk * ((p.G + 15) / 16) * p.Tq < (int64_t(1) << 31);
 }
 
@@ -566,14 +596,16 @@ hipError_t tile_launch(Params& p, int dtype, hipStream_t stream) {
   TileParams tp{};
   tp.p = p;
   tp.negate = p.scale_log2 < 0.0f;
-  tp.far = 2 * p.T * std::max(p.k_st, p.v_st) >= (int64_t(1) << 31) - 4096;
+  tp.far = dtype_size(dtype) * p.T * std::max(p.k_st, p.v_st) >= (int64_t(1) << 31) - 4096;
   // A scale of 0 as the smallest number: scores of 0 for the keys, -inf for the masked.
   tp.c = std::max(std::fabs(p.scale_log2), 1e-37f);
-  if (p.BS % kMostKeys == 0)
-    return dtype == RLM_BF16 ? launch_type<bf16, true>(tp, stream)
-                             : launch_type<f16, true>(tp, stream);
-  return dtype == RLM_BF16 ? launch_type<bf16, false>(tp, stream)
-                           : launch_type<f16, false>(tp, stream);
+  const bool whole = p.BS % kMostKeys == 0;
+#define RLM_TILE_TYPE(T) \
+  return whole ? launch_type<T, true>(tp, stream) : launch_type<T, false>(tp, stream);
+  if (dtype == RLM_F32) RLM_TILE_TYPE(float)
+  if (dtype == RLM_BF16) RLM_TILE_TYPE(bf16)
+  RLM_TILE_TYPE(f16)
+#undef RLM_TILE_TYPE
 }
 
 }  // namespace attention

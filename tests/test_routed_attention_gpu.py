@@ -140,10 +140,12 @@ def test_unseen_rows_do_not_reach_the_output(device, bad, dtype):
     key[:, 60], value[:, 60] = bad, bad
     got = run_seq_raw(device, (query, key, value, positions, picks), 16, 8)
     others = (positions[0] < 60) | (positions[0] > 67)
-    half = torch.finfo(dtype).eps / 2
-    near = (got[0][:, others] - clean[0][:, others]).abs().float()
-    assert (near <= 4 * half * clean[0][:, others].abs().float() + 4 * half).all()
-    assert torch.allclose(got[1][:, others], clean[1][:, others], rtol=1e-5, atol=1e-5)
+    # (within the bound that the file states; a row with bad values among its neighbours' may be
+    # summed in another order than before)
+    expected = routed_layer.attention(host(query[:, others]), host(key), host(value),
+                                      picks[:, others].numpy(), positions[:, others].numpy(), 16, 8,
+                                      64 ** -0.5)
+    check(got[0][:, others], got[1][:, others], expected, dtype, 64)
     if bad != bad:
         assert torch.isnan(got[0][:, ~others]).all()
 
