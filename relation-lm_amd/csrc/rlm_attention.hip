@@ -106,6 +106,7 @@ extern "C" hipError_t rlm_routed_attention(
   p.by_kv = FastDiv(static_cast<uint32_t>(Hk));
   p.by_queries = FastDiv(static_cast<uint32_t>(Tq));
   p.by_block = FastDiv(static_cast<uint32_t>(block_size));
-  return tile_fits(p, query->dtype) ? tile_launch(p, query->dtype, stream)
-                                    : query_launch(p, query->dtype, stream);
+  return tile_fits(p, query->dtype) && tile_faster(p, query->dtype)
+             ? tile_launch(p, query->dtype, stream)
+             : query_launch(p, query->dtype, stream);
 }

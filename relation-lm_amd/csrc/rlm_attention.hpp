@@ -44,8 +44,9 @@ __device__ __forceinline__ float rows_sum(float v) { return swap32_sum(swap16_su
 
 // One query to a workgroup (rlm_attention_query.hip).
 hipError_t query_launch(const Params& p, int dtype, hipStream_t stream);
-// Kernels of 64-key tiles shared by up to 128 rows (16-bit types; rlm_attention_tile.hip).
+// Key tiles shared by the rows of a workgroup (rlm_attention_tile.hip).
 bool tile_fits(const Params& p, int dtype);
+bool tile_faster(const Params& p, int dtype);
 hipError_t tile_launch(Params& p, int dtype, hipStream_t stream);
 
 }  // namespace attention

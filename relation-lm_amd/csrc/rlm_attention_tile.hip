@@ -592,6 +592,34 @@ bool tile_fits(const Params& p, int dtype) {
          static_cast<int64_t>(p.B) * p.Hk * ((p.G + 15) / 16) * p.Tq < (int64_t(1) << 31);
 }
 
+// Whether the shared tiles are the faster kernel.  Both times (us) are modelled; measured, with
+// picks half of which 64 neighbouring queries share (batch, key heads, group, dim, rows, block,
+// window, picks; then queries: one query to a workgroup / shared tiles):
+//   bf16  1,4,3,64,4096,64,128,8     64: 9.5 / 33    512: 29 / 41    1024: 52 / 40
+//         1,2,8,128,8192,64,256,8    64: 13 / 55     512: 35 / 66    1024: 64 / 63
+//         8,4,4,128,4096,64,128,8    16: 22 / 65      64: 59 / 64     128: 106 / 63
+//         2,8,1,32,1024,16,32,8     256: 13 / 19     512: 20 / 16    1024: 34 / 12
+//         4,8,2,64,16384,64,256,16   64: 53 / 110    128: 111 / 104   256: 213 / 110
+//   fp32  1,4,3,64,4096,64,128,8    512: 73 / 149   1024: 137 / 141
+//         8,4,4,128,4096,64,128,8    64: 255 / 263   128: 468 / 271   512: 1358 / 649
+// One query: 8 us and its keys' products.  Tiles: a chain of the union of a workgroup's keys, which
+// grows with about the root of its queries, a step of about 1.1 us (fp32: the slower matrix
+// instructions) while the workgroups find room on the chip.
+bool tile_faster(const Params& p, int dtype) {
+  const bool is32 = dtype == RLM_F32;
+  const double keys = static_cast<double>(std::min<int64_t>(p.T, p.local_window + p.TOP * p.BS));
+  const double query = 8.0 + p.items * keys * p.D * (is32 ? 8.5e-7 : 2.7e-7);
+  const int chunks = (p.G + kRows - 1) / kRows, heads = (p.G + chunks - 1) / chunks;
+  const int queries = 4 * (kRows / heads);  // of a workgroup
+  const double tile_keys = p.D <= 32 || (!is32 && p.D <= 64) ? 64.0 : 32.0;
+  const double alone = keys / tile_keys + 1.0;
+  const double steps =
+      std::min(p.T / tile_keys + 1.0, alone * (1.0 + 0.45 * std::sqrt(static_cast<double>(queries))));
+  const double step = is32 ? 2.2 * std::max(1.0, p.D / 64.0) : 1.1 * std::max(1.0, p.D / 128.0);
+  const double groups = static_cast<double>(p.B) * p.Hk * chunks * ((p.Tq + queries - 1) / queries);
+  return 5.0 + steps * step * std::max(1.0, groups / 820.0) < query;
+}
+
 hipError_t tile_launch(Params& p, int dtype, hipStream_t stream) {
   TileParams tp{};
   tp.p = p;
