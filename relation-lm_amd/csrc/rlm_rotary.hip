@@ -231,9 +231,9 @@ hipError_t rotary_common(const rlm_tensor* query, const rlm_tensor* key, const r
   RLM_REQUIRE(B * Tq < (int64_t(1) << 31), "at most 2^31 - 1 tokens");
 
   RotaryParams p{};
-  RLM_REQUIRE(position != nullptr && is_index_dtype(position->dtype),
-              "position: expected an int32/int64 tensor");
   if (to_cache) {
+    RLM_REQUIRE(position != nullptr && is_index_dtype(position->dtype),
+                "position: expected an int32/int64 tensor");
     RLM_TRY(check_view(value, "value", Hk, B, Tq, D));
     RLM_TRY(check_same_dtype(value, "value", query, "query"));
     for (const rlm_tensor* c : {out_key, out_value}) {
