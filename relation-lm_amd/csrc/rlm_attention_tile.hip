@@ -2,9 +2,10 @@
 // workgroup.
 //
 // A workgroup holds 4 waves of 16 rows, a row being one query head of one query; the rows of a
-// wave are whole queries with the heads of one key head, consecutive positions of the sequence.  It walks the 64-key tiles that any of its queries sees -- its windows' and its
-// picked blocks' union, found from the picks in LDS -- and every wave takes part in those that
-// its own queries see.  Neighbouring queries share their windows and much of their picks, so a
+// wave are whole queries with the heads of one key head, consecutive positions of the sequence.
+// It walks the tiles of 64 or 32 keys that any of its queries sees -- its windows' and its picked
+// blocks' union, found from the picks in LDS -- and every wave takes part in those that its own
+// queries see.  Neighbouring queries share their windows and much of their picks, so a
 // tile is read once for all of them; a query's own picks decide only which of its scores count.
 //
 // Tiles come by DMA (buffer_load ... lds), the next one in flight while one is worked on.  With
@@ -14,7 +15,9 @@
 //   O^T[dim, row] += V^T P^T over 32 keys whose order is free: a lane's eight weights of two
 //     16-key groups are its operand as they stand, and V^T's operand is two transposing reads
 //     (ds_read_b64_tr_b16) of four keys each from the row-major tile.
-// LDS rows are swizzled in 16-byte pieces, so that both reads spread over all banks.
+// LDS rows are swizzled in 16-byte pieces, which spreads the key reads over all banks.  A third of
+// the LDS cycles (4 x 4096 queries) still count as conflicts; an exchange that gives the transposing
+// reads columns of their own too left that count and the time as they were.
 //
 // The weights are rounded to the 16-bit type for the second product (half a step, relative to
 // each weight); scores, maxima, sums and outputs stay fp32.
@@ -121,8 +124,8 @@ __device__ void attend_row_alone(const Params& p, int64_t b, int64_t step, int64
 }
 
 // DC: head dim in 32s, WHOLE: a tile lies within one block; tiles of kKeys keys for kWaves waves,
-// kStages of them in LDS.
-template <typename T, int DC, bool WHOLE, int kKeys, int kWaves, int kStages>
+// two of them in LDS.
+template <typename T, int DC, bool WHOLE, int kKeys, int kWaves>
 __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_kernel(TileParams tp) {
   constexpr int kThreads = kWaves * kWave;
   constexpr int KT = kKeys / 16;                           // 16-key groups of a tile
@@ -133,7 +136,7 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
   constexpr int kDma = kPitch * kKeys / kThreads;          // DMA instructions of a wave per tile
   constexpr int DT = 2 * DC;                               // head dim in 16s
   constexpr int kWords = kWaves / 2;                       // 16 queries of a wave: half a word
-  extern __shared__ __align__(1024) char lds[];            // [stage][key tile, value tile]
+  extern __shared__ __align__(1024) char lds[];            // [2][key tile, value tile]
   __shared__ __align__(16) uint32_t sel[(kWindowTiles + 2) * kWords];  // [block]: who picked it
   __shared__ __align__(16) uint32_t act[kWindowTiles * kWords];        // [tile]: who sees it
   __shared__ int32_t s_high[kWaves * kRows], s_start[kWaves * kRows];
@@ -320,9 +323,6 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
     const uint32_t own = 0xffffu << (16 * (wave & 1));
     int entry = list[min(lane, count - 1)];
     uint32_t seen = act[entry * kWords + word] & own;
-    // Tile i of the list goes to stage i mod kStages; kStages - 1 of them are on their way while
-    // one is worked on.
-    constexpr int kQueue = kStages - 1;
     auto tile_of = [&](int i) {
       if ((i & (kWave - 1)) == 0 && i != 0) {
         entry = list[min(i + lane, count - 1)];
@@ -330,41 +330,21 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
       }
       return __builtin_amdgcn_readlane(entry, i & (kWave - 1));
     };
-    int ahead = 0, stage = 0;
-    int tiles_ahead[kQueue];
-    uint32_t see_ahead[kQueue];
-#pragma unroll
-    for (int i = 0; i < kQueue; ++i) {
-      tiles_ahead[i] = see_ahead[i] = 0;
-      if (i < count) {
-        tiles_ahead[i] = tile_of(i);
-        see_ahead[i] = __builtin_amdgcn_readlane(seen, i & (kWave - 1));
-        issue(i, w0 + kKeys * tiles_ahead[i]);
-        ++ahead;
-      }
-    }
+    // Tile n of the list is in LDS half n mod 2; the next one is on its way while it is worked on.
+    int next = tile_of(0);
+    uint32_t next_see = __builtin_amdgcn_readlane(seen, 0);
+    issue(0, w0 + kKeys * next);
     for (int n = 0; n < count; ++n) {
-      const int t = tiles_ahead[0];
-      const uint32_t see = see_ahead[0];
-#pragma unroll
-      for (int i = 0; i + 1 < kQueue; ++i) {
-        tiles_ahead[i] = tiles_ahead[i + 1];
-        see_ahead[i] = see_ahead[i + 1];
-      }
-      // Tile n has arrived when at most the loads of the tiles after it are outstanding.
-      if (kStages > 2 && n + kStages - 2 < count)
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm((kQueue - 1) * 2 * kDma));
-      else
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      const int t = next;
+      const uint32_t see = next_see;
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
       barrier();  // tile n is in LDS for every wave, tile n - 1 has been read by every wave
-      if (ahead < count) {
-        tiles_ahead[kQueue - 1] = tile_of(ahead);
-        see_ahead[kQueue - 1] = __builtin_amdgcn_readlane(seen, ahead & (kWave - 1));
-        issue(stage == 0 ? kStages - 1 : stage - 1, w0 + kKeys * tiles_ahead[kQueue - 1]);
-        ++ahead;
+      if (n + 1 < count) {
+        next = tile_of(n + 1);
+        next_see = __builtin_amdgcn_readlane(seen, (n + 1) & (kWave - 1));
+        issue((n + 1) & 1, w0 + kKeys * next);
       }
-      const uint32_t tile0 = lds0 + stage * 2 * kTile;
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      const uint32_t tile0 = lds0 + (n & 1) * 2 * kTile;
       if (see == 0) continue;
       const int32_t p0 = w0 + t * kKeys;
       const bool near = p0 + kKeys > remote;
@@ -534,7 +514,7 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
   }
 }
 
-template <typename T, int DC, bool WHOLE, int kKeys, int kWaves, int kStages>
+template <typename T, int DC, bool WHOLE, int kKeys, int kWaves>
 hipError_t launch(TileParams& tp, hipStream_t stream) {
   const Params& p = tp.p;
   // Rows of a wave: whole queries, the heads of one key head each.
@@ -550,16 +530,16 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
   tp.by_picks = FastDiv(static_cast<uint32_t>(p.TOP + 1));
   tp.by_wave_queries = FastDiv(static_cast<uint32_t>(tp.nqw));
   tp.by_block = FastDiv(static_cast<uint32_t>(p.BS));
-  const size_t lds = kStages * 2 * kKeys * 16 * pitch<T, DC>();
+  const size_t lds = 2 * 2 * kKeys * 16 * pitch<T, DC>();  // two tiles of keys and values
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, WHOLE, kKeys, kWaves, kStages>),
+        reinterpret_cast<const void*>(&attend_tile_kernel<T, DC, WHOLE, kKeys, kWaves>),
         hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     RLM_REQUIRE(e == hipSuccess, "routed_attention: %zu bytes of LDS refused: %s", lds,
                 hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((attend_tile_kernel<T, DC, WHOLE, kKeys, kWaves, kStages>), dim3(tp.pairs * tp.tiles),
-                     dim3(kWaves * kWave), lds, stream, tp);
+  hipLaunchKernelGGL((attend_tile_kernel<T, DC, WHOLE, kKeys, kWaves>),
+                     dim3(tp.pairs * tp.tiles), dim3(kWaves * kWave), lds, stream, tp);
   return launch_status("routed_attention");
 }
 
@@ -574,11 +554,11 @@ template <typename T, bool WHOLE>
 hipError_t launch_type(TileParams& tp, hipStream_t stream) {
   constexpr int kSmall = sizeof(T) == 4 ? 32 : 64;
   const int dc = (tp.p.D + 31) / 32;
-  if (dc <= 1) return launch<T, 1, WHOLE, 64, 4, 2>(tp, stream);
-  if (dc <= 2) return launch<T, 2, WHOLE, kSmall, 4, 2>(tp, stream);
-  if (dc <= 3) return launch<T, 3, WHOLE, 32, 4, 2>(tp, stream);
-  if (dc <= 4) return launch<T, 4, WHOLE, 32, 4, 2>(tp, stream);
-  return launch<T, 8, WHOLE, 32, 4, 2>(tp, stream);
+  if (dc <= 1) return launch<T, 1, WHOLE, 64, 4>(tp, stream);
+  if (dc <= 2) return launch<T, 2, WHOLE, kSmall, 4>(tp, stream);
+  if (dc <= 3) return launch<T, 3, WHOLE, 32, 4>(tp, stream);
+  if (dc <= 4) return launch<T, 4, WHOLE, 32, 4>(tp, stream);
+  return launch<T, 8, WHOLE, 32, 4>(tp, stream);
 }
 
 }  // namespace
