@@ -29,6 +29,8 @@ constexpr int kKeys = 32;  // keys of a wave's tile
 template <typename T>
 constexpr bool kIs32 = sizeof(T) == 4;
 
+__device__ const uint4 zeros = {0, 0, 0, 0};
+
 // DC: head dim in 32s.
 template <typename T, int DC, int MAXW>
 __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
@@ -127,13 +129,16 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
     }
     if constexpr (!kIs32<T>) {
       // The values' rows into the wave's LDS, pieces where the swizzle puts them (pieces past
-      // the head dim hold anything: they are features that nobody reads).
+      // the head dim hold anything: they are features that nobody reads).  Keys that do not
+      // count have values of 0: their weight 0 times an infinity of the row that stands for them
+      // would be NaN.
 #pragma unroll
       for (int i = 0; i < kKeys * kPitch / kWave; ++i) {
         const int to = i * (kWave / kPitch) + lane / kPitch;
         const int piece = (lane % kPitch) ^ swizzle<kPitch>(to);
         const T* src = vbase + static_cast<int64_t>(__shfl(row, to, kWave)) * p.v_st +
                        (8 * piece < D ? 8 * piece : 0);
+        src = (mask >> to) & 1 ? src : reinterpret_cast<const T*>(&zeros);
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) void*)(src),
             (__attribute__((address_space(3))) void*)static_cast<uintptr_t>(mine + i * kWave * 16), 16, 0, 0);
@@ -150,7 +155,8 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
 #pragma unroll
           for (int j = 0; j < DT; ++j) {
             const int d = 16 * j + r;
-            vs[j][kt][i] = src[d < D ? d : 0];
+            const float v = src[d < D ? d : 0];
+            vs[j][kt][i] = (mask >> (16 * kt + 4 * quad + i)) & 1 ? v : 0.0f;
           }
         }
     }

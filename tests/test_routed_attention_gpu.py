@@ -310,6 +310,24 @@ def test_ring_decode(device, t, dtype):
     check(out[:, None], lse[:, None], expected, dtype, 64)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("batch,window,top", [(1, 1, 0), (2, 20, 3), (300, 33, 1)])
+def test_an_infinity_that_is_seen_stays_one(device, batch, window, top, dtype):
+    """The window's last row holds an infinite value feature: that feature is infinite, whatever
+    keys of the same tile do not count, and the other features are as they were."""
+    g = torch.Generator().manual_seed(13)
+    query, key, value, _, picks = case(g, batch, 1, 4, 2, 64, 100, 7, top, 1, dtype)
+    args = [x.to(device) for x in (query[:, 0], key, value, picks[:, 0, 0], torch.tensor(90))]
+    clean, lse = routed_attention(*args, 7, window)
+    args[2] = args[2].clone()
+    args[2][:, 90, :, 5] = float("inf")
+    out, again = routed_attention(*args, 7, window)
+    torch.cuda.synchronize()
+    assert torch.isposinf(out[..., 5]).all()
+    rest = [i for i in range(64) if i != 5]
+    assert torch.equal(out[..., rest], clean[..., rest]) and torch.equal(lse, again)
+
+
 def test_ring_equals_linear_before_it_wraps(device):
     g = torch.Generator().manual_seed(9)
     query, key, value, positions, picks = case(g, 5, 1, 8, 2, 128, 256, 32, 4, 1, torch.bfloat16)
