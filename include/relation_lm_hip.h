@@ -774,7 +774,8 @@ hipError_t rlm_block_statistics(const rlm_tensor* keys, int64_t block_size,
  * path picks one anchor and K partners where these attend)
  *
  * Inputs may be strided views with unit stride in their last dim; outputs are
- * contiguous.  `positions` is 0-d, [Tq] (shared by the batch) or [B,Tq], int32
+ * contiguous.  What is written (outputs, caches) shares no memory with what is
+ * read.  `positions` is 0-d, [Tq] (shared by the batch) or [B,Tq], int32
  * or int64.
  * ---------------------------------------------------------------------- */
 
@@ -816,7 +817,8 @@ hipError_t rlm_rotary_to_caches(const rlm_tensor* query, const rlm_tensor* key,
  *   router_query [B,Tq,S,RD], block_mean/std [B,NB,H,HD] f32 (H*HD == RD <= 1024,
  *   HD a multiple of 4), gamma [H], bias [H,RB] (H*RB <= 2048), top_blocks in
  *   [1, 64].  ring: slot j holds the newest block of index j mod NB (NB and
- *   block_size powers of two); blocks stay absolute.
+ *   block_size powers of two); blocks stay absolute, those past int32 are not
+ *   picked.
  * Outputs: out_blocks int32 [B,Tq,S,TOP], out_scores f32 [B,Tq,S,TOP]; -1 and
  * -inf where a query has fewer blocks to pick from.  A block whose score is NaN
  * or at most -1e30 is not picked.

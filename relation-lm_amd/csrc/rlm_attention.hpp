@@ -34,6 +34,13 @@ struct Params {
   bool ring;
 };
 
+// A query's position, within what its sums below hold in 64 bits (any negative one sees nothing).
+__device__ __forceinline__ int64_t position_of(const Params& p, int64_t b, int64_t step) {
+  const int64_t t = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_sq);
+  constexpr int64_t kMost = INT64_MAX - 1;
+  return t < -1 ? -1 : t < kMost ? t : kMost;
+}
+
 __device__ __forceinline__ float rows_max(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
   const int head = static_cast<int>(hk) * p.G + (row_ok ? in_group : 0);
   const int D = p.D;
 
-  const int64_t t = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_sq);
+  const int64_t t = position_of(p, b, step);
   const int32_t* picks = p.blocks + b * p.blk_sb + step * p.blk_st + hk * p.blk_sh;
   int32_t pick = lane < p.TOP ? picks[lane] : -1;
 
@@ -269,6 +269,7 @@ hipError_t launch(const Params& p, hipStream_t stream) {
   const int64_t tiles = (p.local_window + p.TOP * p.BS + kKeys - 1) / kKeys;
   int waves = 1;
   while (waves < MAXW && waves < tiles && static_cast<int64_t>(p.items) * waves < 4096) waves *= 2;
+  RLM_TRY(check_launch("routed_attention", p.items, kWave * waves));
   const size_t values = sizeof(T) == 4 ? 0 : static_cast<size_t>(waves) * kKeys * 16 * kPitch;
   const size_t merge = waves == 1 ? 0 : static_cast<size_t>(waves) * (DT * kWave * 16 + 16 * 8);
   const size_t lds = std::max(values, merge);

@@ -72,7 +72,7 @@ __device__ void attend_row_alone(const Params& p, int64_t b, int64_t step, int64
   const T* vbase = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
   const int32_t* picks = p.blocks + b * p.blk_sb + step * p.blk_st + hk * p.blk_sh;
   const int32_t mine = lane < p.TOP ? picks[lane] : -1;
-  const int64_t t = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_sq);
+  const int64_t t = position_of(p, b, step);
   const int64_t high = t + 1 < p.T ? t + 1 : p.T;
   int64_t start = t - p.local_window + 1;
   start = start > 0 ? start : 0;
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kWaves* kWave, DC <= 4 ? 4 : 2) void attend_tile_ke
     const int q = q0 + threadIdx.x;
     int32_t high = 0, start = 0;
     if (q < p.Tq) {
-      const int64_t t = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + q * p.pos_sq);
+      const int64_t t = position_of(p, b, q);
       int64_t s = t - p.local_window + 1;
       s = s > 0 ? s : 0;
       high = static_cast<int32_t>(t < 0 ? 0 : t + 1 < p.T ? t + 1 : p.T);
@@ -522,7 +522,9 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
   tp.hg = (p.G + tp.chunks - 1) / tp.chunks;
   tp.nqw = kRows / tp.hg;
   tp.pairs = static_cast<uint32_t>(p.B * p.Hk * tp.chunks);
-  tp.tiles = static_cast<uint32_t>((p.Tq + kWaves * tp.nqw - 1) / (kWaves * tp.nqw));
+  tp.tiles = (static_cast<uint32_t>(p.Tq) + kWaves * tp.nqw - 1) / (kWaves * tp.nqw);
+  RLM_TRY(check_launch("routed_attention", static_cast<int64_t>(tp.pairs) * tp.tiles,
+                       kWaves * kWave));
   tp.by_pairs = FastDiv(tp.pairs);
   tp.by_chunks = FastDiv(static_cast<uint32_t>(tp.chunks));
   tp.by_kv = FastDiv(static_cast<uint32_t>(p.Hk));

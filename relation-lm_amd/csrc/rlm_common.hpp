@@ -526,6 +526,8 @@ bool check_no_overlap(const rlm_tensor* t, const char* name);
 // [B,Tq]; gives their strides.
 bool check_positions(const rlm_tensor* t, const char* name, int64_t B, int64_t Tq,
                      int64_t* stride_b, int64_t* stride_q);
+// Checks that a launch stays within what the device takes: fewer than 2^32 threads.
+bool check_launch(const char* what, int64_t groups, int64_t threads);
 // Checks t->shape[dim] == value.
 bool check_dim(const rlm_tensor* t, const char* name, int dim, int64_t value);
 bool check_dtype_float(const rlm_tensor* t, const char* name);

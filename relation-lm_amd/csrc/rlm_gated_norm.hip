@@ -201,6 +201,7 @@ template <typename T, typename W, int V, int R, int NV>
 hipError_t launch(const GatedNormParams& p, hipStream_t stream) {
   constexpr int kRows = kThreads / R;
   const dim3 grid(static_cast<unsigned>((p.rows + kRows - 1) / kRows));
+  RLM_TRY(check_launch("gated_residual_norm", grid.x, kThreads));
   hipLaunchKernelGGL((gated_norm_kernel<T, W, V, R, NV>), grid, dim3(kThreads), 0, stream, p);
   return launch_status("gated_residual_norm");
 }

@@ -171,6 +171,14 @@ bool check_positions(const rlm_tensor* t, const char* name, int64_t B, int64_t T
   return check_dense(t, name, 2) && check_dim(t, name, 0, B) && check_dim(t, name, 1, Tq);
 }
 
+bool check_launch(const char* what, int64_t groups, int64_t threads) {
+  if (groups * threads < (int64_t(1) << 32)) return true;
+  set_error("%s: too many rows for one call (%lld workgroups of %lld threads, fewer than 2^32 "
+            "threads in all)",
+            what, (long long)groups, (long long)threads);
+  return false;
+}
+
 bool check_dim(const rlm_tensor* t, const char* name, int dim, int64_t value) {
   if (t->shape[dim] != value) {
     set_error("%s: size %lld in dim %d does not match the expected %lld", name,

@@ -167,12 +167,14 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
 
 template <typename T, int V>
 hipError_t launch_rotary(const RotaryParams& p, bool interleaved, hipStream_t stream) {
+  const char* name = p.to_cache ? "rotary_to_caches" : "rotary_positions";
   const dim3 grid((p.tokens + p.per_group - 1) / p.per_group);
+  RLM_TRY(check_launch(name, grid.x, kThreads));
   if (interleaved)
     hipLaunchKernelGGL((rotary_kernel<T, V, true>), grid, dim3(kThreads), 0, stream, p);
   else
     hipLaunchKernelGGL((rotary_kernel<T, V, false>), grid, dim3(kThreads), 0, stream, p);
-  return launch_status(p.to_cache ? "rotary_to_caches" : "rotary_positions");
+  return launch_status(name);
 }
 
 template <typename T>

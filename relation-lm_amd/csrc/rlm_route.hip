@@ -169,7 +169,8 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
     const uint32_t row = min(row0 + i, p.rows_per_batch - 1);
     const uint32_t step = p.by_slots.div(row, slot);
     const int64_t at = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_sq);
-    t[i] = at < (int64_t(1) << 56) ? at : (int64_t(1) << 56);
+    // Within what the sums below hold in 64 bits (any negative one has no block).
+    t[i] = at < -1 ? -1 : at < INT64_MAX - 1 ? at : INT64_MAX - 1;
     tmax = t[i] > tmax ? t[i] : tmax;
   }
   __syncthreads();
@@ -237,7 +238,9 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
       // In a ring, slot j holds the block of remainder j among [lowest, lowest + NB).
       block[k] = p.ring ? lowest[k] + ((j - lowest[k]) & (p.NB - 1)) : j;
       const int64_t end = block[k] * p.BS + p.BS - 1;
-      ok[k] = j < slots && block[k] >= 0 && end <= mine[k] && (!p.strict || end < start[k]);
+      // (A ring's block that the picks' type does not hold is no pick.)
+      ok[k] = j < slots && block[k] >= 0 && block[k] <= INT32_MAX && end <= mine[k] &&
+              (!p.strict || end < start[k]);
       const int64_t away = mine[k] > end ? mine[k] - end : 0;
       const int log2 = 63 - __builtin_clzll(static_cast<uint64_t>(away + 1));
       bucket[k] = log2 < p.RB ? log2 : p.RB - 1;
@@ -337,6 +340,7 @@ hipError_t launch_route(RouteParams& p, int64_t B, hipStream_t stream) {
     const int rounds = (p.NB + kWave / P - 1) / (kWave / P);
     const int waves = std::min(16, std::max(1, rounds));
     const size_t bytes = shared + sizeof(double) * RD + sizeof(uint64_t) * waves * kWave;
+    RLM_TRY(check_launch("block_route", p.groups, waves * kWave));
     hipLaunchKernelGGL((route_kernel<TQ, P, 1, true>), dim3(p.groups), dim3(waves * kWave), bytes,
                        stream, p);
     return launch_status("block_route");
@@ -346,7 +350,9 @@ hipError_t launch_route(RouteParams& p, int64_t B, hipStream_t stream) {
   p.groups = static_cast<uint32_t>(B * p.groups_per_batch);
   p.by_groups = FastDiv(p.groups_per_batch);
   const size_t bytes = shared + sizeof(double) * kWaves * kQueries * RD;
-  hipLaunchKernelGGL((route_kernel<TQ, P, kQueries, false>), dim3((p.groups + kWaves - 1) / kWaves),
+  const dim3 grid((p.groups + kWaves - 1) / kWaves);
+  RLM_TRY(check_launch("block_route", grid.x, kWaves * kWave));
+  hipLaunchKernelGGL((route_kernel<TQ, P, kQueries, false>), grid,
                      dim3(kWaves * kWave), bytes, stream, p);
   return launch_status("block_route");
 }

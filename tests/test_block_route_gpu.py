@@ -100,6 +100,53 @@ def test_ring(device, t, strict):
     check(got, [w[:, 0] for w in want])
 
 
+def test_ring_blocks_past_int32_are_not_picked(device):
+    """16 blocks on both sides of number 2^31: the picks are those below it."""
+    g = torch.Generator().manual_seed(7)
+    x = inputs(g, 3, 1, 2, 4, 16, 16, 16, torch.bfloat16)
+    t = 32 * (2**31 + 4) + 31
+    got = block_route(x["query"][:, 0].to(device), *(x[k].to(device) for k in
+                                                     ("mean", "std", "gamma", "bias")),
+                      torch.tensor(t, device=device), 32, 64, 14, False, True)
+    torch.cuda.synchronize()
+    ranked = oracle(x, np.array(t), 32, 64, 16, False, True)     # blocks from 2^31 on: negative
+    want = [np.full((3, 2, 14), -1, np.int32), np.full((3, 2, 14), -np.inf, np.float32)]
+    for row in np.ndindex(3, 2):
+        blocks, scores = (w[row[0], 0, row[1]] for w in ranked)
+        held = blocks >= 0
+        assert held.sum() == 11
+        want[0][row][:11], want[1][row][:11] = blocks[held], scores[held]
+    check(got, want)
+
+
+@pytest.mark.parametrize("queries", [5, 700])
+def test_positions_at_the_ends_of_int64(device, queries):
+    """The last one has every block of the cache, all in the farthest bucket; the first none."""
+    g = torch.Generator().manual_seed(8)
+    x = inputs(g, 1, queries, 1, 4, 16, 20, 16, torch.bfloat16)
+    positions = torch.full((queries,), 2**62)
+    want = oracle(x, positions.numpy(), 8, 16, 20, True)
+    want[0][:, 1::2], want[1][:, 1::2] = -1, -np.inf
+    positions[::4], positions[1::2] = 2**63 - 1, -2**63
+    got = block_route_seq(x["query"][:, :, 0].to(device), *(x[k].to(device) for k in
+                                                            ("mean", "std", "gamma", "bias")),
+                          positions.to(device), 8, 16, 20, True)
+    torch.cuda.synchronize()
+    check(got, [w[:, :, 0] for w in want])
+
+
+def test_widest_tables(device):
+    """64 heads of 4 features with 32 buckets, four queries to a wave: the most shared memory."""
+    g = torch.Generator().manual_seed(9)
+    x = inputs(g, 1, 530, 1, 64, 4, 70, 32, torch.bfloat16)
+    positions = torch.arange(530)
+    got = block_route_seq(x["query"][:, :, 0].to(device), *(x[k].to(device) for k in
+                                                            ("mean", "std", "gamma", "bias")),
+                          positions.to(device), 7, 9, 11, False)
+    torch.cuda.synchronize()
+    check(got, [w[:, :, 0] for w in oracle(x, positions.numpy(), 7, 9, 11, False)])
+
+
 @pytest.mark.parametrize("queries", [1, 600])
 @pytest.mark.parametrize("ring", [False, True])
 def test_ties_go_to_the_lowest_block(device, queries, ring):

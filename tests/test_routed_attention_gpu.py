@@ -169,6 +169,20 @@ def test_rows_that_see_nothing_and_positions_past_the_cache(device, tiles, dtype
         assert tile_kernel(lambda: routed_attention_seq(*args, 16, 24))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tiles", [False, True])
+def test_positions_at_the_ends_of_int64(device, tiles, dtype):
+    """The last one sees what was picked, as any position past the window does; the first one
+    nothing."""
+    g = torch.Generator().manual_seed(14)
+    query, key, value, positions, picks = (many(g, dtype, 8, 4) if tiles else
+                                           case(g, 2, 40, 4, 2, 64, 96, 16, 3, 1, dtype))
+    positions[0, 1::4] = 2 ** 63 - 1
+    positions[1, 2::4] = -2 ** 63
+    out, lse = run_seq(device, (query, key, value, positions, picks), 16, 24, 1)
+    assert (out[1, 2::4] == 0).all() and torch.isneginf(lse[1, 2::4]).all()
+
+
 def test_scores_past_a_tiles_limit(device):
     """Keys that grow along the cache: every tile's scores pass the base of the one before, by
     more than fp16 weights could hold; and all scores equal (a scale of 0)."""

@@ -253,3 +253,24 @@ def test_calls_without_elements_return_at_once(lib):
                      lse=tensor([2, 0, 6], RLM_F32))[0] == 0
     none = tensor([0, 64], RLM_BF16)
     assert norm(lib, branch=none, residual=none, hidden=none, normalized=none)[0] == 0
+
+
+def test_more_threads_than_one_launch_takes(lib):
+    n = 1 << 29
+    rows = dict(query=tensor([1, n, 1, 8], RLM_BF16), key=tensor([1, n, 1, 8], RLM_BF16),
+                positions=tensor([n], RLM_I64), frequencies=tensor([4], RLM_F32),
+                out_query=tensor([1, n, 1, 8], RLM_BF16), out_key=tensor([1, n, 1, 8], RLM_BF16))
+    refused(rotary(lib, **rows), "rotary_positions", "too many rows")
+    refused(route(lib, query=tensor([1, n, 1, 4], RLM_BF16), mean=tensor([1, 1, 1, 4], RLM_F32),
+                  std=tensor([1, 1, 1, 4], RLM_F32), gamma=tensor([1], RLM_F32),
+                  bias=tensor([1, 1], RLM_F32), positions=tensor([n], RLM_I64),
+                  blocks=tensor([1, n, 1, 4], RLM_I32), scores=tensor([1, n, 1, 4], RLM_F32)),
+            "block_route", "too many rows")
+    one = dict(query=tensor([n, 1, 1, 8], RLM_BF16), key=tensor([n, 1, 1, 8], RLM_BF16),
+               value=tensor([n, 1, 1, 8], RLM_BF16), blocks=tensor([n, 1, 1], RLM_I32),
+               positions=tensor([n, 1], RLM_I64), out=tensor([n, 1, 1, 8], RLM_BF16),
+               lse=tensor([n, 1, 1], RLM_F32))
+    refused(attention(lib, **one), "routed_attention", "too many rows")
+    wide = tensor([n, 8], RLM_BF16)
+    refused(norm(lib, branch=wide, residual=wide, weight=tensor([8], RLM_BF16), hidden=wide,
+                 normalized=wide), "gated_residual_norm", "too many rows")
