@@ -17,11 +17,11 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 typedef const __attribute__((address_space(3))) s16x8* lds_s16x8;
 typedef const __attribute__((address_space(3))) float* lds_f32;
 
-// 16-byte pieces of an LDS row of at most 32 DC features: a power of two, 8 at least.
-template <typename T, int DC>
+// 16-byte pieces of an LDS row of at most 32 DC features: a power of two, LEAST at least.
+template <typename T, int DC, int LEAST = 8>
 constexpr int pitch() {
   constexpr int pieces = DC * 32 * static_cast<int>(sizeof(T)) / 16;
-  return pieces <= 8 ? 8 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : 64;
+  return pieces <= LEAST ? LEAST : pieces <= 8 ? 8 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : 64;
 }
 
 // c + a b over 32 (16-bit types) or 16 (fp32: four steps of four) features or keys.
@@ -50,10 +50,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, f16) {
 }
 
 // 16-byte pieces of an LDS row: rows of 8 pieces alternate between the halves of the 16 piece
-// columns that the banks form, so their swizzle goes by pairs of rows.
+// columns that the banks form, so their swizzle goes by pairs of rows (of 4: by four rows).
 template <int PITCH>
 __device__ __forceinline__ int swizzle(int row) {
-  return PITCH == 8 ? (row >> 1) & 7 : row & 15;
+  return PITCH == 4 ? (row >> 2) & 3 : PITCH == 8 ? (row >> 1) & 7 : row & 15;
 }
 
 // Lane l reads four values of key l / 16 * 4 + l % 16 / 4 at `at` and gets four keys of value

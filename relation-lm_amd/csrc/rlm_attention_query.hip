@@ -2,7 +2,8 @@
 // prompts that the shared tiles (rlm_attention_tile.hip) do not take.
 //
 // A workgroup has up to 16 query heads of one query and key head (the rows or columns of a
-// matrix product) and shares the query's keys among its waves, 32 at a time.  The keys are one
+// matrix product) and shares the query's keys among its waves, 32 at a time; where there are fewer
+// such items than half the CUs, workgroups share the value features of each.  The keys are one
 // list: the window's positions, then every picked block's; a lane finds one of a tile's keys
 // -- its cache row and whether it counts -- and hands it to the lanes that load it, so blocks
 // shorter than a tile share one.  A key that does not count (past the position, in the window
@@ -31,11 +32,11 @@ constexpr bool kIs32 = sizeof(T) == 4;
 
 __device__ const uint4 zeros = {0, 0, 0, 0};
 
-// DC: head dim in 32s.
-template <typename T, int DC, int MAXW>
+// DC: head dim in 32s; PARTS workgroups have a share of the value features each.
+template <typename T, int DC, int MAXW, int PARTS>
 __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
-  constexpr int DT = 2 * DC;                               // head dim in 16s
-  constexpr int kPitch = pitch<T, DC>();                   // 16-byte pieces of an LDS row
+  constexpr int DT = 2 * DC / PARTS;                       // value features in 16s
+  constexpr int kPitch = pitch<T, DC / PARTS, 4>();                   // 16-byte pieces of an LDS row
   constexpr int kRow = 16 * kPitch;
   extern __shared__ __align__(1024) char lds[];
   const int lane = threadIdx.x & (kWave - 1);
@@ -43,7 +44,13 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
   const int r = lane & 15, quad = lane >> 4;
   const int W = blockDim.x / kWave;
   uint32_t chunk, hk, step;
-  const int64_t b = p.by_queries.div(p.by_kv.div(p.by_chunks.div(blockIdx.x, chunk), hk), step);
+  // The parts of an item a grid apart: on one XCD where 8 divides the items.
+  uint32_t part = 0;
+#pragma unroll
+  for (int i = 1; i < PARTS; ++i) part += blockIdx.x >= i * p.items;
+  const uint32_t item = blockIdx.x - part * p.items;
+  const int first = 16 * DT * part;  // value feature
+  const int64_t b = p.by_queries.div(p.by_kv.div(p.by_chunks.div(item, chunk), hk), step);
   const int in_group = static_cast<int>(chunk) * p.heads_per_chunk + r;
   const bool row_ok = r < p.heads_per_chunk && in_group < p.G;
   const int head = static_cast<int>(hk) * p.G + (row_ok ? in_group : 0);
@@ -54,7 +61,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
   int32_t pick = lane < p.TOP ? picks[lane] : -1;
 
   typedef typename std::conditional<kIs32<T>, float4, s16x8>::type frag_t;
-  constexpr int kFrags = kIs32<T> ? DT : DC;   // 16-byte pieces of a lane's row
+  constexpr int kFrags = kIs32<T> ? 2 * DC : DC;   // 16-byte pieces of a lane's row
   constexpr int kFeatures = kIs32<T> ? 4 : 8;  // in each
   const int d0 = kFeatures * quad;             // and between them 4 kFeatures
   frag_t qf[kFrags];
@@ -137,7 +144,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
         const int to = i * (kWave / kPitch) + lane / kPitch;
         const int piece = (lane % kPitch) ^ swizzle<kPitch>(to);
         const T* src = vbase + static_cast<int64_t>(__shfl(row, to, kWave)) * p.v_st +
-                       (8 * piece < D ? 8 * piece : 0);
+                       (first + 8 * piece < D ? first + 8 * piece : 0);
         src = (mask >> to) & 1 ? src : reinterpret_cast<const T*>(&zeros);
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) void*)(src),
@@ -154,7 +161,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
               vbase + static_cast<int64_t>(__shfl(row, 16 * kt + 4 * quad + i, kWave)) * p.v_st;
 #pragma unroll
           for (int j = 0; j < DT; ++j) {
-            const int d = 16 * j + r;
+            const int d = first + 16 * j + r;
             const float v = src[d < D ? d : 0];
             vs[j][kt][i] = (mask >> (16 * kt + 4 * quad + i)) & 1 ? v : 0.0f;
           }
@@ -220,11 +227,11 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
   const int64_t row = (b * p.Tq + step) * p.Hq + head;
   T* out = static_cast<T*>(p.out) + row * D;
   auto write = [&](int j, f32x4 v, float inv) {
-    const int d = 16 * j + 4 * quad;
+    const int d = first + 16 * j + 4 * quad;
     if (row_ok && d < D) put4<T>(out + d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
   };
   auto write_lse = [&](float base, float total) {
-    if (row_ok && quad == 0)
+    if (row_ok && quad == 0 && part == 0)
       p.lse[row] = total == 0.0f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
   };
   if (W == 1) {
@@ -261,28 +268,58 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
   if (wave == 0) write_lse(top, total);
 }
 
-template <typename T, int DC, int MAXW>
+template <typename T, int DC, int MAXW, int PARTS>
 hipError_t launch(const Params& p, hipStream_t stream) {
-  constexpr int DT = 2 * DC;
-  constexpr int kPitch = pitch<T, DC>();
+  constexpr int DT = 2 * DC / PARTS;
+  constexpr int kPitch = pitch<T, DC / PARTS, 4>();
   // Waves of a query: enough to fill the chip, and one tile each at least.
   const int64_t tiles = (p.local_window + p.TOP * p.BS + kKeys - 1) / kKeys;
   int waves = 1;
   while (waves < MAXW && waves < tiles && static_cast<int64_t>(p.items) * waves < 4096) waves *= 2;
-  RLM_TRY(check_launch("routed_attention", p.items, kWave * waves));
+  RLM_TRY(check_launch("routed_attention", int64_t{PARTS} * p.items, kWave * waves));
   const size_t values = sizeof(T) == 4 ? 0 : static_cast<size_t>(waves) * kKeys * 16 * kPitch;
   const size_t merge = waves == 1 ? 0 : static_cast<size_t>(waves) * (DT * kWave * 16 + 16 * 8);
   const size_t lds = std::max(values, merge);
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(&attend_query_kernel<T, DC, MAXW>),
+        reinterpret_cast<const void*>(&attend_query_kernel<T, DC, MAXW, PARTS>),
         hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     RLM_REQUIRE(e == hipSuccess, "routed_attention: %zu bytes of LDS refused: %s", lds,
                 hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((attend_query_kernel<T, DC, MAXW>), dim3(p.items), dim3(kWave * waves), lds,
-                     stream, p);
+  hipLaunchKernelGGL((attend_query_kernel<T, DC, MAXW, PARTS>), dim3(PARTS * p.items),
+                     dim3(kWave * waves), lds, stream, p);
   return launch_status("routed_attention");
+}
+
+// Parts of the value features: as many as leave every workgroup a CU of its own.  Each part
+// computes the weights anew and reads the keys again (from the L2 that they share), but its
+// values, its sums and their merge are the shorter for it.  Measured, one part / two / four (us;
+// a window of 512 and 16 blocks of 64):
+//   bf16, 128 features    8 items: 20.9 / 17.3 / 15.6    64: 24.1 / 19.5 / 17.7
+//                         128: 26.1 / 21.9               192: 31.1 / 42.8
+//   fp32, 128 features    8 items: 63 / 47 / 31          64: 126 / 82 / 35    192: 176 / 209
+//   bf16, 64 features     8 items: 11.6 / 10.6           128: 13.3 / 13.3
+constexpr int kUnits = 256;  // compute units
+template <typename T, int DC, int MAXW>
+hipError_t launch_parts(const Params& p, hipStream_t stream) {
+  const uint32_t room = kUnits / p.items;
+  if constexpr (DC >= 4)
+    if (room >= 4) return launch<T, DC, MAXW, 4>(p, stream);
+  if constexpr (DC == 3)
+    if (room >= 3) return launch<T, DC, MAXW, 3>(p, stream);
+  if constexpr (DC % 2 == 0)
+    if (room >= 2) return launch<T, DC, MAXW, 2>(p, stream);
+  return launch<T, DC, MAXW, 1>(p, stream);
+}
+template <typename T, int WIDE>
+hipError_t launch_type(const Params& p, hipStream_t stream) {
+  const int dc = (p.D + 31) / 32;
+  if (dc <= 1) return launch_parts<T, 1, 16>(p, stream);
+  if (dc <= 2) return launch_parts<T, 2, WIDE>(p, stream);
+  if (dc <= 3) return launch_parts<T, 3, WIDE>(p, stream);
+  if (dc <= 4) return launch_parts<T, 4, WIDE>(p, stream);
+  return launch_parts<T, 8, 8>(p, stream);
 }
 
 }  // namespace
@@ -290,17 +327,9 @@ hipError_t launch(const Params& p, hipStream_t stream) {
 namespace attention {
 
 hipError_t query_launch(const Params& p, int dtype, hipStream_t stream) {
-  const int dc = (p.D + 31) / 32;
-#define RLM_QUERY_TYPE(T, W4)                                                         \
-  return dc <= 1 ? launch<T, 1, 16>(p, stream)                                        \
-         : dc <= 2 ? launch<T, 2, W4>(p, stream)                                      \
-         : dc <= 3 ? launch<T, 3, W4>(p, stream)                                      \
-         : dc <= 4 ? launch<T, 4, W4>(p, stream)                                      \
-                   : launch<T, 8, 8>(p, stream);
-  if (dtype == RLM_F32) RLM_QUERY_TYPE(float, 8)
-  if (dtype == RLM_BF16) RLM_QUERY_TYPE(bf16, 16)
-  RLM_QUERY_TYPE(f16, 16)
-#undef RLM_QUERY_TYPE
+  if (dtype == RLM_F32) return launch_type<float, 8>(p, stream);
+  if (dtype == RLM_BF16) return launch_type<bf16, 16>(p, stream);
+  return launch_type<f16, 16>(p, stream);
 }
 
 }  // namespace attention

@@ -302,6 +302,22 @@ def test_decode_form(device, shape, dtype):
         check(out[:, None], lse[:, None], expected, dtype, dim)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("items", [64, 65, 85, 86, 128, 129, 257])
+@pytest.mark.parametrize("dim", [40, 72, 96, 104, 136, 200])
+def test_features_shared_by_workgroups(device, dim, items, dtype):
+    """Both sides of every number of (row, key head) items where the value features are shared
+    by one workgroup more, and head dims that leave the last of them part of its share or none."""
+    g = torch.Generator().manual_seed(items + dim)
+    query, key, value, positions, picks = case(g, items, 1, 3, 1, dim, 150, 16, 3, 1, dtype)
+    out, lse = routed_attention(query[:, 0].to(device), key.to(device), value.to(device),
+                                picks[:, 0, 0].to(device), positions[:, 0].to(device), 16, 50)
+    torch.cuda.synchronize()
+    expected = routed_layer.attention(host(query), host(key), host(value), picks.numpy(),
+                                      positions.numpy(), 16, 50, dim ** -0.5)
+    check(out[:, None], lse[:, None], expected, dtype, dim)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("t", [0, 5, 63, 64, 100, 127, 128, 1000, 2**33 + 77])
 def test_ring_decode(device, t, dtype):
