@@ -9,7 +9,9 @@
 // to be right to its rounding or equal inputs would not tie.  Bound: VALU issue of the float64
 // products and of the exponentials, 2 RD products and H exponentials per (query, block).
 // A wave takes Q queries of one batch row over 64 / P blocks at a time, P lanes to a block;
-// each statistics access (16 bytes a lane, P lanes together) then serves Q queries.  After a
+// each statistics access (16 bytes a lane, P lanes together) then serves Q queries.  Where there
+// are too few queries to fill the chip, a workgroup's waves share the blocks of its queries
+// (SPLIT) and their lists are merged.  After a
 // head's products the P lanes share their sums, and each of them carries on the exponentials
 // of its own Q / P queries.
 #include "rlm_common.hpp"
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
   double* spread = lds;                       // [H]: softplus(gamma)
   double* bias = spread + p.H;                // [H,RB]
   double* q = bias + p.H * p.RB + (SPLIT ? 0 : wave * Q * RD);
-  uint64_t* lists = reinterpret_cast<uint64_t*>(bias + p.H * p.RB + Q * RD);  // SPLIT: [waves,64]
+  uint64_t* lists = reinterpret_cast<uint64_t*>(bias + p.H * p.RB + Q * RD);  // SPLIT: [waves,Q,64]
 
   uint32_t group = SPLIT ? blockIdx.x : blockIdx.x * waves + wave;
   const bool live = group < p.groups;
@@ -194,7 +196,7 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
   const int slots = static_cast<int>(complete < p.NB ? complete : p.NB);
   const bool short_list = p.TOP <= 16;
   uint64_t list[Q] = {};
-  // Four queries, four lanes to a block: the first 64 blocks' keys wait in registers (a lane has
+  // Four queries, four lanes to a block: the wave's first 64 blocks' keys wait in registers (a lane has
   // its own query's), and the lists start from their TOP largest, found for the four queries
   // at once.  Blocks after those enter one by one where they pass the list's last.
   constexpr bool kFirst = Q == 4 && P == 4;
@@ -226,9 +228,11 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
     m = *reinterpret_cast<const float4*>(p.mean + at);
     s4 = *reinterpret_cast<const float4*>(p.std + at);
   }
-  for (int j0 = (SPLIT ? wave : 0) * kBlocks; j0 < slots; j0 += (SPLIT ? waves : 1) * kBlocks) {
+  const int stride = (SPLIT ? waves : 1) * kBlocks;
+  int pass = 0;
+  for (int j0 = (SPLIT ? wave : 0) * kBlocks; j0 < slots; j0 += stride, ++pass) {
     const int j = j0 + in_wave;
-    const int64_t at = block_at(j0), next_at = block_at(j0 + (SPLIT ? waves : 1) * kBlocks);
+    const int64_t at = block_at(j0), next_at = block_at(j0 + stride);
     int64_t block[kPer];
     int bucket[kPer];
     bool ok[kPer];
@@ -295,11 +299,11 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
                    ? select_key(score, static_cast<uint32_t>(block[k] - lowest[k]))
                    : 0;
     }
-    if (kFirst && j0 < kWave) {
+    if (kFirst && pass < P) {
 #pragma unroll
       for (int i = 0; i < P; ++i)
-        if (j0 == i * kBlocks) waiting[kFirst ? i : 0] = key[0];
-      if (j0 + kBlocks >= slots || j0 + kBlocks == kWave) start_lists();
+        if (pass == i) waiting[kFirst ? i : 0] = key[0];
+      if (j0 + stride >= slots || pass == P - 1) start_lists();
     } else {
 #pragma unroll
       for (int i = 0; i < Q; ++i)
@@ -308,16 +312,21 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
   }
 
   if constexpr (SPLIT) {
-    // The waves' lists into the first wave's.
-    if (wave != 0) lists[wave * kWave + lane] = lane < p.TOP ? list[0] : 0;
+    // The waves' lists into one, each query's by a wave of its own.
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+      lists[(wave * Q + i) * kWave + lane] = lane < p.TOP ? list[i] : 0;
     __syncthreads();
-    if (wave != 0) return;
-    for (int w = 1; w < waves; ++w)
-      insert_keys(list[0], lists[w * kWave + lane], p.TOP, short_list);
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+      if (i % waves == wave)
+        for (int w = 0; w < waves; ++w)
+          if (w != wave) insert_keys(list[i], lists[(w * Q + i) * kWave + lane], p.TOP, short_list);
   }
   if (!live) return;
 #pragma unroll
   for (int i = 0; i < Q; ++i) {
+    if (SPLIT && i % waves != wave) continue;
     if (row0 + i >= p.rows_per_batch || lane >= p.TOP) continue;
     const int64_t low = p.ring ? t[i] / p.BS - p.NB + 1 : 0;
     const int64_t at =
@@ -328,23 +337,41 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
   }
 }
 
+template <typename TQ, int P, int Q>
+hipError_t launch_split(RouteParams& p, int64_t B, int waves, size_t shared, hipStream_t stream) {
+  p.groups_per_batch = (p.rows_per_batch + Q - 1) / Q;
+  p.groups = static_cast<uint32_t>(B * p.groups_per_batch);
+  p.by_groups = FastDiv(p.groups_per_batch);
+  RLM_TRY(check_launch("block_route", p.groups, waves * kWave));
+  const size_t bytes =
+      shared + sizeof(double) * Q * p.H * p.HD + sizeof(uint64_t) * waves * Q * kWave;
+  hipLaunchKernelGGL((route_kernel<TQ, P, Q, true>), dim3(p.groups), dim3(waves * kWave), bytes,
+                     stream, p);
+  return launch_status("block_route");
+}
+
+// Waves that the chip holds at this register count, four to a SIMD.  Measured, all queries at the
+// caches' end, router of 4 x 16 (us: one query to a workgroup with all its waves / four queries
+// with as many waves as are resident / four queries to a wave):
+//     64 blocks    256 queries: 8.4 / 11.0 / 17.0    1024: 12.0 / 11.4 / 17.2    4096: 29 / 18 / 17
+//    512 blocks    256: 18.7 / 23 / 107              1024: 52 / 24 / 108         4096: 191 / 57 / 109
+//   2048 blocks    256: 38 / 58 / 393                1024: 127 / 60 / 396        4096: 491 / 193 / 398
+//   2048 blocks    16384: 1942 / 716 / 717
+constexpr int kResident = 4096;
 template <typename TQ, int P>
 hipError_t launch_route(RouteParams& p, int64_t B, hipStream_t stream) {
   const int RD = p.H * p.HD;
   const size_t shared = sizeof(double) * (p.H + static_cast<size_t>(p.H) * p.RB);
-  // Up to two queries per CU a workgroup takes one query, its waves sharing the blocks.
-  if (B * p.rows_per_batch <= 512 || RD > 256) {
-    p.groups_per_batch = p.rows_per_batch;
-    p.groups = static_cast<uint32_t>(B * p.groups_per_batch);
-    p.by_groups = FastDiv(p.groups_per_batch);
-    const int rounds = (p.NB + kWave / P - 1) / (kWave / P);
-    const int waves = std::min(16, std::max(1, rounds));
-    const size_t bytes = shared + sizeof(double) * RD + sizeof(uint64_t) * waves * kWave;
-    RLM_TRY(check_launch("block_route", p.groups, waves * kWave));
-    hipLaunchKernelGGL((route_kernel<TQ, P, 1, true>), dim3(p.groups), dim3(waves * kWave), bytes,
-                       stream, p);
-    return launch_status("block_route");
-  }
+  const int64_t queries = B * p.rows_per_batch;
+  const int passes = (p.NB + kWave / P - 1) / (kWave / P);
+  const int most = std::min(16, passes);
+  // One query to a workgroup while all its waves are resident: the shortest chain.  Also where a
+  // batch row has fewer than the four queries that share its statistics (a decode batch).
+  if (queries * most <= kResident || p.rows_per_batch < 4 || RD > 256)
+    return launch_split<TQ, P, 1>(p, B, most, shared, stream);
+  int waves = 1;
+  while (2 * waves <= most && queries / 4 * waves < kResident) waves *= 2;
+  if (waves > 1) return launch_split<TQ, P, 4>(p, B, waves, shared, stream);
   constexpr int kWaves = 4, kQueries = 4;
   p.groups_per_batch = (p.rows_per_batch + kQueries - 1) / kQueries;
   p.groups = static_cast<uint32_t>(B * p.groups_per_batch);

@@ -87,6 +87,36 @@ def test_decode_form(device, batch, blocks, top, slots, dtype):
         check(got, [w[:, 0] if slots > 1 else w[:, 0, 0] for w in want])
 
 
+@pytest.mark.parametrize("queries,blocks,head_dim,top", [
+    (256, 300, 16, 9), (257, 300, 16, 9),        # one query / four to a workgroup, 16 waves
+    (1030, 300, 16, 64), (1030, 300, 12, 20),    # four, fewer waves; a lane to a block
+    (4095, 16, 16, 3), (4097, 16, 16, 3),        # one wave for all blocks: one query / four
+    (17000, 40, 16, 5),                          # four queries to a wave
+])
+def test_queries_that_share_workgroups(device, queries, blocks, head_dim, top):
+    g = torch.Generator().manual_seed(queries)
+    x = inputs(g, 1, queries, 1, 2, head_dim, blocks, 9, torch.bfloat16)
+    positions = torch.randint(-1, blocks * 8 + 20, (1, queries), generator=g)
+    got = block_route_seq(x["query"][:, :, 0].to(device), *(x[k].to(device) for k in
+                                                            ("mean", "std", "gamma", "bias")),
+                          positions.to(device), 8, 20, top, False)
+    torch.cuda.synchronize()
+    check(got, [w[:, :, 0] for w in oracle(x, positions.numpy(), 8, 20, top, False)])
+
+
+@pytest.mark.parametrize("batch,blocks", [(300, 300), (4100, 16)])
+def test_large_decode_batches(device, batch, blocks):
+    g = torch.Generator().manual_seed(batch)
+    x = inputs(g, batch, 1, 1, 2, 16, blocks, 9, torch.bfloat16)
+    position = torch.randint(0, blocks * 8, (batch,), generator=g)
+    got = block_route(x["query"][:, 0, 0].to(device), *(x[k].to(device) for k in
+                                                        ("mean", "std", "gamma", "bias")),
+                      position.to(device), 8, 20, 4, False)
+    torch.cuda.synchronize()
+    want = oracle(x, position.numpy()[:, None], 8, 20, 4, False)
+    check(got, [w[:, 0, 0] for w in want])
+
+
 @pytest.mark.parametrize("strict", [False, True])
 @pytest.mark.parametrize("t", [-1, 0, 31, 32, 500, 511, 512, 700, 4095, 2**35 + 3])
 def test_ring(device, t, strict):
