@@ -106,6 +106,20 @@ def test_gated_residual_norm(device, case, dtype):
     check(got, *args, dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [520, 768, 1016, 2040])
+@pytest.mark.parametrize("rows", [1024, 1025])
+def test_rows_on_a_wave_and_on_a_workgroup(device, rows, width, dtype):
+    """Up to 1024 rows of more than 64 accesses have a workgroup each, more of them a wave each."""
+    g = torch.Generator().manual_seed(rows + width)
+    branch, residual = (torch.randn(rows, width, generator=g).to(dtype) for _ in range(2))
+    weight, bias, post = (torch.randn(width, generator=g).to(dtype) for _ in range(3))
+    args = (branch, residual, torch.tensor(0.4), weight, bias, 1e-5, post, None, 1.5, False, 1e-5)
+    got = gated_residual_norm(*(x.to(device) if isinstance(x, torch.Tensor) else x for x in args))
+    torch.cuda.synchronize()
+    check(got, *args, dtype)
+
+
 def test_strided_rows_and_mixed_parameters(device):
     g = torch.Generator().manual_seed(2)
     for dtype, skip in ((torch.bfloat16, 8), (torch.bfloat16, 3), (torch.float32, 4)):
