@@ -17,6 +17,10 @@
 //
 // Bound: the latency of three dependent reads (positions and picks; keys and values; the merge
 // of the waves), and the memory's rate for large batches: every row is read once per key head.
+// 8 queries of 9 heads on 3 of 64 features, a window of 64 and four blocks of 32: 5.2 us.  20
+// queries of 32 heads on 4 of 128 over caches of 131072 rows, a window of 512 and 16 blocks of 64:
+// 20.3 us, 3.1 TB/s of the rows it needs.  With one head to a key head only one of a product's 16
+// rows is used: 666 fp32 queries of 8 heads of 32, 32.8 us, two thirds of the issue slots taken.
 #include "rlm_attention.hpp"
 #include "rlm_attention_mfma.hpp"
 

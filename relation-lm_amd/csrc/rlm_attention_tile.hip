@@ -19,6 +19,13 @@
 // the LDS cycles (4 x 4096 queries) still count as conflicts; an exchange that gives the transposing
 // reads columns of their own too left that count and the time as they were.
 //
+// Bound: waits.  4 x 4096 queries of 12 heads on 4 of 64 features (a window of 128, eight blocks of
+// 64) take 110 us and 8192 of 16 on 2 of 128 (256, eight) 124 us: 270 and 400 TFLOP/s over the keys
+// that each query sees.  A wave's rows see about twice the tiles that one query does, and a
+// workgroup's 1.4 times those of a wave; the waves spend half their life at the loads' wait and the
+// barrier of each tile, with VALU issuing 60% and the matrix cores busy 23% of the time.  Taking a
+// tenth of the VALU instructions out left the time as it was.
+//
 // The weights are rounded to the 16-bit type for the second product (half a step, relative to
 // each weight); scores, maxima, sums and outputs stay fp32.
 //

@@ -7,7 +7,9 @@
 //
 // The score is formed in float64: two blocks are ranked by their fp32 scores, so a score has
 // to be right to its rounding or equal inputs would not tie.  Bound: VALU issue of the float64
-// products and of the exponentials, 2 RD products and H exponentials per (query, block).
+// products and of the exponentials, 2 RD products and H exponentials per (query, block): 4 x 4096
+// queries over up to 64 blocks (router of 4 x 16) take 24.2 us, 85% of them issuing (2760
+// instructions a wave).  8 queries over 16 blocks take 6.0 us, one wave's chain.
 // A wave takes Q queries of one batch row over 64 / P blocks at a time, P lanes to a block;
 // each statistics access (16 bytes a lane, P lanes together) then serves Q queries.  Where there
 // are too few queries to fill the chip, a workgroup's waves share the blocks of its queries
