@@ -23,7 +23,7 @@
 // 64) take 110 us and 8192 of 16 on 2 of 128 (256, eight) 124 us: 270 and 400 TFLOP/s over the keys
 // that each query sees.  A wave's rows see about twice the tiles that one query does, and a
 // workgroup's 1.4 times those of a wave; the waves spend half their life at the loads' wait and the
-// barrier of each tile, with VALU issuing 60% and the matrix cores busy 23% of the time.  Taking a
+// barrier of each tile, with VALU issuing 61% and the matrix cores busy 24% of the time.  Taking a
 // tenth of the VALU instructions out left the time as it was.
 //
 // The weights are rounded to the 16-bit type for the second product (half a step, relative to

@@ -177,6 +177,19 @@ def test_widest_tables(device):
     check(got, [w[:, :, 0] for w in oracle(x, positions.numpy(), 7, 9, 11, False)])
 
 
+@pytest.mark.parametrize("queries,blocks", [(300, 300), (17000, 20), (200, 300)])
+def test_widest_router_with_most_buckets(device, queries, blocks):
+    """16 heads of 16 with 128 buckets: the most shared memory of each launch form."""
+    g = torch.Generator().manual_seed(queries)
+    x = inputs(g, 1, queries, 1, 16, 16, blocks, 128, torch.bfloat16)
+    positions = torch.randint(0, blocks * 8, (1, queries), generator=g)
+    got = block_route_seq(x["query"][:, :, 0].to(device), *(x[k].to(device) for k in
+                                                            ("mean", "std", "gamma", "bias")),
+                          positions.to(device), 8, 20, 64, False)
+    torch.cuda.synchronize()
+    check(got, [w[:, :, 0] for w in oracle(x, positions.numpy(), 8, 20, 64, False)])
+
+
 @pytest.mark.parametrize("queries", [1, 600])
 @pytest.mark.parametrize("ring", [False, True])
 def test_ties_go_to_the_lowest_block(device, queries, ring):

@@ -314,3 +314,37 @@ def test_leading_dims_of_the_norm(device):
     across = x.permute(3, 0, 1, 2, 4)           # no view as rows: copied
     c = gated_residual_norm(across, across, gate.permute(3, 0, 1, 2, 4), w, None, 1e-5)
     assert torch.equal(c[1], a[1].permute(3, 0, 1, 2, 4))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_calls_without_rows(device, dtype):
+    """No queries, no batch rows, a cache without rows, no picks: outputs of the right shapes, and
+    where there are queries, ones that saw nothing."""
+    def some(*shape):
+        return torch.randn(*shape, device=device).to(dtype)
+
+    positions = torch.zeros(0, dtype=torch.int64, device=device)
+    out, lse = routed_attention_seq(some(2, 0, 4, 32), some(2, 8, 2, 32), some(2, 8, 2, 32),
+                                    torch.zeros(2, 0, 3, dtype=torch.int32, device=device),
+                                    positions, 4, 4)
+    assert out.shape == (2, 0, 4, 32) and lse.shape == (2, 0, 4)
+    at = torch.tensor(3, device=device)
+    for batch, rows, top in ((0, 8, 3), (2, 0, 3), (2, 0, 0)):
+        picks = torch.zeros(batch, top, dtype=torch.int32, device=device)
+        out, lse = routed_attention(some(batch, 4, 32), some(batch, rows, 2, 32),
+                                    some(batch, rows, 2, 32), picks, at, 4, 4)
+        assert (out == 0).all() and torch.isneginf(lse).all() and out.shape == (batch, 4, 32)
+    freq = torch.ones(16, device=device)
+    q, k = rotary_positions(some(2, 0, 4, 32), some(2, 0, 2, 32), positions, freq)
+    assert q.shape == (2, 0, 4, 32) and k.shape == (2, 0, 2, 32)
+    cache = some(2, 0, 2, 32)
+    query = some(2, 1, 4, 32)
+    turned = rotary_to_caches(query, some(2, 1, 2, 32), some(2, 1, 2, 32),
+                              torch.tensor(0, device=device), freq, cache, cache.clone())
+    assert torch.equal(turned, query)          # position 0, and no cache row to write
+    blocks, scores = block_route_seq(some(2, 0, 32), torch.zeros(2, 3, 2, 16, device=device),
+                                     torch.zeros(2, 3, 2, 16, device=device),
+                                     torch.zeros(2, device=device), torch.zeros(2, 5, device=device),
+                                     positions, 4, 4, 2, False)
+    assert blocks.shape == scores.shape == (2, 0, 2)
+    torch.cuda.synchronize()
