@@ -3,7 +3,7 @@
 //
 // A workgroup has up to 16 query heads of one query and key head (the rows or columns of a
 // matrix product) and shares the query's keys among its waves, 32 at a time; where there are fewer
-// such items than half the CUs, workgroups share the value features of each.  The keys are one
+// such items than half the CUs (fp32: see below), workgroups share the value features of each.  The keys are one
 // list: the window's positions, then every picked block's; a lane finds one of a tile's keys
 // -- its cache row and whether it counts -- and hands it to the lanes that load it, so blocks
 // shorter than a tile share one.  A key that does not count (past the position, in the window
@@ -19,8 +19,8 @@
 // of the waves), and the memory's rate for large batches: every row is read once per key head.
 // 8 queries of 9 heads on 3 of 64 features, a window of 64 and four blocks of 32: 5.2 us.  20
 // queries of 32 heads on 4 of 128 over caches of 131072 rows, a window of 512 and 16 blocks of 64:
-// 20.3 us, 3.1 TB/s of the rows it needs.  With one head to a key head only one of a product's 16
-// rows is used: 666 fp32 queries of 8 heads of 32, 32.8 us, two thirds of the issue slots taken.
+// 19.8 us, 3.2 TB/s of the rows it needs.  With one head to a key head only one of a product's 16
+// rows is used: 666 fp32 queries of 8 heads of 32, 32.3 us, two thirds of the issue slots taken.
 #include "rlm_attention.hpp"
 #include "rlm_attention_mfma.hpp"
 
@@ -34,7 +34,7 @@ constexpr int kKeys = 32;  // keys of a wave's tile
 template <typename T>
 constexpr bool kIs32 = sizeof(T) == 4;
 
-__device__ const uint4 zeros = {0, 0, 0, 0};
+__device__ const uint4 zeros[64] = {};  // a row of values
 
 // DC: head dim in 32s; PARTS workgroups have a share of the value features each.
 template <typename T, int DC, int MAXW, int PARTS>
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
         const int piece = (lane % kPitch) ^ swizzle<kPitch>(to);
         const T* src = vbase + static_cast<int64_t>(__shfl(row, to, kWave)) * p.v_st +
                        (first + 8 * piece < D ? first + 8 * piece : 0);
-        src = (mask >> to) & 1 ? src : reinterpret_cast<const T*>(&zeros);
+        src = (mask >> to) & 1 ? src : reinterpret_cast<const T*>(zeros);
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) void*)(src),
             (__attribute__((address_space(3))) void*)static_cast<uintptr_t>(mine + i * kWave * 16), 16, 0, 0);
@@ -163,11 +163,11 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_query_kernel(Params p) {
         for (int i = 0; i < 4; ++i) {
           const T* src =
               vbase + static_cast<int64_t>(__shfl(row, 16 * kt + 4 * quad + i, kWave)) * p.v_st;
+          src = (mask >> (16 * kt + 4 * quad + i)) & 1 ? src : reinterpret_cast<const T*>(zeros);
 #pragma unroll
           for (int j = 0; j < DT; ++j) {
             const int d = first + 16 * j + r;
-            const float v = src[d < D ? d : 0];
-            vs[j][kt][i] = (mask >> (16 * kt + 4 * quad + i)) & 1 ? v : 0.0f;
+            vs[j][kt][i] = src[d < D ? d : 0];
           }
         }
     }
@@ -296,34 +296,52 @@ hipError_t launch(const Params& p, hipStream_t stream) {
   return launch_status("routed_attention");
 }
 
-// Parts of the value features: as many as leave every workgroup a CU of its own.  Each part
-// computes the weights anew and reads the keys again (from the L2 that they share), but its
-// values, its sums and their merge are the shorter for it.  Measured, one part / two / four (us;
-// a window of 512 and 16 blocks of 64):
+// Parts of the value features.  Each part computes the weights anew and reads the keys again (from
+// the L2 that they share), but its values, its sums and their merge are the shorter for it.
+// As many as leave every workgroup a CU of its own.  Measured, one part / two / four (us; single
+// tokens, a window of 512 and 16 blocks of 64):
 //   bf16, 128 features    8 items: 20.9 / 17.3 / 15.6    64: 24.1 / 19.5 / 17.7
 //                         128: 26.1 / 21.9               192: 31.1 / 42.8
-//   fp32, 128 features    8 items: 63 / 47 / 31          64: 126 / 82 / 35    192: 176 / 209
 //   bf16, 64 features     8 items: 11.6 / 10.6           128: 13.3 / 13.3
+//   fp32, 64 features     8 items: 25.8 / 21.5           128: 28.9 / 24.6    256: 35 / 50
+// fp32 beyond 64 features fills the registers with a tile's keys and values.  96 and 128 features
+// take three and four parts while two workgroups to a CU hold them (one part / all):
+//   128 features    8 items: 54 / 31    128: 95 / 56    132: 98 / 97    512: 294 / 359
+//                   256 items that are 64 neighbouring queries: 27 / 49
+//    96 features    8 items: 44 / 27    128: 75 / 49    256 items of neighbours: 27 / 34
+// 256 features always take two, one part spilling (8 items: 221 / 67; 4096: 6274 / 3278).
+// Waves: sixteen, but eight where sixteen would spill (bf16, 128 features, one part, 16 / 8 waves:
+// 256 items 40 / 34, 1024 162 / 153; two parts, 128 items 21.9 / 20.2; four parts fit, and 64 items
+// of 5120 keys take 47 / 54).
 constexpr int kUnits = 256;  // compute units
-template <typename T, int DC, int MAXW>
+template <typename T, int DC>
 hipError_t launch_parts(const Params& p, hipStream_t stream) {
-  const uint32_t room = kUnits / p.items;
-  if constexpr (DC >= 4)
-    if (room >= 4) return launch<T, DC, MAXW, 4>(p, stream);
-  if constexpr (DC == 3)
-    if (room >= 3) return launch<T, DC, MAXW, 3>(p, stream);
-  if constexpr (DC % 2 == 0)
-    if (room >= 2) return launch<T, DC, MAXW, 2>(p, stream);
-  return launch<T, DC, MAXW, 1>(p, stream);
+  if constexpr (kIs32<T> && DC == 8) {
+    return launch<T, DC, 8, 2>(p, stream);
+  } else if constexpr (kIs32<T> && DC >= 3) {
+    return DC * p.items <= 2 * kUnits ? launch<T, DC, 8, DC>(p, stream)
+                                      : launch<T, DC, 8, 1>(p, stream);
+  } else {
+    constexpr int kWaves = DC == 8 || (kIs32<T> && DC == 2) ? 8 : 16;
+    constexpr int kFewer = DC == 4 ? 8 : kWaves;
+    const uint32_t room = kUnits / p.items;
+    if constexpr (DC >= 4)
+      if (room >= 4) return launch<T, DC, kWaves, 4>(p, stream);
+    if constexpr (DC == 3)
+      if (room >= 3) return launch<T, DC, kWaves, 3>(p, stream);
+    if constexpr (DC % 2 == 0)
+      if (room >= 2) return launch<T, DC, kFewer, 2>(p, stream);
+    return launch<T, DC, kFewer, 1>(p, stream);
+  }
 }
-template <typename T, int WIDE>
+template <typename T>
 hipError_t launch_type(const Params& p, hipStream_t stream) {
   const int dc = (p.D + 31) / 32;
-  if (dc <= 1) return launch_parts<T, 1, 16>(p, stream);
-  if (dc <= 2) return launch_parts<T, 2, WIDE>(p, stream);
-  if (dc <= 3) return launch_parts<T, 3, WIDE>(p, stream);
-  if (dc <= 4) return launch_parts<T, 4, WIDE>(p, stream);
-  return launch_parts<T, 8, 8>(p, stream);
+  if (dc <= 1) return launch_parts<T, 1>(p, stream);
+  if (dc <= 2) return launch_parts<T, 2>(p, stream);
+  if (dc <= 3) return launch_parts<T, 3>(p, stream);
+  if (dc <= 4) return launch_parts<T, 4>(p, stream);
+  return launch_parts<T, 8>(p, stream);
 }
 
 }  // namespace
@@ -331,9 +349,9 @@ hipError_t launch_type(const Params& p, hipStream_t stream) {
 namespace attention {
 
 hipError_t query_launch(const Params& p, int dtype, hipStream_t stream) {
-  if (dtype == RLM_F32) return launch_type<float, 8>(p, stream);
-  if (dtype == RLM_BF16) return launch_type<bf16, 16>(p, stream);
-  return launch_type<f16, 16>(p, stream);
+  if (dtype == RLM_F32) return launch_type<float>(p, stream);
+  if (dtype == RLM_BF16) return launch_type<bf16>(p, stream);
+  return launch_type<f16>(p, stream);
 }
 
 }  // namespace attention

@@ -303,7 +303,7 @@ def test_decode_form(device, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("items", [64, 65, 85, 86, 128, 129, 257])
+@pytest.mark.parametrize("items", [64, 65, 85, 86, 128, 129, 170, 171, 257])
 @pytest.mark.parametrize("dim", [40, 72, 96, 104, 136, 200])
 def test_features_shared_by_workgroups(device, dim, items, dtype):
     """Both sides of every number of (row, key head) items where the value features are shared
