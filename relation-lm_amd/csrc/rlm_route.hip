@@ -287,7 +287,8 @@ __global__ __launch_bounds__(SPLIT ? 1024 : 256, 4) void route_kernel(RouteParam
           most[k] = x;
           sum[k] = 1.0;
         } else {
-          const double e = exp_down(-fabs(x - most[k]));
+          // (Equal terms may be infinite: their difference is none, not inf - inf.)
+          const double e = exp_down(x == most[k] ? 0.0 : -fabs(x - most[k]));
           sum[k] = x > most[k] ? fma(sum[k], e, 1.0) : sum[k] + e;
           most[k] = x > most[k] ? x : most[k];
         }
