@@ -77,15 +77,20 @@ __device__ __forceinline__ void insert_keys(uint64_t& list, uint64_t key, int to
   }
 }
 
-// exp(x) for x <= 0 to 1e-11, NaN for NaN: x = k ln 2 + r with |r| <= ln 2 / 2, the Taylor
-// polynomial of degree 9 in r (its remainder is r^10 / 10! < 7e-12).  A score is rounded to fp32
-// (6e-8) once; two blocks with equal inputs run the same steps and tie.
+// exp(x) for x <= 0 to 4e-16, NaN for NaN: x = k ln 2 + r with |r| <= ln 2 / 2, the Taylor
+// polynomial of degree 12 in r (its remainder is r^13 / 13! < 2e-16).  The score is rounded to fp32
+// after it, as the selection's is, whose exponentials are float64 ones: a polynomial that stops at
+// 1e-11 rounded some 4e-6 of the scores to another number and picked other blocks than the
+// selection where two scores are next to each other.
 __device__ __forceinline__ double exp_down(double x) {
   x = x < -700.0 ? -700.0 : x;  // 1e-304: nothing beside a sum of at least 1
   const double k = rint(x * 1.44269504088896340736);
-  double r = fma(k, -6.93147180369123816490e-01, x);  // ln 2: 33 bits, and the rest
-  r = fma(k, -1.90821492927058770002e-10, r);
-  double y = 1.0 / 362880.0;
+  double r = fma(k, -0x1.62e42fefap-1, x);  // ln 2: its first 36 bits (k takes 10), and the rest
+  r = fma(k, -0x1.cf79abc9e3b3ap-40, r);
+  double y = 1.0 / 479001600.0;
+  y = fma(y, r, 1.0 / 39916800.0);
+  y = fma(y, r, 1.0 / 3628800.0);
+  y = fma(y, r, 1.0 / 362880.0);
   y = fma(y, r, 1.0 / 40320.0);
   y = fma(y, r, 1.0 / 5040.0);
   y = fma(y, r, 1.0 / 720.0);
@@ -97,8 +102,8 @@ __device__ __forceinline__ double exp_down(double x) {
   y = fma(y, r, 1.0);
   return ldexp(y, static_cast<int>(k));
 }
-// log(s) for s >= 1: the fp32 logarithm y, corrected by log(s exp(-y)) = z - z^2 / 2 + O(z^3),
-// |z| <= 1e-6.
+// log(s) for s >= 1 to 8e-16: the fp32 logarithm y, corrected by log(s exp(-y)) = z - z^2 / 2 +
+// O(z^3), |z| <= 1e-6.
 __device__ __forceinline__ double log_up(double s) {
   const double y = static_cast<double>(__builtin_amdgcn_logf(static_cast<float>(s)) * 0.69314718055994530942f);
   const double z = fma(s, exp_down(-y), -1.0);
