@@ -799,8 +799,9 @@ hipError_t rlm_rotary_positions(const rlm_tensor* query, const rlm_tensor* key,
  * value [B,Tq,Hk,D] written to row position[b] + i of key_cache / value_cache
  * [B,T,Hk,D] (mutated; any non-overlapping strides) instead of an output.
  * Positions outside [0, T) and tokens from lengths[b] on (lengths [B] or NULL)
- * leave the caches as they are.  ring: row (position[b] + i) mod T for any
- * position >= 0, T a power of two, Tq <= T.
+ * leave the caches as they are, and so do tokens past int64's last position, which
+ * turn as that one does.  ring: row (position[b] + i) mod T for any position >= 0, T
+ * a power of two, Tq <= T.
  */
 hipError_t rlm_rotary_to_caches(const rlm_tensor* query, const rlm_tensor* key,
                                 const rlm_tensor* value, const rlm_tensor* position,

@@ -70,9 +70,11 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
     uint32_t f, step;
     const uint32_t local = p.by_pairs.div(i, f);
     const uint32_t b = p.by_queries.div(first + local, step);
-    int64_t at = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_st);
+    // (Sums of float64 numbers do not pass the end of int64; exact up to 2^53.)
+    double at = static_cast<double>(
+        load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_st));
     if (p.to_cache) at += step;
-    const double turns = static_cast<double>(at) * static_cast<double>(p.freq[f]) *
+    const double turns = at * static_cast<double>(p.freq[f]) *
                          0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
@@ -83,7 +85,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
     const uint32_t b = p.by_queries.div(first + threadIdx.x, step);
     int64_t row = step;
     if (p.to_cache) {
-      const int64_t at = load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_st) + step;
+      // Past the end of int64 the sum wraps to a negative position, which is not written.
+      const int64_t at = static_cast<int64_t>(
+          static_cast<uint64_t>(load_any_i(p.pos, p.pos_dtype, b * p.pos_sb + step * p.pos_st)) +
+          step);
       const bool real =
           p.lengths == nullptr || static_cast<int64_t>(step) < load_any_i(p.lengths, p.lengths_dtype, b);
       row = p.ring ? (at & (p.rows - 1)) : at;

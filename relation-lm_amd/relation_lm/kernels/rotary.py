@@ -40,7 +40,8 @@ def rotary_to_caches(query: Tensor, key: Tensor, value: Tensor, position: Tensor
     ``value_cache`` [B,T,Hk,D] (any strides with unit stride in D).
 
     Tokens from ``lengths[b]`` on (padding of a ragged prompt batch) and positions
-    outside [0, T) leave the caches as they are.  ``ring``: position p goes to row
+    outside [0, T) leave the caches as they are, and so do tokens that would stand past
+    int64's last position (they turn as that one does).  ``ring``: position p goes to row
     p mod T, T a power of two, Tq <= T.  A decode step passes Tq = 1.
     """
     return torch.ops.rlm.rotary_to_caches(query, key, value, position, frequencies, key_cache,
