@@ -782,7 +782,7 @@ hipError_t rlm_block_statistics(const rlm_tensor* keys, int64_t block_size,
 /*
  * Rotary positions of query [B,Tq,Hq,D] and key [B,Tq,Hk,D]: pair i of a head
  * turns by position * frequencies[i] (frequencies [F] f32, 2 F <= D; the angle
- * is reduced in float64), both features times `scale`:
+ * is reduced in float64, its sine and cosine are fp32), both features times `scale`:
  *   (a, b) -> scale * (a cos - b sin, a sin + b cos).
  * Pair i is the features (i, F + i), or (2 i, 2 i + 1) where `interleaved`;
  * features from 2 F on pass unchanged.  D <= 1024.
@@ -813,8 +813,8 @@ hipError_t rlm_rotary_to_caches(const rlm_tensor* query, const rlm_tensor* key,
 /*
  * The block router by itself: for each query the top_blocks best complete
  * blocks (strict: complete blocks wholly before the local window), with the
- * scores and the tie rule of rlm_relation_select_packed: score descending, ties
- * to the lowest block.
+ * scores and the tie rule of rlm_relation_select_packed: float64 log-sum-exps,
+ * rounded to fp32 once; score descending, ties to the lowest block.
  *   router_query [B,Tq,S,RD], block_mean/std [B,NB,H,HD] f32 (H*HD == RD <= 1024,
  *   HD a multiple of 4), gamma [H], bias [H,RB] (H*RB <= 2048), top_blocks in
  *   [1, 64].  ring: slot j holds the newest block of index j mod NB (NB and
@@ -841,9 +841,12 @@ hipError_t rlm_block_route(const rlm_tensor* router_query, const rlm_tensor* blo
  * of 8 up to 256; 16-byte aligned, strides multiples of 8 elements.  A position
  * counts once however often it is named; picks outside the cache (-1) name
  * nothing.  A query that sees no position gives 0 and lse -inf; what the caches
- * hold in rows that a query does not see does not reach it.
- * ring: position p in row p mod T, positions (t - T, t] held; T a power of two
- * and a multiple of block_size.
+ * hold in rows that a query does not see does not reach it.  Scores, their
+ * exponentials and sums are fp32; in the 16-bit types each weight is rounded to
+ * the type (bf16: by 2^-8 of itself at most) before it meets the values.
+ * ring: position p in row p mod T, positions (t - T, t] held for every query's t; T
+ * a power of two and a multiple of block_size.  Queries of several positions need
+ * caches in which no row that one of them sees holds a later position yet.
  * Outputs: out [B,Tq,Hq,D] in query's dtype, out_lse f32 [B,Tq,Hq].
  */
 hipError_t rlm_routed_attention(const rlm_tensor* query, const rlm_tensor* key_cache,

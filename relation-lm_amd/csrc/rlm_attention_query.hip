@@ -1,5 +1,5 @@
-// Attention over a window and picked blocks, one query to a workgroup: single tokens, fp32, and
-// prompts that the shared tiles (rlm_attention_tile.hip) do not take.
+// Attention over a window and picked blocks, one query to a workgroup: single tokens, ring caches, and
+// prompts that the shared tiles (rlm_attention_tile.hip) do not take or that are faster here.
 //
 // A workgroup has up to 16 query heads of one query and key head (the rows or columns of a
 // matrix product) and shares the query's keys among its waves, 32 at a time; where there are fewer
@@ -14,6 +14,11 @@
 // from memory into operands, 16-bit values through a piece of LDS of the wave's own for the
 // transposing reads.  fp32 uses v_mfma_f32_16x16x4_f32, whose operands need no transposing: the
 // features of the first product are summed in an order that gives a lane four neighbours.
+//
+// 16-bit types: the weights are rounded to the type for the second product, which takes no other
+// operands (half a step, relative to each weight; the outputs of the measured cases are 0.0020 to 0.0021
+// off in bf16, where weights of 32 bits would leave the output's own rounding, 0.0016); scores, maxima,
+// sums and outputs stay fp32.
 //
 // Bound: the latency of three dependent reads (positions and picks; keys and values; the merge
 // of the waves), and the memory's rate for large batches: every row is read once per key head.
@@ -312,7 +317,8 @@ hipError_t launch(const Params& p, hipStream_t stream) {
 // 256 features always take two, one part spilling (8 items: 221 / 67; 4096: 6274 / 3278).
 // Waves: sixteen, but eight where sixteen would spill (bf16, 128 features, one part, 16 / 8 waves:
 // 256 items 40 / 34, 1024 162 / 153; two parts, 128 items 21.9 / 20.2; four parts fit, and 64 items
-// of 5120 keys take 47 / 54).
+// of 5120 keys take 47 / 54).  At 256 features one part of eight waves still spills 3 registers; single
+// tokens over 512 keys: 256 items 25.3, 512 50, 1024 107, 4096 378.
 constexpr int kUnits = 256;  // compute units
 template <typename T, int DC>
 hipError_t launch_parts(const Params& p, hipStream_t stream) {

@@ -20,14 +20,15 @@
 // reads columns of their own too left that count and the time as they were.
 //
 // Bound: waits.  4 x 4096 queries of 12 heads on 4 of 64 features (a window of 128, eight blocks of
-// 64) take 110 us and 8192 of 16 on 2 of 128 (256, eight) 124 us: 270 and 400 TFLOP/s over the keys
-// that each query sees.  A wave's rows see about twice the tiles that one query does, and a
+// 64) take 110 us and 8192 of 16 on 2 of 128 (256, eight) 124 us: 260 and 400 TFLOP/s over the keys
+// that each query sees (567 and 730 on average).  A wave's rows see about twice the tiles that one query does, and a
 // workgroup's 1.4 times those of a wave; the waves spend half their life at the loads' wait and the
 // barrier of each tile, with VALU issuing 61% and the matrix cores busy 24% of the time.  Taking a
 // tenth of the VALU instructions out left the time as it was.
 //
-// The weights are rounded to the 16-bit type for the second product (half a step, relative to
-// each weight); scores, maxima, sums and outputs stay fp32.
+// The weights are rounded to the 16-bit type for the second product, which takes no other operands
+// (half a step, relative to each weight: the measured outputs are 0.0021 off in bf16, where weights of
+// 32 bits would leave the output's own rounding, 0.0016); scores, maxima, sums and outputs stay fp32.
 //
 // A masked key's weight is 0, which is no protection from what its value row holds if that is
 // an infinity or NaN (0 x inf): a row whose sums are not finite at the end is computed again,
@@ -559,6 +560,13 @@ hipError_t launch(TileParams& tp, hipStream_t stream) {
 // Fewer waves share a tile's loads with fewer queries but wait for fewer of them: what counts is
 // the number of workgroups on a CU (four).  One tile in LDS (seven fit) 120 / 144: registers
 // still allow only four.  Three in LDS (two or three workgroups) 179 / 207.
+// WHOLE by multiples of 64, the largest tile, whatever the instance's own.  Other blocks take the form
+// that looks up the picks per 16 keys and spills registers above 96 features (bf16 and fp16 20, fp32 30;
+// 5 at fp32 above 128).  Measured, as many keys in blocks of 64 / 32 / 16 (us, bf16): 4 x 4096 queries of 12
+// heads on 4 of 64 features 115 / 164 / 181, 8192 of 16 on 2 of 128 121 / 160 / 230, of 96 - / 123 / -; fp32, 2
+// x 4096 of 8 on 4 of 128 535 / 617 / -.  8 x 512 queries of 12 on 4 of 64, blocks of 32: 16.8.  Tiles of 32 keys
+// would take blocks of 32 in the WHOLE form as well: 8192 queries 160 -> 119 (128 features), 123 -> 104
+// (96), fp32 617 -> 514, 2 x 4096 of 8 on 2 of 256 173 -> 138; fp32 of 64 features 284 -> 275.
 template <typename T, bool WHOLE>
 hipError_t launch_type(TileParams& tp, hipStream_t stream) {
   constexpr int kSmall = sizeof(T) == 4 ? 32 : 64;

@@ -7,7 +7,7 @@
 //
 // Bound: memory, two rows read and two written for each row: 16384 rows of 768 bf16 features take
 // 22.2 us, 4.5 TB/s, where a large copy reaches 4.7; few rows take the chain of their reads and four
-// sums, 3.5 us for 8 of 576.  The statistics are wave reductions over a row held in registers, the
+// sums, 4.3 to 4.6 us for 8 of 576 by the profiler (3.9 at least).  The statistics are wave reductions over a row held in registers, the
 // variance in a second sweep of those registers (no cancellation between mean x^2 and mean^2).
 #include "rlm_common.hpp"
 
@@ -226,6 +226,11 @@ hipError_t launch_wide(const GatedNormParams& p, hipStream_t stream) {
   if (accesses <= 4 * kThreads) return launch<T, W, V, kThreads, 4>(p, stream);
   return launch<T, W, V, kThreads, 8>(p, stream);
 }
+// Widths, strides or addresses that are not whole 16-byte accesses: an element each, with a switch on
+// each parameter's type.  Measured (us, bf16 rows, both norms, parameters bf16 or fp32 / some of each):
+//   16384 rows of 768 features: 22.8 / 77    of 767: 57    4096 of 2048: 17.5 / 54    of 2047: 32
+// so parameters of one type are what whole accesses want: with some of each they still read the rows
+// whole, but switch for every element of every parameter.
 template <typename T>
 hipError_t launch_narrow(const GatedNormParams& p, hipStream_t stream) {
   if (p.D <= 8 * kWave) return launch<T, void, 1, kWave, 8>(p, stream);

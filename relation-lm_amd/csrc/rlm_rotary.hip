@@ -7,12 +7,20 @@
 //
 // The angle is reduced in float64 (p f_i reaches 10^6 turns far into a context, where fp32
 // has no bits left for the turn's fraction): p f_i / (2 pi) less its nearest whole number,
-// then fp32 sine and cosine of pi times that.  They depend on the token alone, so a
+// then fp32 sine and cosine of pi times that (5.6e-8 off in fp32 outputs, where float64 ones would be
+// 4.1e-8 off; half a step of a 16-bit output is 2e-3 or 2e-4).  They depend on the token alone, so a
 // workgroup computes them once for its tokens into LDS and every head reads them there.
 //
 // Bound: memory, every row read once and written once: 4 x 4096 tokens of 12 + 4 + 4 heads of 64
-// bf16 features (84 MB, which the MALL holds) into caches take 13.3 us, 6.3 TB/s; 2 x 1999 of 8 + 8
-// fp32 heads 9.4 us.  A decode step of 8 tokens takes 3.1 us, a launch and two round trips.
+// bf16 features into caches, 63% of the tokens real on average (71.5 MB, which the MALL holds), take
+// 13.2 to 14.0 us, 5.1 to 5.4 TB/s.  2 x 1999 of 8 + 8 fp32 heads, 48 of whose 64 features turn, take 9.4
+// us (3.5 TB/s) and wait (74% of the waves' life): a wave's lanes turn some pieces and copy
+// others, one after the other, each a load, its wait and a store, in seven rounds.  A decode step of 8
+// tokens takes 3.1 us, a launch and two round trips.
+//
+// Accesses are of 16 bytes where pairs, head dim, strides and addresses allow, else of one element: the
+// 4 x 4096 tokens with every token real, into caches, take 15.5 us in bf16 (26.5 in fp32), 37.2 (35.4) with
+// 31 pairs in place of 32 and 29.5 (28.5) from rows one element off; 8 single tokens 6.0 either way.
 #include "rlm_common.hpp"
 #include "rlm_fastdiv.hpp"
 

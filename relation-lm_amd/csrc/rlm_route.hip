@@ -6,10 +6,12 @@
 // floor(log2(distance + 1)) of the block's last position, ties to the lowest block.
 //
 // The score is formed in float64: two blocks are ranked by their fp32 scores, so a score has
-// to be right to its rounding or equal inputs would not tie.  Bound: VALU issue of the float64
-// products and of the exponentials, 2 RD products and H exponentials per (query, block): 4 x 4096
-// queries over up to 64 blocks (router of 4 x 16) take 24.2 us, 85% of them issuing (2760
-// instructions a wave).  8 queries over 16 blocks take 6.0 us, one wave's chain.
+// to be right to its rounding or equal inputs would not tie.  Bound: VALU issue, 85% of the time: 4 x
+// 4096 queries over up to 64 blocks (router of 4 x 16) take 24.9 us and 2860 instructions a wave.
+// Of the some 150 that a head of 64 (query, block) pairs takes, 65 are float64 arithmetic (2 RD products
+// and H exponentials per pair); the rest are conversions, the lanes' sums, the selects that give each
+// lane its own query, and addresses.  A pick of the first 64 blocks takes about 74 more.  8 queries over
+// 16 blocks take 6.1 us, one wave's chain.
 // A wave takes Q queries of one batch row over 64 / P blocks at a time, P lanes to a block;
 // each statistics access (16 bytes a lane, P lanes together) then serves Q queries.  Where there
 // are too few queries to fill the chip, a workgroup's waves share the blocks of its queries
@@ -360,11 +362,16 @@ hipError_t launch_split(RouteParams& p, int64_t B, int waves, size_t shared, hip
 
 // Waves that the chip holds at this register count, four to a SIMD.  Measured, all queries at the
 // caches' end, router of 4 x 16 (us: one query to a workgroup with all its waves / four queries
-// with as many waves as are resident / four queries to a wave):
+// with as many waves as are resident / four queries to a wave; with exponentials of degree 9, which
+// took 2 to 4% off each):
 //     64 blocks    256 queries: 8.4 / 11.0 / 17.0    1024: 12.0 / 11.4 / 17.2    4096: 29 / 18 / 17
 //    512 blocks    256: 18.7 / 23 / 107              1024: 52 / 24 / 108         4096: 191 / 57 / 109
 //   2048 blocks    256: 38 / 58 / 393                1024: 127 / 60 / 396        4096: 491 / 193 / 398
 //   2048 blocks    16384: 1942 / 716 / 717
+// Routers wider than 256 take one query to a workgroup at any number of queries, each reading all
+// statistics: four queries to each of four waves would take 128 bytes of LDS per feature.  4 x 4096
+// queries over up to 64 blocks: router of 4 x 64 46.6 us, of 5 x 64 115.8, of 8 x 64 171; 4096 queries over
+// up to 512 blocks, 4 x 64 112 and 8 x 64 525.
 constexpr int kResident = 4096;
 template <typename TQ, int P>
 hipError_t launch_route(RouteParams& p, int64_t B, hipStream_t stream) {
@@ -392,6 +399,11 @@ hipError_t launch_route(RouteParams& p, int64_t B, hipStream_t stream) {
   return launch_status("block_route");
 }
 
+// Four lanes to a block where they divide a head in 16-byte pieces, one lane otherwise; that lane has
+// four queries' sums and exponentials to itself (24 registers spilled at four queries to a wave) and
+// picks enter one by one.  4 x 4096 queries, each asking for itself, over up to 64 blocks: router of 4 x 16
+// 27 us, of 8 x 8 58.8, of 4 x 8 41.6; 4096 queries over up to 512: 4 x 16 63.8, 8 x 8 97.0; 256 queries over
+// 64: 8.8 and 11.2.
 template <typename TQ>
 hipError_t launch_route_type(RouteParams& p, int64_t B, hipStream_t stream) {
   if (p.HD % 16 == 0) return launch_route<TQ, 4>(p, B, stream);

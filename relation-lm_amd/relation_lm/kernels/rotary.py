@@ -24,7 +24,8 @@ def rotary_positions(query: Tensor, key: Tensor, positions: Tensor, frequencies:
     ``interleaved``.  ``frequencies`` is [F] fp32 with 2 F <= D: features from 2 F on
     pass unchanged.  Long contexts are a matter of ``frequencies`` (stretched, or
     stretched per pair) and ``scale``.  ``positions`` is 0-d, [Tq] or [B,Tq]; the
-    angle is reduced in float64, so far positions keep their turn's fraction.
+    angle is reduced in float64, so far positions keep their turn's fraction, and its
+    sine and cosine are fp32.
     query and key may be strided views (of one projection's rows, say).
     """
     return torch.ops.rlm.rotary_positions(query, key, positions, frequencies, interleaved, scale)
@@ -42,7 +43,8 @@ def rotary_to_caches(query: Tensor, key: Tensor, value: Tensor, position: Tensor
     Tokens from ``lengths[b]`` on (padding of a ragged prompt batch) and positions
     outside [0, T) leave the caches as they are, and so do tokens that would stand past
     int64's last position (they turn as that one does).  ``ring``: position p goes to row
-    p mod T, T a power of two, Tq <= T.  A decode step passes Tq = 1.
+    p mod T, T a power of two, Tq <= T.  A decode step passes Tq = 1; several tokens
+    written into a ring at once overwrite what the first of them could still see.
     """
     return torch.ops.rlm.rotary_to_caches(query, key, value, position, frequencies, key_cache,
                                           value_cache, interleaved, scale, ring, lengths)

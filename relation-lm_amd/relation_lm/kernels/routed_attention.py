@@ -59,7 +59,10 @@ def routed_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, bloc
     with unit stride in D), blocks int32 [B,TOP] or, with picks per key head, [B,Hk,TOP];
     scale defaults to D^-1/2.  Positions [t - local_window + 1, t] and the picked blocks'
     positions before them, each once.  Returns (out [B,Hq,D] in query's dtype,
-    log-sum-exp fp32 [B,Hq]).  ``ring``: position p lives in row p mod T.
+    log-sum-exp fp32 [B,Hq]).  Sums and exponentials are fp32; 16-bit types round each
+    weight to the type before it meets the values (bf16: 2^-8 at most, relative).
+    ``ring``: position p lives in row p mod T, and the rows hold (t - T, t]: a chunk whose
+    later tokens are in the ring already has lost the earlier ones' farthest positions.
     D a multiple of 8 up to 256, TOP <= 64.
     """
     return torch.ops.rlm.routed_attention(query, key_cache, value_cache, blocks, position,
@@ -70,6 +73,7 @@ def routed_attention_seq(query: Tensor, key_cache: Tensor, value_cache: Tensor, 
                          positions: Tensor, block_size: int, local_window: int,
                          scale: float | None = None) -> tuple[Tensor, Tensor]:
     """Sequence form: query [B,Tq,Hq,D], blocks [B,Tq,TOP] or [B,Tq,Hk,TOP], positions [Tq]
-    or [B,Tq]; returns (out [B,Tq,Hq,D], log-sum-exp fp32 [B,Tq,Hq])."""
+    or [B,Tq]; returns (out [B,Tq,Hq,D], log-sum-exp fp32 [B,Tq,Hq]).  Linear caches
+    only; weights are rounded as there."""
     return torch.ops.rlm.routed_attention_seq(query, key_cache, value_cache, blocks, positions,
                                               block_size, local_window, scale)
