@@ -822,7 +822,8 @@ hipError_t rlm_rotary_to_caches(const rlm_tensor* query, const rlm_tensor* key,
  *   picked.
  * Outputs: out_blocks int32 [B,Tq,S,TOP], out_scores f32 [B,Tq,S,TOP]; -1 and
  * -inf where a query has fewer blocks to pick from.  A block whose score is NaN
- * or at most -1e30 is not picked.
+ * or at most -1e30 is not picked; a head of -inf adds nothing to a score, one of
+ * +inf makes it +inf, which is picked first (the selection takes it for no number).
  */
 hipError_t rlm_block_route(const rlm_tensor* router_query, const rlm_tensor* block_mean,
                            const rlm_tensor* block_std, const rlm_tensor* gamma,

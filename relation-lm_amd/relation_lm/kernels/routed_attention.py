@@ -33,7 +33,7 @@ def block_route(router_query: Tensor, block_mean: Tensor, block_std: Tensor, gam
     ``router_cache_update``), gamma [H], bias [H,RB].  Returns (blocks int32 [B,(S,)TOP],
     scores fp32), best first, ties to the lowest block, -1 and -inf where fewer blocks are
     complete (``strict_valid``: wholly before the local window).  A block whose score is
-    NaN or at most -1e30 is not picked.  ``ring``: the statistics are a ring buffer's;
+    NaN or at most -1e30 is not picked; a head of -inf adds nothing to a score.  ``ring``: the statistics are a ring buffer's;
     blocks stay absolute.
     """
     return torch.ops.rlm.block_route(router_query, block_mean, block_std, gamma, bias, position,
