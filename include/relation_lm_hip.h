@@ -36,6 +36,7 @@ enum rlm_dtype {
   RLM_F16 = 2,
   RLM_I32 = 3,
   RLM_I64 = 4,
+  RLM_F8E4M3 = 5,                /* e4m3: 1 sign, 4 exponent, 3 mantissa bits, no infinity */
 };
 
 #define RLM_MAX_DIMS 4
@@ -811,6 +812,31 @@ hipError_t rlm_rotary_to_caches(const rlm_tensor* query, const rlm_tensor* key,
                                 const rlm_tensor* out_query, hipStream_t stream);
 
 /*
+ * rlm_rotary_to_caches into caches of 8 bits: key_cache / value_cache [B,T,Hk,D] of
+ * RLM_F8E4M3 with key_scale / value_scale f32 [B,T,Hk] (all mutated; any non-overlapping
+ * strides).  A row (the features of one token and key head, fp32 after the rotation) is
+ * written as its scale s = max |x| / 448, not below 2^-126, and the codes e4m3(x / s); a
+ * row of zeros has scale 0; one with an infinity or NaN has scale NaN and codes 0, so that
+ * it reads back as NaN.  D <= 256.
+ */
+hipError_t rlm_rotary_to_quantized_caches(
+    const rlm_tensor* query, const rlm_tensor* key, const rlm_tensor* value,
+    const rlm_tensor* position, const rlm_tensor* frequencies, const rlm_tensor* key_cache,
+    const rlm_tensor* value_cache, const rlm_tensor* key_scale, const rlm_tensor* value_scale,
+    const rlm_tensor* lengths, int32_t interleaved, double scale, int32_t ring,
+    const rlm_tensor* out_query, hipStream_t stream);
+
+/*
+ * Rows of an 8-bit cache in a float type: out [B,N,Hk,D] = cache * scale, rounded once.
+ * cache [B,T,Hk,D] RLM_F8E4M3 and scale [B,T,Hk] f32 of any strides; rows [B,N] int32/int64
+ * names cache rows in any order (those outside [0, T) give zeros), or NULL for all of them
+ * (N == T).
+ */
+hipError_t rlm_quantized_rows(const rlm_tensor* cache, const rlm_tensor* scale,
+                              const rlm_tensor* rows, const rlm_tensor* out,
+                              hipStream_t stream);
+
+/*
  * The block router by itself: for each query the top_blocks best complete
  * blocks (strict: complete blocks wholly before the local window), with the
  * scores and the tie rule of rlm_relation_select_packed: float64 log-sum-exps,
@@ -856,6 +882,48 @@ hipError_t rlm_routed_attention(const rlm_tensor* query, const rlm_tensor* key_c
                                 int64_t local_window, double scale, int32_t ring,
                                 const rlm_tensor* out, const rlm_tensor* out_lse,
                                 hipStream_t stream);
+
+/*
+ * rlm_routed_attention over caches of 8 bits: key_cache / value_cache [B,T,Hk,D] of
+ * RLM_F8E4M3 (any 16-byte aligned strides that are multiples of 16), key_scale /
+ * value_scale f32 [B,T,Hk] of any strides; D a multiple of 16 up to 256:
+ *   out = softmax(scale * key_scale q . k) (value_scale v).
+ * Queries and weights enter the matrix products as sums of bf16 parts (codes are exact in
+ * bf16): 16-bit queries exactly, their weights to within 2^-18, fp32 to its precision.  Scores, exponentials and sums are
+ * fp32.  A scale that is not finite gives NaN where its row is seen.
+ */
+hipError_t rlm_routed_attention_quantized(
+    const rlm_tensor* query, const rlm_tensor* key_cache, const rlm_tensor* value_cache,
+    const rlm_tensor* key_scale, const rlm_tensor* value_scale, const rlm_tensor* blocks,
+    const rlm_tensor* positions, int64_t block_size, int64_t local_window, double scale,
+    int32_t ring, const rlm_tensor* out, const rlm_tensor* out_lse, hipStream_t stream);
+
+/*
+ * Products with weights of 4 bits: out [M,N] = input [M,K] W^T + bias with
+ *   W[n][k] = (c[n][k] - zeros[k / group_size][n]) * scales[k / group_size][n],
+ * codes c in 0..15 packed as int32 [ceil(N/16), ceil(K/128), 64, 4] (contiguous): word s of
+ * lane 16 q + r of tile (i, j) holds the codes of row 16 i + r and inputs
+ * 128 j + 32 s + 8 q + e, e = 0..7, at bit 4 (e / 2) + 16 (e mod 2); codes past N or K may
+ * hold anything.  scales and zeros [ceil(K/group_size), N] share a float dtype; zeros NULL
+ * means 8; bias [N] of any float dtype or NULL.  group_size 32, 64 or a multiple of 128.
+ * input row-strided, of any float dtype, as out (dense).  Products are summed in fp32:
+ * codes are exact in 16 bits, fp32 inputs enter as three bf16 parts.
+ */
+hipError_t rlm_linear_4bit(const rlm_tensor* input, const rlm_tensor* codes,
+                           const rlm_tensor* scales, const rlm_tensor* zeros,
+                           int64_t group_size, const rlm_tensor* bias, const rlm_tensor* out,
+                           hipStream_t stream);
+
+/*
+ * Two such products of one input and the activation of one times the other:
+ *   out = act(input Wg^T) * (input Wu^T), activation 0: x / (1 + exp(-x)), 1: exact (erf) GELU.
+ * Both weights have one shape, group size and dtype of scales; zeros for both or neither.
+ */
+hipError_t rlm_gated_linear_4bit(const rlm_tensor* input, const rlm_tensor* gate_codes,
+                                 const rlm_tensor* gate_scales, const rlm_tensor* gate_zeros,
+                                 const rlm_tensor* up_codes, const rlm_tensor* up_scales,
+                                 const rlm_tensor* up_zeros, int64_t group_size,
+                                 int32_t activation, const rlm_tensor* out, hipStream_t stream);
 
 /*
  * What stands between two blocks of a stack, in one pass:

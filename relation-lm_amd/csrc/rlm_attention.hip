@@ -4,24 +4,30 @@
 //   [t - L + 1, t]  and, before them,  [j BS, j BS + BS) of every pick
 // that the cache holds (linear: p < T; ring: p > t - T, position p in row p mod T):
 //   out = sum_p softmax_p(scale q . k_p) v_p,   lse = log sum_p exp(scale q . k_p).
+// Caches of 8 bits hold codes and a scale for each row of a key head: k_p = key_scale_p code_p.
 // A position counts once whichever way it is named; a query that sees none gives 0 and -inf.
 #include "rlm_attention.hpp"
 
-using namespace rlm;
-using namespace rlm::attention;
+namespace rlm {
+namespace {
 
-extern "C" hipError_t rlm_routed_attention(
-    const rlm_tensor* query, const rlm_tensor* key_cache, const rlm_tensor* value_cache,
-    const rlm_tensor* blocks, const rlm_tensor* positions, int64_t block_size,
-    int64_t local_window, double scale, int32_t ring, const rlm_tensor* out,
-    const rlm_tensor* out_lse, hipStream_t stream) {
-  clear_error();
+using namespace attention;
+
+// Checks a call's descriptors and fills its parameters; key_scale and value_scale come with caches
+// of 8 bits.
+hipError_t fill(const rlm_tensor* query, const rlm_tensor* key_cache, const rlm_tensor* value_cache,
+                const rlm_tensor* key_scale, const rlm_tensor* value_scale, bool quantized,
+                const rlm_tensor* blocks, const rlm_tensor* positions, int64_t block_size,
+                int64_t local_window, double scale, int32_t ring, const rlm_tensor* out,
+                const rlm_tensor* out_lse, Params& p) {
   RLM_TRY(check_strided(query, "query", 4));
   RLM_TRY(check_dtype_float(query, "query"));
   const int64_t B = query->shape[0], Tq = query->shape[1], Hq = query->shape[2],
                 D = query->shape[3];
-  RLM_REQUIRE(D >= 8 && D % 8 == 0 && D <= 256,
-              "query: head dim must be a multiple of 8 in [8, 256], got %lld", (long long)D);
+  const int unit = quantized ? 16 : 8;  // features of a 16-byte access
+  RLM_REQUIRE(D >= unit && D % unit == 0 && D <= 256,
+              "query: head dim must be a multiple of %d in [%d, 256], got %lld", unit, unit,
+              (long long)D);
   RLM_TRY(check_strided(key_cache, "key_cache", 4));
   RLM_TRY(check_strided(value_cache, "value_cache", 4));
   const int64_t T = key_cache->shape[1], Hk = key_cache->shape[2];
@@ -30,7 +36,10 @@ extern "C" hipError_t rlm_routed_attention(
               (long long)Hk);
   for (const rlm_tensor* c : {key_cache, value_cache}) {
     const char* name = c == key_cache ? "key_cache" : "value_cache";
-    RLM_TRY(check_same_dtype(c, name, query, "query"));
+    if (quantized)
+      RLM_TRY(check_dtype_is(c, name, RLM_F8E4M3));
+    else
+      RLM_TRY(check_same_dtype(c, name, query, "query"));
     RLM_TRY(check_dim(c, name, 0, B));
     RLM_TRY(check_dim(c, name, 1, T));
     RLM_TRY(check_dim(c, name, 2, Hk));
@@ -55,7 +64,6 @@ extern "C" hipError_t rlm_routed_attention(
   if (blocks->ndim == 4) RLM_TRY(check_dim(blocks, "blocks", 2, Hk));
   const int64_t TOP = blocks->shape[blocks->ndim - 1];
   RLM_REQUIRE(TOP <= kMaxTop, "blocks: at most %d picks, got %lld", kMaxTop, (long long)TOP);
-  Params p{};
   RLM_TRY(check_positions(positions, "positions", B, Tq, &p.pos_sb, &p.pos_sq));
   RLM_TRY(check_dense(out, "out", 4));
   RLM_TRY(check_same_dtype(out, "out", query, "query"));
@@ -64,12 +72,22 @@ extern "C" hipError_t rlm_routed_attention(
   RLM_TRY(check_dtype_is(out_lse, "out_lse", RLM_F32));
   for (int i = 0; i < 3; ++i) RLM_TRY(check_dim(out_lse, "out_lse", i, query->shape[i]));
   for (const rlm_tensor* t : {query, key_cache, value_cache, out}) {
+    const int64_t step = t->dtype == RLM_F8E4M3 ? 16 : 8;
     bool aligned = (reinterpret_cast<uintptr_t>(t->data) & 15u) == 0;
     for (int i = 0; i < 3; ++i)
-      aligned = aligned && (t->shape[i] <= 1 || t->stride[i] % 8 == 0);
+      aligned = aligned && (t->shape[i] <= 1 || t->stride[i] % step == 0);
     RLM_REQUIRE(aligned,
                 "query, key_cache, value_cache and out must be 16-byte aligned with strides that "
-                "are multiples of 8 elements");
+                "are multiples of 8 elements (8-bit caches: 16)");
+  }
+  if (quantized) {
+    RLM_TRY(check_scales(key_scale, "key_scale", B, T, Hk));
+    RLM_TRY(check_scales(value_scale, "value_scale", B, T, Hk));
+    p.ks = static_cast<const float*>(key_scale->data);
+    p.ks_sb = key_scale->stride[0], p.ks_st = key_scale->stride[1], p.ks_sh = key_scale->stride[2];
+    p.vs = static_cast<const float*>(value_scale->data);
+    p.vs_sb = value_scale->stride[0], p.vs_st = value_scale->stride[1],
+    p.vs_sh = value_scale->stride[2];
   }
   p.q = query->data;
   p.q_sb = query->stride[0], p.q_st = query->stride[1], p.q_sh = query->stride[2];
@@ -106,7 +124,39 @@ extern "C" hipError_t rlm_routed_attention(
   p.by_kv = FastDiv(static_cast<uint32_t>(Hk));
   p.by_queries = FastDiv(static_cast<uint32_t>(Tq));
   p.by_block = FastDiv(static_cast<uint32_t>(block_size));
+  return hipSuccess;
+}
+
+}  // namespace
+}  // namespace rlm
+
+using namespace rlm;
+
+extern "C" hipError_t rlm_routed_attention(
+    const rlm_tensor* query, const rlm_tensor* key_cache, const rlm_tensor* value_cache,
+    const rlm_tensor* blocks, const rlm_tensor* positions, int64_t block_size,
+    int64_t local_window, double scale, int32_t ring, const rlm_tensor* out,
+    const rlm_tensor* out_lse, hipStream_t stream) {
+  clear_error();
+  Params p{};
+  const hipError_t e = fill(query, key_cache, value_cache, nullptr, nullptr, false, blocks,
+                            positions, block_size, local_window, scale, ring, out, out_lse, p);
+  if (e != hipSuccess || p.items == 0) return e;
   return tile_fits(p, query->dtype) && tile_faster(p, query->dtype)
              ? tile_launch(p, query->dtype, stream)
              : query_launch(p, query->dtype, stream);
+}
+
+extern "C" hipError_t rlm_routed_attention_quantized(
+    const rlm_tensor* query, const rlm_tensor* key_cache, const rlm_tensor* value_cache,
+    const rlm_tensor* key_scale, const rlm_tensor* value_scale, const rlm_tensor* blocks,
+    const rlm_tensor* positions, int64_t block_size, int64_t local_window, double scale,
+    int32_t ring, const rlm_tensor* out, const rlm_tensor* out_lse, hipStream_t stream) {
+  clear_error();
+  Params p{};
+  const hipError_t e =
+      fill(query, key_cache, value_cache, key_scale, value_scale, true, blocks, positions,
+           block_size, local_window, scale, ring, out, out_lse, p);
+  if (e != hipSuccess || p.items == 0) return e;
+  return quantized_launch(p, query->dtype, stream);
 }

@@ -17,6 +17,8 @@ constexpr float kLn2 = 0.69314718055994530942f;
 struct Params {
   const void *q, *k, *v;   // [B,Tq,Hq,D], [B,T,Hk,D] twice; unit stride in D
   int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  const float *ks, *vs;    // 8-bit caches: their rows' scales [B,T,Hk]
+  int64_t ks_sb, ks_st, ks_sh, vs_sb, vs_st, vs_sh;
   const int32_t* blocks;   // [B,Tq,(Hk),TOP]
   int64_t blk_sb, blk_st, blk_sh;
   const void* pos;
@@ -51,6 +53,8 @@ __device__ __forceinline__ float rows_sum(float v) { return swap32_sum(swap16_su
 
 // One query to a workgroup (rlm_attention_query.hip).
 hipError_t query_launch(const Params& p, int dtype, hipStream_t stream);
+// The same over caches of 8 bits (rlm_attention_quantized.hip).
+hipError_t quantized_launch(const Params& p, int dtype, hipStream_t stream);
 // Key tiles shared by the rows of a workgroup (rlm_attention_tile.hip).
 bool tile_fits(const Params& p, int dtype);
 bool tile_faster(const Params& p, int dtype);

@@ -1,4 +1,5 @@
 // Matrix-core operands of the attention kernels: products, packing, and the LDS layout of tiles.
+// (The products and the sums of bf16 parts also serve rlm_linear_4bit.hip.)
 #pragma once
 
 #include <type_traits>
@@ -47,6 +48,24 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, f16) {
   typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
   const f32x2_t v = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+}
+
+// x as a sum of N bf16 numbers each.
+template <int N>
+__device__ __forceinline__ void split(float (&x)[8], s16x8 (&part)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+      if (n + 1 < N) {
+        x[2 * i] -= bf16_lo(w[i]);
+        x[2 * i + 1] -= bf16_hi(w[i]);
+      }
+    }
+    part[n] = __builtin_bit_cast(s16x8, make_uint4(w[0], w[1], w[2], w[3]));
+  }
 }
 
 // 16-byte pieces of an LDS row: rows of 8 pieces alternate between the halves of the 16 piece

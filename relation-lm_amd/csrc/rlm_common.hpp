@@ -508,7 +508,9 @@ inline bool is_float_dtype(int d) { return d == RLM_F32 || d == RLM_BF16 || d ==
 inline bool is_index_dtype(int d) { return d == RLM_I32 || d == RLM_I64; }
 const char* dtype_name(int d);
 // Bytes per element of an rlm dtype.
-inline int64_t dtype_size(int d) { return (d == RLM_F32 || d == RLM_I32) ? 4 : (d == RLM_I64 ? 8 : 2); }
+inline int64_t dtype_size(int d) {
+  return (d == RLM_F32 || d == RLM_I32) ? 4 : d == RLM_I64 ? 8 : d == RLM_F8E4M3 ? 1 : 2;
+}
 
 // Checks that `t` is a non-null, contiguous tensor of the given rank.
 bool check_tensor(const rlm_tensor* t, const char* name, int ndim);
@@ -528,6 +530,8 @@ bool check_positions(const rlm_tensor* t, const char* name, int64_t B, int64_t T
                      int64_t* stride_b, int64_t* stride_q);
 // Checks that a launch stays within what the device takes: fewer than 2^32 threads.
 bool check_launch(const char* what, int64_t groups, int64_t threads);
+// Checks the fp32 scales [B,T,H] of an 8-bit cache's rows (any strides).
+bool check_scales(const rlm_tensor* t, const char* name, int64_t B, int64_t T, int64_t H);
 // Checks t->shape[dim] == value.
 bool check_dim(const rlm_tensor* t, const char* name, int dim, int64_t value);
 bool check_dtype_float(const rlm_tensor* t, const char* name);

@@ -23,6 +23,7 @@ const char* dtype_name(int d) {
     case RLM_F16: return "float16";
     case RLM_I32: return "int32";
     case RLM_I64: return "int64";
+    case RLM_F8E4M3: return "float8_e4m3fn";
     default: return "unknown";
   }
 }
@@ -177,6 +178,23 @@ bool check_launch(const char* what, int64_t groups, int64_t threads) {
             "threads in all)",
             what, (long long)groups, (long long)threads);
   return false;
+}
+
+bool check_scales(const rlm_tensor* t, const char* name, int64_t B, int64_t T, int64_t H) {
+  if (t == nullptr) {
+    set_error("%s: missing tensor", name);
+    return false;
+  }
+  if (t->ndim != 3) {
+    set_error("%s: expected a 3-d tensor, got %d-d", name, t->ndim);
+    return false;
+  }
+  // Any strides, the last dim's among them: with a dim of one element behind it.
+  rlm_tensor with_last = *t;
+  with_last.ndim = 4;
+  with_last.shape[3] = with_last.stride[3] = 1;
+  return check_strided(&with_last, name, 4) && check_dtype_is(t, name, RLM_F32) &&
+         check_dim(t, name, 0, B) && check_dim(t, name, 1, T) && check_dim(t, name, 2, H);
 }
 
 bool check_dim(const rlm_tensor* t, const char* name, int dim, int64_t value) {

@@ -30,12 +30,15 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxAngles = 2048;  // per workgroup: 16 KiB of LDS
 constexpr int kMaxTokens = 16;    // per workgroup
+constexpr int kMaxQuantized = 256;  // head dim of 8-bit caches
 
 struct RotaryParams {
   const void *q, *k, *v;           // [B,Tq,H*,D], unit stride in D
   int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
   void *oq, *ok, *ov;              // ok / ov: [B,Tq,Hk,D], or the caches [B,T,Hk,D]
   int64_t ok_sb, ok_st, ok_sh, ov_sb, ov_st, ov_sh;
+  float *ks, *vs;                  // 8-bit caches: their scales [B,T,Hk]
+  int64_t ks_sb, ks_st, ks_sh, vs_sb, vs_st, vs_sh;
   const void* pos;
   int pos_dtype;
   int64_t pos_sb, pos_st;
@@ -49,7 +52,7 @@ struct RotaryParams {
   int heads;                       // Hq + Hk (+ Hk value heads)
   int per_group;                   // tokens of a workgroup
   bool to_cache, ring;
-  FastDiv by_queries, by_pairs, by_units, by_token_units;
+  FastDiv by_queries, by_pairs, by_units, by_token_units, by_heads;
 };
 
 template <int BYTES>
@@ -61,19 +64,10 @@ struct Raw<4> { using type = uint32_t; };
 template <>
 struct Raw<2> { using type = uint16_t; };
 
-// V: elements of one access (16 bytes, or one element for unaligned shapes).
-template <typename T, int V, bool INTERLEAVED>
-__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
-  using raw_t = typename Raw<V * sizeof(T)>::type;
-  struct Vec {
-    T e[V];
-  };
-  __shared__ float2 turn[kMaxAngles];
-  __shared__ int64_t dest[kMaxTokens];  // row of ok / ov, negative: not written
-  const uint32_t first = blockIdx.x * static_cast<uint32_t>(p.per_group);
-  const uint32_t count = min(static_cast<uint32_t>(p.per_group), p.tokens - first);
+// The turns of a workgroup's `count` tokens and their rows of ok / ov (negative: not written).
+__device__ __forceinline__ void set_up(const RotaryParams& p, uint32_t first, uint32_t count,
+                                       float2* turn, int64_t* dest) {
   const uint32_t F = p.F;
-
   for (uint32_t i = threadIdx.x; i < count * F; i += kThreads) {
     uint32_t f, step;
     const uint32_t local = p.by_pairs.div(i, f);
@@ -105,6 +99,21 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
     dest[threadIdx.x] = row;
   }
   __syncthreads();
+}
+
+// V: elements of one access (16 bytes, or one element for unaligned shapes).
+template <typename T, int V, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
+  using raw_t = typename Raw<V * sizeof(T)>::type;
+  struct Vec {
+    T e[V];
+  };
+  __shared__ float2 turn[kMaxAngles];
+  __shared__ int64_t dest[kMaxTokens];
+  const uint32_t first = blockIdx.x * static_cast<uint32_t>(p.per_group);
+  const uint32_t count = min(static_cast<uint32_t>(p.per_group), p.tokens - first);
+  const uint32_t F = p.F;
+  set_up(p, first, count, turn, dest);
 
   const int D = p.D;
   // Units of a head: one pair of accesses (INTERLEAVED: one access), or one that is copied.
@@ -204,6 +213,175 @@ hipError_t launch_rotary_type(RotaryParams& p, bool aligned, bool interleaved,
                  : launch_rotary<T, 1>(p, interleaved, stream);
 }
 
+// Eight elements from `src`, of which `count` are read (WIDE: whole 16-byte accesses).
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T* src, int count, float (&x)[8]) {
+  if constexpr (WIDE) {
+    struct Raws {
+      uint4 part[sizeof(T) / 2];
+    };
+    struct Vec {
+      T e[8];
+    };
+    Raws raw;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      raw.part[i] = reinterpret_cast<const uint4*>(src)[i];
+    const Vec v = __builtin_bit_cast(Vec, raw);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = to_f32(v.e[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < count ? to_f32(src[e]) : 0.0f;
+  }
+}
+
+// Rotation with the key and value rows written as e4m3 codes and a scale each.  L lanes have a
+// row, eight features each, so that its largest magnitude is a few lane exchanges; a pair's
+// other half is read a second time (from L1) by the lane that has it not.
+template <typename T, int L, bool WIDE, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void rotary_quantize_kernel(RotaryParams p) {
+  __shared__ float2 turn[kMaxAngles];
+  __shared__ int64_t dest[kMaxTokens];
+  const uint32_t first = blockIdx.x * static_cast<uint32_t>(p.per_group);
+  const uint32_t count = min(static_cast<uint32_t>(p.per_group), p.tokens - first);
+  set_up(p, first, count, turn, dest);
+
+  const int D = p.D, F = p.F;
+  const int at = 8 * (threadIdx.x % L);
+  const int mine = min(8, D - at);  // features of this lane, none where negative
+  const uint32_t total = count * p.by_heads.d;
+  for (uint32_t i = threadIdx.x / L; i < total; i += kThreads / L) {
+    uint32_t head, step;
+    const uint32_t local = p.by_heads.div(i, head);
+    const uint32_t b = p.by_queries.div(first + local, step);
+    const int64_t row = dest[local];
+    const bool is_q = head < static_cast<uint32_t>(p.Hq);
+    const bool is_v = head >= static_cast<uint32_t>(p.Hq + p.Hk);
+    if (!is_q && row < 0) continue;  // all of a row's lanes
+    const int64_t h = is_q ? head : is_v ? head - p.Hq - p.Hk : head - p.Hq;
+    const T* src = is_q ? static_cast<const T*>(p.q) + b * p.q_sb + step * p.q_st + h * p.q_sh
+                   : is_v ? static_cast<const T*>(p.v) + b * p.v_sb + step * p.v_st + h * p.v_sh
+                          : static_cast<const T*>(p.k) + b * p.k_sb + step * p.k_st + h * p.k_sh;
+    const float2* tr = turn + local * F;
+    float x[8] = {};
+    if (mine > 0) {
+      load8<T, WIDE>(src + at, mine, x);
+      if (!is_v && at < 2 * F) {
+        if constexpr (INTERLEAVED) {
+          // Pairs do not straddle lanes.
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            if (WIDE || at + e < 2 * F) {
+              const float2 cs = tr[(at + e) >> 1];
+              const float a = x[e], bb = x[e + 1];
+              x[e] = fmaf(a, cs.x, -(bb * cs.y));
+              x[e + 1] = fmaf(a, cs.y, bb * cs.x);
+            }
+          }
+        } else if constexpr (WIDE) {
+          // F is a multiple of 8: a lane's features are all of one half.
+          const bool low = at < F;
+          float y[8];
+          load8<T, true>(src + (low ? at + F : at - F), 8, y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 cs = tr[(low ? at : at - F) + e];
+            x[e] = low ? fmaf(x[e], cs.x, -(y[e] * cs.y)) : fmaf(y[e], cs.y, x[e] * cs.x);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int d = at + e;
+            if (d < 2 * F) {  // 2 F <= D
+              const bool low = d < F;
+              const float2 cs = tr[low ? d : d - F];
+              const float y = to_f32(src[low ? d + F : d - F]);
+              x[e] = low ? fmaf(x[e], cs.x, -(y * cs.y)) : fmaf(y, cs.y, x[e] * cs.x);
+            }
+          }
+        }
+      }
+    }
+    if (is_q) {
+      T* dst = static_cast<T*>(p.oq) + (static_cast<int64_t>(first + local) * p.Hq + h) * D + at;
+      if constexpr (WIDE) {
+        if (mine > 0) {
+          put4<T>(dst, x[0], x[1], x[2], x[3]);
+          put4<T>(dst + 4, x[4], x[5], x[6], x[7]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < mine) dst[e] = from_f32<T>(x[e]);
+      }
+      continue;
+    }
+    // The largest magnitude as bits: NaN above infinity above every number.
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int off = 1; off < L; off <<= 1)
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), off, kWave)));
+    const bool finite = most < 0x7f800000u;
+    // Not below the smallest normal number, whose reciprocal is finite.
+    const float least = fmaxf(__uint_as_float(most) / 448.0f, 1.17549435e-38f);
+    const float inv = finite ? 1.0f / least : 0.0f;
+    const float scale = !finite ? __uint_as_float(0x7fc00000u) : most == 0 ? 0.0f : least;
+    uint32_t codes[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // x / s as the correctly rounded reciprocal and one correction give it: values that are
+        // few-bit fractions of the largest fall on or beside the codes' ties.
+        const float q = x[4 * w + e] * inv;
+        y[e] = finite ? fmaf(fmaf(-q, least, x[4 * w + e]), inv, q) : 0.0f;
+      }
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      codes[w] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true));
+    }
+    uint8_t* dst = is_v ? static_cast<uint8_t*>(p.ov) + b * p.ov_sb + row * p.ov_st + h * p.ov_sh
+                        : static_cast<uint8_t*>(p.ok) + b * p.ok_sb + row * p.ok_st + h * p.ok_sh;
+    if constexpr (WIDE) {
+      if (mine > 0) *reinterpret_cast<uint2*>(dst + at) = make_uint2(codes[0], codes[1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < mine) dst[at + e] = static_cast<uint8_t>(codes[e / 4] >> (8 * (e % 4)));
+    }
+    if (at == 0) {
+      float* to = is_v ? p.vs + b * p.vs_sb + row * p.vs_st + h * p.vs_sh
+                       : p.ks + b * p.ks_sb + row * p.ks_st + h * p.ks_sh;
+      *to = scale;
+    }
+  }
+}
+
+template <typename T, int L, bool WIDE>
+hipError_t launch_quantize(const RotaryParams& p, bool interleaved, hipStream_t stream) {
+  const dim3 grid((p.tokens + p.per_group - 1) / p.per_group);
+  RLM_TRY(check_launch("rotary_to_quantized_caches", grid.x, kThreads));
+  if (interleaved)
+    hipLaunchKernelGGL((rotary_quantize_kernel<T, L, WIDE, true>), grid, dim3(kThreads), 0, stream,
+                       p);
+  else
+    hipLaunchKernelGGL((rotary_quantize_kernel<T, L, WIDE, false>), grid, dim3(kThreads), 0, stream,
+                       p);
+  return launch_status("rotary_to_quantized_caches");
+}
+
+template <typename T, bool WIDE>
+hipError_t launch_quantize_lanes(const RotaryParams& p, int lanes, bool interleaved,
+                                 hipStream_t stream) {
+  if (lanes <= 4) return launch_quantize<T, 4, WIDE>(p, interleaved, stream);
+  if (lanes <= 8) return launch_quantize<T, 8, WIDE>(p, interleaved, stream);
+  if (lanes <= 16) return launch_quantize<T, 16, WIDE>(p, interleaved, stream);
+  return launch_quantize<T, 32, WIDE>(p, interleaved, stream);
+}
+
 // A 4-d tensor of unit stride in its last dim (the others as they come, 0 included: they
 // are read only).
 bool check_view(const rlm_tensor* t, const char* name, int64_t heads, int64_t B, int64_t Tq,
@@ -212,8 +390,8 @@ bool check_view(const rlm_tensor* t, const char* name, int64_t heads, int64_t B,
          (heads < 0 || check_dim(t, name, 2, heads)) && check_dim(t, name, 3, D);
 }
 
-bool wide_access(const rlm_tensor* t, int64_t per_vec) {
-  if ((reinterpret_cast<uintptr_t>(t->data) & 15u) != 0) return false;
+bool wide_access(const rlm_tensor* t, int64_t per_vec, uintptr_t bytes = 16) {
+  if ((reinterpret_cast<uintptr_t>(t->data) & (bytes - 1)) != 0) return false;
   for (int i = 0; i + 1 < t->ndim; ++i)
     if (t->shape[i] > 1 && t->stride[i] % per_vec != 0) return false;
   return true;
@@ -222,14 +400,17 @@ bool wide_access(const rlm_tensor* t, int64_t per_vec) {
 hipError_t rotary_common(const rlm_tensor* query, const rlm_tensor* key, const rlm_tensor* value,
                          const rlm_tensor* position, const rlm_tensor* frequencies,
                          const rlm_tensor* out_key, const rlm_tensor* out_value,
-                         const rlm_tensor* lengths, int32_t interleaved, double scale,
-                         int32_t ring, const rlm_tensor* out_query, hipStream_t stream) {
+                         const rlm_tensor* key_scale, const rlm_tensor* value_scale,
+                         bool quantized, const rlm_tensor* lengths, int32_t interleaved,
+                         double scale, int32_t ring, const rlm_tensor* out_query,
+                         hipStream_t stream) {
   const bool to_cache = value != nullptr;
   RLM_TRY(check_strided(query, "query", 4));
   RLM_TRY(check_dtype_float(query, "query"));
   const int64_t B = query->shape[0], Tq = query->shape[1], Hq = query->shape[2],
                 D = query->shape[3];
-  RLM_REQUIRE(D >= 1 && D <= 1024, "query: head dim must be in [1, 1024], got %lld",
+  const int most = quantized ? kMaxQuantized : 1024;
+  RLM_REQUIRE(D >= 1 && D <= most, "query: head dim must be in [1, %d], got %lld", most,
               (long long)D);
   RLM_TRY(check_view(key, "key", -1, B, Tq, D));
   RLM_TRY(check_same_dtype(key, "key", query, "query"));
@@ -257,13 +438,28 @@ hipError_t rotary_common(const rlm_tensor* query, const rlm_tensor* key, const r
       const char* name = c == out_key ? "key_cache" : "value_cache";
       RLM_TRY(check_strided(c, name, 4));
       RLM_TRY(check_no_overlap(c, name));
-      RLM_TRY(check_same_dtype(c, name, query, "query"));
+      if (quantized)
+        RLM_TRY(check_dtype_is(c, name, RLM_F8E4M3));
+      else
+        RLM_TRY(check_same_dtype(c, name, query, "query"));
       RLM_TRY(check_dim(c, name, 0, B));
       RLM_TRY(check_dim(c, name, 2, Hk));
       RLM_TRY(check_dim(c, name, 3, D));
     }
     p.rows = out_key->shape[1];
     RLM_TRY(check_dim(out_value, "value_cache", 1, p.rows));
+    if (quantized) {
+      for (const rlm_tensor* s : {key_scale, value_scale}) {
+        const char* name = s == key_scale ? "key_scale" : "value_scale";
+        RLM_TRY(check_scales(s, name, B, p.rows, Hk));
+        RLM_TRY(check_no_overlap(s, name));
+      }
+      p.ks = static_cast<float*>(key_scale->data);
+      p.ks_sb = key_scale->stride[0], p.ks_st = key_scale->stride[1], p.ks_sh = key_scale->stride[2];
+      p.vs = static_cast<float*>(value_scale->data);
+      p.vs_sb = value_scale->stride[0], p.vs_st = value_scale->stride[1],
+      p.vs_sh = value_scale->stride[2];
+    }
     RLM_REQUIRE(!ring || (p.rows >= 1 && (p.rows & (p.rows - 1)) == 0),
                 "ring-buffer caches need a power-of-two cache length, got %lld",
                 (long long)p.rows);
@@ -324,7 +520,10 @@ hipError_t rotary_common(const rlm_tensor* query, const rlm_tensor* key, const r
   //   16384 tokens of 12 + 4 heads of 64    17.4 / 12.4 / 12.7 / 12.6
   //    4096 tokens of the same               5.9 /  4.4 /  5.8 /  4.7
   //       8 tokens of 32 + 8 heads of 128    3.0 /  4.6 /  7.3 /  3.0
-  const int64_t work = static_cast<int64_t>(p.heads) * ((D + per_vec - 1) / per_vec);
+  const int lanes = static_cast<int>(D + 7) / 8;
+  const int64_t work = static_cast<int64_t>(p.heads) *
+                       (quantized ? lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32
+                                  : (D + per_vec - 1) / per_vec);
   int64_t group = (8 * kThreads) / work;
   group = std::min<int64_t>(group, p.tokens / 512);
   group = std::min<int64_t>(group, std::min<int64_t>(kMaxTokens, kMaxAngles / F));
@@ -333,6 +532,23 @@ hipError_t rotary_common(const rlm_tensor* query, const rlm_tensor* key, const r
   aligned = aligned && wide_access(query, per_vec) && wide_access(key, per_vec) &&
             wide_access(out_query, per_vec) && wide_access(out_key, per_vec) &&
             (!to_cache || (wide_access(value, per_vec) && wide_access(out_value, per_vec)));
+  if (quantized) {
+    p.by_heads = FastDiv(static_cast<uint32_t>(p.heads));
+    // Eight features to a lane: whole accesses of them, and of their codes.
+    const bool wide = D % 8 == 0 && (interleaved ? (2 * F) % 8 == 0 : F % 8 == 0) &&
+                      wide_access(query, per_vec) && wide_access(key, per_vec) &&
+                      wide_access(value, per_vec) && wide_access(out_query, per_vec) &&
+                      wide_access(out_key, 8, 8) && wide_access(out_value, 8, 8);
+#define RLM_QUANTIZE(T)                                                          \
+  return wide ? launch_quantize_lanes<T, true>(p, lanes, interleaved != 0, stream) \
+              : launch_quantize_lanes<T, false>(p, lanes, interleaved != 0, stream);
+    switch (query->dtype) {
+      case RLM_F32: RLM_QUANTIZE(float)
+      case RLM_BF16: RLM_QUANTIZE(bf16)
+      default: RLM_QUANTIZE(f16)
+    }
+#undef RLM_QUANTIZE
+  }
   switch (query->dtype) {
     case RLM_F32: return launch_rotary_type<float>(p, aligned, interleaved != 0, stream);
     case RLM_BF16: return launch_rotary_type<bf16>(p, aligned, interleaved != 0, stream);
@@ -352,7 +568,7 @@ extern "C" hipError_t rlm_rotary_positions(const rlm_tensor* query, const rlm_te
                                            const rlm_tensor* out_key, hipStream_t stream) {
   clear_error();
   return rotary_common(query, key, nullptr, positions, frequencies, out_key, nullptr, nullptr,
-                       interleaved, scale, 0, out_query, stream);
+                       nullptr, false, nullptr, interleaved, scale, 0, out_query, stream);
 }
 
 extern "C" hipError_t rlm_rotary_to_caches(
@@ -362,6 +578,18 @@ extern "C" hipError_t rlm_rotary_to_caches(
     int32_t ring, const rlm_tensor* out_query, hipStream_t stream) {
   clear_error();
   RLM_REQUIRE(value != nullptr, "value: missing tensor");
-  return rotary_common(query, key, value, position, frequencies, key_cache, value_cache, lengths,
-                       interleaved, scale, ring, out_query, stream);
+  return rotary_common(query, key, value, position, frequencies, key_cache, value_cache, nullptr,
+                       nullptr, false, lengths, interleaved, scale, ring, out_query, stream);
+}
+
+extern "C" hipError_t rlm_rotary_to_quantized_caches(
+    const rlm_tensor* query, const rlm_tensor* key, const rlm_tensor* value,
+    const rlm_tensor* position, const rlm_tensor* frequencies, const rlm_tensor* key_cache,
+    const rlm_tensor* value_cache, const rlm_tensor* key_scale, const rlm_tensor* value_scale,
+    const rlm_tensor* lengths, int32_t interleaved, double scale, int32_t ring,
+    const rlm_tensor* out_query, hipStream_t stream) {
+  clear_error();
+  RLM_REQUIRE(value != nullptr, "value: missing tensor");
+  return rotary_common(query, key, value, position, frequencies, key_cache, value_cache, key_scale,
+                       value_scale, true, lengths, interleaved, scale, ring, out_query, stream);
 }

@@ -39,6 +39,22 @@ rlm_tensor desc(const at::Tensor& t, const char* name) {
   return d;
 }
 
+// The descriptor of an 8-bit cache (e4m3 codes), which only some operators take.
+rlm_tensor codes_desc(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.defined() && t.scalar_type() == at::kFloat8_e4m3fn, name,
+              ": expected a float8_e4m3fn tensor, got ", t.scalar_type());
+  TORCH_CHECK(t.dim() <= RLM_MAX_DIMS, name, ": at most ", RLM_MAX_DIMS, " dims supported");
+  rlm_tensor d{};
+  d.data = t.data_ptr();
+  d.dtype = RLM_F8E4M3;
+  d.ndim = static_cast<int32_t>(t.dim());
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    d.shape[i] = t.size(i);
+    d.stride[i] = t.stride(i);
+  }
+  return d;
+}
+
 // All tensors must live on one ROCm device; returns its current stream.
 hipStream_t device_stream(const char* op, std::initializer_list<const at::Tensor*> tensors) {
   const at::Tensor* first = *tensors.begin();

@@ -1,8 +1,8 @@
 """Loads the HIP operator library and registers fake (meta) kernels.
 
 Importing this module makes ``torch.ops.relation_lm.*``,
-``torch.ops.relationlex.*`` and ``torch.ops.rlm.*`` available.  There is no fallback: when the built
-library is missing the import fails with instructions to build it, and calling
+``torch.ops.relationlex.*``, ``torch.ops.rlm.*`` and
+``torch.ops.rlm_quantized.*`` available.  There is no fallback: when the built library is missing the import fails with instructions to build it, and calling
 an op with CPU tensors raises (only the ROCm-device implementation exists) --
 except ``packed_sparse_cache_projection``, whose CPU tensors take ``at::linear``
 as the reference's ``F.linear`` does.
@@ -226,6 +226,24 @@ def _register_fakes() -> None:
 
     torch.library.register_fake("rlm::routed_attention")(fake_attention)
     torch.library.register_fake("rlm::routed_attention_seq")(fake_attention)
+
+    @torch.library.register_fake("rlm_quantized::rotary_to_quantized_caches")
+    def _(query, *rest, **options):
+        return query.new_empty(query.shape)
+
+    @torch.library.register_fake("rlm_quantized::quantized_rows")
+    def _(cache, scale, rows=None, dtype=torch.bfloat16):
+        count = cache.shape[1] if rows is None else rows.shape[1]
+        return cache.new_empty((cache.shape[0], count) + tuple(cache.shape[2:]), dtype=dtype)
+
+    torch.library.register_fake("rlm_quantized::routed_attention_quantized")(fake_attention)
+    torch.library.register_fake("rlm_quantized::routed_attention_quantized_seq")(fake_attention)
+
+    def fake_product(input, codes, scales, *rest, **options):
+        return input.new_empty(tuple(input.shape[:-1]) + (scales.shape[1],))
+
+    torch.library.register_fake("rlm_quantized::linear_4bit")(fake_product)
+    torch.library.register_fake("rlm_quantized::gated_linear_4bit")(fake_product)
 
     @torch.library.register_fake("rlm::gated_residual_norm")
     def _(branch, *rest, **options):

@@ -12,6 +12,9 @@ selection's, [B] (requests of different lengths); sequence forms take a query ax
 one position per query, [Tq] or [B,Tq].  A query at a negative position (a padded row)
 sees nothing: its picks are -1, its output 0, its log-sum-exp -inf.
 
+``routed_attention_quantized`` and its sequence form read the 8-bit caches that
+``rotary_to_quantized_caches`` writes (``kernels/quantized_cache.py``).
+
 Inference only: the operators have no gradient.
 """
 from __future__ import annotations
@@ -19,7 +22,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from relation_lm import _native  # noqa: F401  (registers torch.ops.rlm)
+from relation_lm import _native  # noqa: F401  (registers torch.ops.rlm, .rlm_quantized)
 
 
 def block_route(router_query: Tensor, block_mean: Tensor, block_std: Tensor, gamma: Tensor,
@@ -77,3 +80,33 @@ def routed_attention_seq(query: Tensor, key_cache: Tensor, value_cache: Tensor, 
     only; weights are rounded as there."""
     return torch.ops.rlm.routed_attention_seq(query, key_cache, value_cache, blocks, positions,
                                               block_size, local_window, scale)
+
+
+def routed_attention_quantized(query: Tensor, key_cache: Tensor, value_cache: Tensor,
+                               key_scale: Tensor, value_scale: Tensor, blocks: Tensor,
+                               position: Tensor, block_size: int, local_window: int,
+                               scale: float | None = None, ring: bool = False
+                               ) -> tuple[Tensor, Tensor]:
+    """``routed_attention`` over caches of 8 bits: key_cache / value_cache [B,T,Hk,D] of
+    float8_e4m3fn codes, key_scale / value_scale fp32 [B,T,Hk] (any strides); a row is its
+    codes times its scale.  query of any float type.  D a multiple of 16 up to 256, caches
+    16-byte aligned with strides that are multiples of 16.
+
+    Codes meet the query and the weights as products with sums of bf16 parts: 16-bit queries
+    exactly, weights to within 2^-18 of themselves, fp32 to its precision.  A seen row whose
+    scale is not finite gives NaN.
+    """
+    return torch.ops.rlm_quantized.routed_attention_quantized(
+        query, key_cache, value_cache, key_scale, value_scale, blocks, position, block_size,
+        local_window, scale, ring)
+
+
+def routed_attention_quantized_seq(query: Tensor, key_cache: Tensor, value_cache: Tensor,
+                                   key_scale: Tensor, value_scale: Tensor, blocks: Tensor,
+                                   positions: Tensor, block_size: int, local_window: int,
+                                   scale: float | None = None) -> tuple[Tensor, Tensor]:
+    """Sequence form (a chunk of a prompt over what the caches hold already), as
+    ``routed_attention_seq``; linear caches only."""
+    return torch.ops.rlm_quantized.routed_attention_quantized_seq(
+        query, key_cache, value_cache, key_scale, value_scale, blocks, positions, block_size,
+        local_window, scale)
