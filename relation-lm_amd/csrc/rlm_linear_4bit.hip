@@ -13,139 +13,95 @@
 // instructions (16 rows of weights, 32 inputs each), a wave's load is 1 KiB in a row.  A
 // workgroup has R tiles of 16 weight rows; its waves share out the inputs and add up in LDS, in
 // the waves' order.
-#include "rlm_common.hpp"
-#include "rlm_attention_mfma.hpp"
+#include "rlm_linear_4bit.hpp"
 
 namespace rlm {
 namespace {
 
-using attention::product;
-using attention::s16x8;
+using namespace linear4;
 
-constexpr int kDeep = 128;  // inputs of a tile of codes
+constexpr int kMaxStaged = 64 * 1024;  // bytes of inputs that a workgroup keeps in LDS
+constexpr int kMaxWaves = 8;
 
-enum Activation { kNone = -1, kSilu = 0, kGelu = 1 };
-
-struct LinearParams {
-  const void* x;
-  int64_t x_s;                  // row stride
-  const uint4* codes[2];        // [NT][KT][64]
-  const void* scales[2];        // [G][N]
-  const void* zeros[2];         // or null
-  const void* bias;             // or null
-  int bias_dtype;
-  void* out;                    // [M][N]
-  int M, N, K, KT, NT;
-  int group;
-  FastDiv by_group_tiles;       // group / 128 where that is above 1
-  int activation;
-  bool wide_x, wide_s;          // whole accesses of inputs; of four scales
+// Raw values of four neighbouring scales or zero points (WIDE: one access), and one of them.
+template <typename S, bool WIDE>
+struct Four {
+  typedef typename std::conditional<sizeof(S) == 4, uint32_t, uint16_t>::type one_t;
+  typedef typename std::conditional<sizeof(S) == 4, uint4, uint2>::type all_t;
+  struct Each {
+    one_t e[4];
+  };
+  typename std::conditional<WIDE, all_t, Each>::type v;
+  // `row`: a row of [groups, N], or null.
+  __device__ __forceinline__ void load(const S* row, int n, int N) {
+    if constexpr (WIDE) {
+      v = *reinterpret_cast<const all_t*>(row + (n < N ? n : 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v.e[i] = reinterpret_cast<const one_t*>(row)[min(n + i, N - 1)];
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    return to_f32(__builtin_bit_cast(S, __builtin_bit_cast(Each, v).e[i]));
+  }
 };
 
+// Eight inputs as they are in memory.
 template <typename T>
-constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
-template <typename T>
-using matrix_t = typename std::conditional<sizeof(T) == 4, bf16, T>::type;
-// What the matrix unit sees of code c: kBase<T> + c.
-template <typename T>
-constexpr float kBase = sizeof(T) == 4 ? -8.0f : 16.0f;
-
-// Eight codes as an operand.  Codes 2 i and 2 i + 1 are at bits 4 i and 16 + 4 i.
-template <typename T>
-__device__ __forceinline__ s16x8 decode(uint32_t w) {
-  uint32_t o[4];
-  if constexpr (__is_same(T, f16)) {
-    constexpr uint32_t kMask = 0x03c003c0u, kOne = 0x4c004c00u;  // fp16 of 16: mantissa bits 9..6
-    o[0] = ((w << 6) & kMask) | kOne;
-    o[1] = ((w << 2) & kMask) | kOne;
-    o[2] = ((w >> 2) & kMask) | kOne;
-    o[3] = ((w >> 6) & kMask) | kOne;
-  } else {
-    constexpr uint32_t kMask = 0x00780078u, kOne = 0x41804180u;  // bf16 of 16: mantissa bits 6..3
-    o[0] = ((w << 3) & kMask) | kOne;
-    o[1] = ((w >> 1) & kMask) | kOne;
-    o[2] = ((w >> 5) & kMask) | kOne;
-    o[3] = ((w >> 9) & kMask) | kOne;
-    if constexpr (sizeof(T) == 4) {
+struct Eight {
+  uint4 part[sizeof(T) / 2];
+  // Inputs k .. k + 7 of a row in whole accesses (past the row's end: its first ones).
+  __device__ __forceinline__ void load(const T* row, int k, int K) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = __float_as_uint(bf16_lo(o[i]) - 24.0f);
-        const uint32_t hi = __float_as_uint(bf16_hi(o[i]) - 24.0f);
-        o[i] = (lo >> 16) | hi;  // whole numbers: the low halves are zeros
-      }
-    }
+    for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h)
+      part[h] = reinterpret_cast<const uint4*>(row + (k < K ? k : 0))[h];
   }
-  return __builtin_bit_cast(s16x8, make_uint4(o[0], o[1], o[2], o[3]));
-}
-
-// Ones as an operand.
-template <typename T>
-__device__ __forceinline__ s16x8 ones() {
-  constexpr uint32_t kOnes = __is_same(T, f16) ? 0x3c003c00u : 0x3f803f80u;
-  return __builtin_bit_cast(s16x8, make_uint4(kOnes, kOnes, kOnes, kOnes));
-}
-
-// Inputs k .. k + 7 of a row as an operand (fp32: as three), 0 past the row's end.
-template <typename T>
-__device__ __forceinline__ void load_x(const LinearParams& p, const T* row, int k,
-                                       s16x8 (&part)[kParts<T>]) {
-  if constexpr (sizeof(T) == 2) {
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (p.wide_x) {
-      x = *reinterpret_cast<const uint4*>(row + (k < p.K ? k : 0));
-      if (k >= p.K) x = make_uint4(0, 0, 0, 0);
-    } else {
-      uint16_t e[8];
+  // The same an input at a time, 0 past the row's end.
+  __device__ __forceinline__ void load_each(const T* row, int k, int K) {
+    struct Raw {
+      T e[8];
+    } raw;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        e[i] = k + i < p.K ? reinterpret_cast<const uint16_t*>(row)[k + i] : uint16_t{0};
+    for (int i = 0; i < 8; ++i) raw.e[i] = k + i < K ? row[k + i] : T{};
+    *this = __builtin_bit_cast(Eight, raw);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h) part[h] = make_uint4(0, 0, 0, 0);
+  }
+  // As an operand (fp32: as three).
+  __device__ __forceinline__ void operands(s16x8 (&to)[kParts<T>]) const {
+    if constexpr (sizeof(T) == 2) {
+      to[0] = __builtin_bit_cast(s16x8, part[0]);
+    } else {
       struct Raw {
-        uint16_t e[8];
-      } raw;
+        float e[8];
+      };
+      const Raw raw = __builtin_bit_cast(Raw, *this);
+      float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) raw.e[i] = e[i];
-      x = __builtin_bit_cast(uint4, raw);
+      for (int i = 0; i < 8; ++i) v[i] = raw.e[i];
+      attention::split<3>(v, to);
     }
-    part[0] = __builtin_bit_cast(s16x8, x);
-  } else {
-    float x[8];
-    if (p.wide_x) {
-      const float4 lo = load4(row + (k < p.K ? k : 0)), hi = load4(row + (k < p.K ? k + 4 : 4));
-      x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
-      x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = k < p.K ? x[i] : 0.0f;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = k + i < p.K ? row[k + i] : 0.0f;
-    }
-    attention::split<3>(x, part);
   }
-}
+};
 
-// Four neighbouring values of a row of scales or zero points.
-template <typename S>
-__device__ __forceinline__ f32x4 load_s(const LinearParams& p, const S* row, int n) {
-  if (p.wide_s) {
-    const float4 v = load4(row + (n < p.N ? n : 0));
-    return f32x4{v.x, v.y, v.z, v.w};
-  }
-  f32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = to_f32(row[min(n + i, p.N - 1)]);
-  return v;
-}
-
-__device__ __forceinline__ float activated(int activation, float x) {
-  return activation == kSilu ? x / (1.0f + expf(-x)) : gelu_erf(x);
+// Bytes between the staged rows of two tokens: one 16-byte piece more than their inputs, so that
+// a piece column of 16 tokens spreads over the banks.
+template <typename T>
+constexpr int64_t staged_pitch(int KT) {
+  return static_cast<int64_t>(KT) * kDeep * sizeof(T) + 16;
 }
 
 // MT token tiles of 16, R tiles of 16 weight rows, G matrices; CH matrix instructions to a group
-// (four also where a group is several tiles of codes).
-template <typename T, typename S, int MT, int R, int G, int CH>
-__global__ __launch_bounds__(512) void linear_4bit_kernel(LinearParams p) {
-  constexpr int NP = kParts<T>;
-  extern __shared__ __align__(16) char lds[];  // [wave][G][MT][64] f32x4
+// (four also where a group is several tiles of codes); U tiles of codes loaded at a time, the next U
+// while these are worked on.  STAGED: the tokens' inputs are put into LDS first (one token tile),
+// else they come with the codes.  WIDE: whole accesses (of inputs: where they are not staged).
+template <typename T, typename S, int MT, int R, int G, int CH, int U, bool WIDE, bool STAGED>
+__global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearParams p) {
+  constexpr int NP = kParts<T>, C = 4 / CH;
+  extern __shared__ __align__(16) char lds[];  // inputs; later [wave][G][MT][64] f32x4
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int W = blockDim.x / kWave;
@@ -153,10 +109,88 @@ __global__ __launch_bounds__(512) void linear_4bit_kernel(LinearParams p) {
   const int nt0 = blockIdx.x * R;
   const int m0 = blockIdx.y * 16 * MT;
 
+  struct Batch {
+    uint4 words[U][G][R];
+    Four<S, WIDE> scale[U][C][G][R], zero[U][C][G][R];
+    Eight<T> x[STAGED ? 1 : U][4][MT];
+  };
   const T* rows[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)  // tokens past the last read its row; their outputs are not kept
     rows[t] = static_cast<const T*>(p.x) + static_cast<int64_t>(min(m0 + 16 * t + r, p.M - 1)) * p.x_s;
+  const bool zeros = p.zeros[0] != nullptr;
+  auto load = [&](int k0, Batch& t) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int kt = min(k0 + u * W, p.KT - 1);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          t.words[u][g][i] =
+              p.codes[g][(static_cast<int64_t>(min(nt0 + i, p.NT - 1)) * p.KT + kt) * kWave + lane];
+    }
+    auto vectors = [&](const void* const* of, Four<S, WIDE> (&to)[U][C][G][R]) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          // Past the last input, the last group's.
+          const int kt = min(k0 + u * W, p.KT - 1);
+          const int at = min(CH < 4 ? C * kt + c
+                                    : static_cast<int>(p.by_group_tiles.div(static_cast<uint32_t>(kt))),
+                             (p.K - 1) / p.group);
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+              to[u][c][g][i].load(static_cast<const S*>(of[g]) + static_cast<int64_t>(at) * p.N,
+                                  16 * min(nt0 + i, p.NT - 1) + 4 * quad, p.N);
+        }
+    };
+    vectors(p.scales, t.scale);
+    if (zeros) vectors(p.zeros, t.zero);
+    if constexpr (!STAGED) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const int k = kDeep * min(k0 + u * W, p.KT - 1) + 32 * s + 8 * quad;
+            if constexpr (WIDE)
+              t.x[u][s][i].load(rows[i], k, p.K);
+            else
+              t.x[u][s][i].load_each(rows[i], k, p.K);
+          }
+    }
+  };
+
+  const int pitch = static_cast<int>(staged_pitch<T>(p.KT));
+  Batch cur;
+  if constexpr (STAGED) {
+    const int tokens = min(16, p.M - m0);
+    const int per = p.KT * (kDeep / 8);  // pieces of eight inputs
+    for (int token = 0; token < tokens; ++token) {
+      const T* row = static_cast<const T*>(p.x) + static_cast<int64_t>(m0 + token) * p.x_s;
+      for (int i = threadIdx.x; i < per; i += blockDim.x) {
+        const int k = 8 * i;
+        Eight<T> x;
+        x.clear();
+        if (p.wide_x) {
+          if (k < p.K) x.load(row, k, p.K);
+        } else {
+          x.load_each(row, k, p.K);
+        }
+        *reinterpret_cast<Eight<T>*>(lds + token * pitch + k * sizeof(T)) = x;
+      }
+    }
+    load(wave, cur);
+    __syncthreads();
+  } else {
+    load(wave, cur);
+  }
+  const char* staged = lds + min(r, p.M - 1 - m0) * pitch;
 
   f32x4 total[G][R][MT];
 #pragma unroll
@@ -166,79 +200,77 @@ __global__ __launch_bounds__(512) void linear_4bit_kernel(LinearParams p) {
 #pragma unroll
       for (int t = 0; t < MT; ++t) total[g][i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (int kt = wave; kt < p.KT; kt += W) {
-    uint4 words[G][R];
+  for (int k0 = wave; k0 < p.KT; k0 += W * U) {
+    Batch next;
+    if (k0 + W * U < p.KT) load(k0 + W * U, next);
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int u = 0; u < U; ++u) {
+      const int kt = k0 + u * W;
+      if (u > 0 && kt >= p.KT) break;
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-        words[g][i] =
-            p.codes[g][(static_cast<int64_t>(min(nt0 + i, p.NT - 1)) * p.KT + kt) * kWave + lane];
-#pragma unroll
-    for (int c = 0; c < 4 / CH; ++c) {
-      f32x4 acc[G][R][MT], sum[MT];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int i = 0; i < R; ++i) acc[g][i][t] = sum[t];
-      }
-#pragma unroll
-      for (int s = c * CH; s < (c + 1) * CH; ++s) {
-        s16x8 x[MT][NP];
+      for (int c = 0; c < C; ++c) {
+        f32x4 acc[G][R][MT], sum[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          load_x<T>(p, rows[t], kDeep * kt + 32 * s + 8 * quad, x[t]);
+          sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int n = 0; n < NP; ++n) sum[t] = product(ones<T>(), x[t][n], sum[t], matrix_t<T>{});
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < R; ++i) acc[g][i][t] = sum[t];
+        }
+#pragma unroll
+        for (int s = c * CH; s < (c + 1) * CH; ++s) {
+          s16x8 x[MT][NP];
+          const int k = kDeep * kt + 32 * s + 8 * quad;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            Eight<T> e;
+            if constexpr (STAGED) {
+              e = *reinterpret_cast<const Eight<T>*>(staged + k * sizeof(T));
+            } else {
+              e = cur.x[u][s][t];
+              if (kDeep * (kt + 1) > p.K && k >= p.K) e.clear();
+            }
+            e.operands(x[t]);
+#pragma unroll
+            for (int n = 0; n < NP; ++n)
+              sum[t] = product(ones<T>(), x[t][n], sum[t], matrix_t<T>{});
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+              const s16x8 a = decode<T>(word_of(cur.words[u][g][i], s));
+#pragma unroll
+              for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int n = 0; n < NP; ++n)
+                  acc[g][i][t] = product(a, x[t][n], acc[g][i][t], matrix_t<T>{});
+            }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int i = 0; i < R; ++i) {
-            const uint32_t w = s == 0 ? words[g][i].x : s == 1 ? words[g][i].y
-                               : s == 2 ? words[g][i].z : words[g][i].w;
-            const s16x8 a = decode<T>(w);
+          for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int e = 0; e < 4; ++e) {
+              const float scale = cur.scale[u][c][g][i].at(e);
+              const float off = kBase<T> + (zeros ? cur.zero[u][c][g][i].at(e) : 8.0f);
 #pragma unroll
-              for (int n = 0; n < NP; ++n)
-                acc[g][i][t] = product(a, x[t][n], acc[g][i][t], matrix_t<T>{});
-          }
+              for (int t = 0; t < MT; ++t)
+                total[g][i][t][e] =
+                    fmaf(scale, fmaf(-off, sum[t][e], acc[g][i][t][e]), total[g][i][t][e]);
+            }
       }
-      // The group's scale and zero point, from its first input on; tiles past the last group
-      // (their inputs are zeros) take the last one's.
-      const int first = kDeep * kt + 32 * c * CH;
-      const int at = min(CH < 4 ? first / (32 * CH)
-                                : static_cast<int>(p.by_group_tiles.div(static_cast<uint32_t>(kt))),
-                         (p.K - 1) / p.group);
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          const int n = 16 * min(nt0 + i, p.NT - 1) + 4 * quad;
-          const int64_t line = static_cast<int64_t>(at) * p.N;
-          const f32x4 scale = load_s<S>(p, static_cast<const S*>(p.scales[g]) + line, n);
-          f32x4 off = f32x4{8.0f, 8.0f, 8.0f, 8.0f};
-          if (p.zeros[g] != nullptr) off = load_s<S>(p, static_cast<const S*>(p.zeros[g]) + line, n);
-          off += kBase<T>;
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              total[g][i][t][e] =
-                  fmaf(scale[e], fmaf(-off[e], sum[t][e], acc[g][i][t][e]), total[g][i][t][e]);
-        }
     }
+    cur = next;
   }
 
+  if constexpr (STAGED) __syncthreads();  // the inputs have been read
   f32x4* sums = reinterpret_cast<f32x4*>(lds);
-  T* out = static_cast<T*>(p.out);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    __syncthreads();
+    if (i > 0) __syncthreads();
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -251,53 +283,51 @@ __global__ __launch_bounds__(512) void linear_4bit_kernel(LinearParams p) {
         v[g] = sums[(g * MT + t) * kWave + lane];
         for (int w = 1; w < W; ++w) v[g] += sums[((w * G + g) * MT + t) * kWave + lane];
       }
-      const int token = m0 + 16 * t + r, n = 16 * (nt0 + i) + 4 * quad;
-      if (token >= p.M || n >= p.N) continue;
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = v[0][e];
-        if constexpr (G == 2) y[e] = activated(p.activation, y[e]) * v[G - 1][e];
-        if (p.bias != nullptr) y[e] += load_any_f(p.bias, p.bias_dtype, min(n + e, p.N - 1));
-      }
-      T* dst = out + static_cast<int64_t>(token) * p.N + n;
-      if (p.N % 4 == 0) {
-        put4<T>(dst, y[0], y[1], y[2], y[3]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < p.N) dst[e] = from_f32<T>(y[e]);
-      }
+      finish<T, G>(p, m0 + 16 * t + r, 16 * (nt0 + i) + 4 * quad, v);
     }
   }
 }
 
-template <typename T, typename S, int MT, int R, int G, int CH>
+template <typename T, typename S, int MT, int R, int G, int CH, int U, bool WIDE, bool STAGED>
 hipError_t launch(const LinearParams& p, hipStream_t stream) {
   const char* name = G == 2 ? "gated_linear_4bit" : "linear_4bit";
   int waves = 1;
-  while (waves < 8 && waves < p.KT) waves *= 2;
+  while (waves < kMaxWaves && waves < p.KT) waves *= 2;
   const dim3 grid((p.NT + R - 1) / R, (p.M + 16 * MT - 1) / (16 * MT));
   RLM_REQUIRE(grid.y < 65536u, "%s: too many tokens for one call", name);
   RLM_TRY(check_launch(name, static_cast<int64_t>(grid.x) * grid.y, kWave * waves));
-  const size_t lds = static_cast<size_t>(waves) * G * MT * kWave * 16;
-  if (lds > 48 * 1024) {
+  size_t bytes = static_cast<size_t>(waves) * G * MT * kWave * 16;
+  if (STAGED) bytes = std::max<size_t>(bytes, std::min(p.M, 16) * staged_pitch<T>(p.KT));
+  if (bytes > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(&linear_4bit_kernel<T, S, MT, R, G, CH>),
-        hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
-    RLM_REQUIRE(e == hipSuccess, "%s: %zu bytes of LDS refused: %s", name, lds,
+        reinterpret_cast<const void*>(&linear_4bit_kernel<T, S, MT, R, G, CH, U, WIDE, STAGED>),
+        hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    RLM_REQUIRE(e == hipSuccess, "%s: %zu bytes of LDS refused: %s", name, bytes,
                 hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((linear_4bit_kernel<T, S, MT, R, G, CH>), grid, dim3(kWave * waves), lds,
-                     stream, p);
+  hipLaunchKernelGGL((linear_4bit_kernel<T, S, MT, R, G, CH, U, WIDE, STAGED>), grid,
+                     dim3(kWave * waves), bytes, stream, p);
   return launch_status(name);
 }
 
 template <typename T, typename S, int G, int CH>
 hipError_t launch_tokens(const LinearParams& p, hipStream_t stream) {
-  if (p.M <= 16) return launch<T, S, 1, 1, G, CH>(p, stream);
-  if (p.M <= 32) return launch<T, S, 2, 1, G, CH>(p, stream);
-  return launch<T, S, 4, 1, G, CH>(p, stream);
+  constexpr int U = CH == 1 ? 2 : 4;
+  if (p.M <= 16 && p.M * staged_pitch<T>(p.KT) <= kMaxStaged) {
+    if (!p.wide_s) return launch<T, S, 1, 1, G, CH, 1, false, true>(p, stream);
+    if constexpr (G == 1)
+      if (p.NT >= 512) return launch<T, S, 1, 2, G, CH, U / 2, true, true>(p, stream);
+    return launch<T, S, 1, 1, G, CH, G == 2 ? U / 2 : U, true, true>(p, stream);
+  }
+  if (!p.wide_s || !p.wide_x) return launch<T, S, 2, 1, G, CH, 1, false, false>(p, stream);
+  if (p.M <= 16) {
+    constexpr int V = sizeof(T) == 4 || CH == 1 ? 1 : 2;
+    if constexpr (G == 1)
+      if (p.NT >= 512) return launch<T, S, 1, 2, G, CH, V, true, false>(p, stream);
+    return launch<T, S, 1, 1, G, CH, V, true, false>(p, stream);
+  }
+  if (p.M <= 32 || sizeof(T) == 4) return launch<T, S, 2, 1, G, CH, 1, true, false>(p, stream);
+  return launch<T, S, 4, 1, G, CH, 1, true, false>(p, stream);
 }
 
 template <typename T, typename S, int G>
@@ -398,6 +428,8 @@ hipError_t linear(const rlm_tensor* input, const Weight (&weights)[2], int count
   p.group = static_cast<int>(group_size);
   p.by_group_tiles = FastDiv(static_cast<uint32_t>(std::max<int64_t>(group_size / kDeep, 1)));
   p.activation = activation;
+  if (p.M > 64 && tile_fits(p, input->dtype))
+    return tile_launch(p, count, input->dtype, weights[0].scales->dtype, stream);
   return count == 2 ? launch_types<2>(p, input->dtype, weights[0].scales->dtype, stream)
                     : launch_types<1>(p, input->dtype, weights[0].scales->dtype, stream);
 }

@@ -1,0 +1,119 @@
+// What the kernels of the products with 4-bit weights share: the call's parameters, codes and
+// scales as they are read.
+#pragma once
+
+#include "rlm_attention_mfma.hpp"
+#include "rlm_common.hpp"
+#include "rlm_fastdiv.hpp"
+
+namespace rlm {
+namespace linear4 {
+
+using attention::product;
+using attention::s16x8;
+
+constexpr int kDeep = 128;  // inputs of a tile of codes
+
+enum Activation { kNone = -1, kSilu = 0, kGelu = 1 };
+
+struct LinearParams {
+  const void* x;
+  int64_t x_s;                  // row stride
+  const uint4* codes[2];        // [NT][KT][64]
+  const void* scales[2];        // [G][N]
+  const void* zeros[2];         // or null
+  const void* bias;             // or null
+  int bias_dtype;
+  void* out;
+  int M, N, K, KT, NT;
+  int group;
+  FastDiv by_group_tiles;       // group / 128 where that is above 1
+  int activation;
+  bool wide_x, wide_s;          // whole accesses of inputs; of four scales
+};
+
+template <typename T>
+constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+template <typename T>
+using matrix_t = typename std::conditional<sizeof(T) == 4, bf16, T>::type;
+// What the matrix unit sees of code c: kBase<T> + c.
+template <typename T>
+constexpr float kBase = sizeof(T) == 4 ? -8.0f : 16.0f;
+
+// Eight codes as an operand.  Codes 2 i and 2 i + 1 are at bits 4 i and 16 + 4 i.
+template <typename T>
+__device__ __forceinline__ s16x8 decode(uint32_t w) {
+  uint32_t o[4];
+  // (The base in a vector register: an and-or takes one constant.)
+  uint32_t one;
+  if constexpr (__is_same(T, f16)) {
+    constexpr uint32_t kMask = 0x03c003c0u;  // fp16 of 16: mantissa bits 9..6
+    asm("v_mov_b32 %0, 0x4c004c00" : "=v"(one));
+    o[0] = ((w << 6) & kMask) | one;
+    o[1] = ((w << 2) & kMask) | one;
+    o[2] = ((w >> 2) & kMask) | one;
+    o[3] = ((w >> 6) & kMask) | one;
+  } else {
+    constexpr uint32_t kMask = 0x00780078u;  // bf16 of 16: mantissa bits 6..3
+    asm("v_mov_b32 %0, 0x41804180" : "=v"(one));
+    o[0] = ((w << 3) & kMask) | one;
+    o[1] = ((w >> 1) & kMask) | one;
+    o[2] = ((w >> 5) & kMask) | one;
+    o[3] = ((w >> 9) & kMask) | one;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = __float_as_uint(bf16_lo(o[i]) - 24.0f);
+        const uint32_t hi = __float_as_uint(bf16_hi(o[i]) - 24.0f);
+        o[i] = (lo >> 16) | hi;  // whole numbers: the low halves are zeros
+      }
+    }
+  }
+  return __builtin_bit_cast(s16x8, make_uint4(o[0], o[1], o[2], o[3]));
+}
+
+// Ones as an operand.
+template <typename T>
+__device__ __forceinline__ s16x8 ones() {
+  constexpr uint32_t kOnes = __is_same(T, f16) ? 0x3c003c00u : 0x3f803f80u;
+  return __builtin_bit_cast(s16x8, make_uint4(kOnes, kOnes, kOnes, kOnes));
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& w, int i) {
+  return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+}
+
+__device__ __forceinline__ float activated(int activation, float x) {
+  return activation == kSilu ? x / (1.0f + expf(-x)) : gelu_erf(x);
+}
+
+// Outputs n .. n + 3 of a token from the sums of its one or two (G) products.
+template <typename T, int G>
+__device__ __forceinline__ void finish(const LinearParams& p, int token, int n,
+                                       const f32x4 (&v)[G]) {
+  if (token >= p.M || n >= p.N) return;
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[e] = v[0][e];
+    if constexpr (G == 2) y[e] = activated(p.activation, y[e]) * v[G - 1][e];
+    if (p.bias != nullptr) y[e] += load_any_f(p.bias, p.bias_dtype, min(n + e, p.N - 1));
+  }
+  T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(token) * p.N + n;
+  if (p.N % 4 == 0) {
+    put4<T>(dst, y[0], y[1], y[2], y[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < p.N) dst[e] = from_f32<T>(y[e]);
+  }
+}
+
+// Many tokens: tiles of tokens in LDS shared by the weight rows of a workgroup
+// (rlm_linear_4bit_tile.hip).
+bool tile_fits(const LinearParams& p, int dtype);
+hipError_t tile_launch(const LinearParams& p, int products, int dtype, int scale_dtype,
+                       hipStream_t stream);
+
+}  // namespace linear4
+}  // namespace rlm
