@@ -20,32 +20,11 @@ namespace {
 
 using namespace linear4;
 
-constexpr int kMaxStaged = 64 * 1024;  // bytes of inputs that a workgroup keeps in LDS
+// Bytes of inputs that a workgroup keeps in LDS: as the faster way, and instead of reading them an
+// element at a time.
+constexpr int kMaxStaged = 36 * 1024, kMostStaged = 144 * 1024;
 constexpr int kMaxWaves = 8;
-
-// Raw values of four neighbouring scales or zero points (WIDE: one access), and one of them.
-template <typename S, bool WIDE>
-struct Four {
-  typedef typename std::conditional<sizeof(S) == 4, uint32_t, uint16_t>::type one_t;
-  typedef typename std::conditional<sizeof(S) == 4, uint4, uint2>::type all_t;
-  struct Each {
-    one_t e[4];
-  };
-  typename std::conditional<WIDE, all_t, Each>::type v;
-  // `row`: a row of [groups, N], or null.
-  __device__ __forceinline__ void load(const S* row, int n, int N) {
-    if constexpr (WIDE) {
-      v = *reinterpret_cast<const all_t*>(row + (n < N ? n : 0));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v.e[i] = reinterpret_cast<const one_t*>(row)[min(n + i, N - 1)];
-    }
-  }
-  __device__ __forceinline__ float at(int i) const {
-    return to_f32(__builtin_bit_cast(S, __builtin_bit_cast(Each, v).e[i]));
-  }
-};
+constexpr int kManyTiles = 512;        // 16-row tiles of a weight from which a workgroup has two
 
 // Eight inputs as they are in memory.
 template <typename T>
@@ -101,12 +80,11 @@ constexpr int64_t staged_pitch(int KT) {
 template <typename T, typename S, int MT, int R, int G, int CH, int U, bool WIDE, bool STAGED>
 __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearParams p) {
   constexpr int NP = kParts<T>, C = 4 / CH;
-  extern __shared__ __align__(16) char lds[];  // inputs; later [wave][G][MT][64] f32x4
+  extern __shared__ __align__(16) char lds[];  // inputs; later [wave][G][R][MT][64] f32x4
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int W = blockDim.x / kWave;
   const int r = lane & 15, quad = lane >> 4;
-  const int nt0 = blockIdx.x * R;
   const int m0 = blockIdx.y * 16 * MT;
 
   struct Batch {
@@ -119,6 +97,26 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
   for (int t = 0; t < MT; ++t)  // tokens past the last read its row; their outputs are not kept
     rows[t] = static_cast<const T*>(p.x) + static_cast<int64_t>(min(m0 + 16 * t + r, p.M - 1)) * p.x_s;
   const bool zeros = p.zeros[0] != nullptr;
+  // Codes and scales by uniform offsets.  Rows past the last read others', and nobody keeps their
+  // outputs.
+  const int nt0 = static_cast<int>(blockIdx.x) * R;
+  const int first = min(nt0, p.NT - R);  // R <= NT; the last workgroup may begin in the one before
+  rsrc_t codes[G], scales[G], zero_points[G];
+  const int groups = (p.K + p.group - 1) / p.group;
+  const uint32_t line = static_cast<uint32_t>(p.N) * sizeof(S);
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    codes[g] = make_rsrc(p.codes[g] + static_cast<int64_t>(first) * p.KT * kWave,
+                         static_cast<uint32_t>(R) * p.KT * 1024u);
+    scales[g] = make_rsrc(p.scales[g], groups * line);
+    zero_points[g] = make_rsrc(p.zeros[g], groups * line);
+  }
+  uint32_t lane_off[R][WIDE ? 1 : 4];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int e = 0; e < (WIDE ? 1 : 4); ++e)
+      lane_off[i][e] = min(16 * (first + i) + 4 * quad + e, p.N - (WIDE ? 4 : 1)) * sizeof(S);
   auto load = [&](int k0, Batch& t) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -127,10 +125,11 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
       for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int i = 0; i < R; ++i)
-          t.words[u][g][i] =
-              p.codes[g][(static_cast<int64_t>(min(nt0 + i, p.NT - 1)) * p.KT + kt) * kWave + lane];
+          t.words[u][g][i] = __builtin_bit_cast(
+              uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                         codes[g], 16u * lane, (static_cast<uint32_t>(i) * p.KT + kt) * 1024u, 0));
     }
-    auto vectors = [&](const void* const* of, Four<S, WIDE> (&to)[U][C][G][R]) {
+    auto vectors = [&](const rsrc_t* of, Four<S, WIDE> (&to)[U][C][G][R]) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -139,17 +138,15 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
           const int kt = min(k0 + u * W, p.KT - 1);
           const int at = min(CH < 4 ? C * kt + c
                                     : static_cast<int>(p.by_group_tiles.div(static_cast<uint32_t>(kt))),
-                             (p.K - 1) / p.group);
+                             groups - 1);
 #pragma unroll
           for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int i = 0; i < R; ++i)
-              to[u][c][g][i].load(static_cast<const S*>(of[g]) + static_cast<int64_t>(at) * p.N,
-                                  16 * min(nt0 + i, p.NT - 1) + 4 * quad, p.N);
+            for (int i = 0; i < R; ++i) to[u][c][g][i].load(of[g], lane_off[i], at * line);
         }
     };
-    vectors(p.scales, t.scale);
-    if (zeros) vectors(p.zeros, t.zero);
+    vectors(scales, t.scale);
+    if (zeros) vectors(zero_points, t.zero);
     if constexpr (!STAGED) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -167,7 +164,8 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
   };
 
   const int pitch = static_cast<int>(staged_pitch<T>(p.KT));
-  Batch cur;
+  Batch cur, next;
+  load(wave, cur);
   if constexpr (STAGED) {
     const int tokens = min(16, p.M - m0);
     const int per = p.KT * (kDeep / 8);  // pieces of eight inputs
@@ -185,10 +183,7 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
         *reinterpret_cast<Eight<T>*>(lds + token * pitch + k * sizeof(T)) = x;
       }
     }
-    load(wave, cur);
     __syncthreads();
-  } else {
-    load(wave, cur);
   }
   const char* staged = lds + min(r, p.M - 1 - m0) * pitch;
 
@@ -201,7 +196,6 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
       for (int t = 0; t < MT; ++t) total[g][i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   for (int k0 = wave; k0 < p.KT; k0 += W * U) {
-    Batch next;
     if (k0 + W * U < p.KT) load(k0 + W * U, next);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -248,19 +242,23 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
                   acc[g][i][t] = product(a, x[t][n], acc[g][i][t], matrix_t<T>{});
             }
         }
+        auto add = [&](auto off) {
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+          for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int i = 0; i < R; ++i)
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float scale = cur.scale[u][c][g][i].at(e);
-              const float off = kBase<T> + (zeros ? cur.zero[u][c][g][i].at(e) : 8.0f);
+              for (int e = 0; e < 4; ++e)
 #pragma unroll
-              for (int t = 0; t < MT; ++t)
-                total[g][i][t][e] =
-                    fmaf(scale, fmaf(-off, sum[t][e], acc[g][i][t][e]), total[g][i][t][e]);
-            }
+                for (int t = 0; t < MT; ++t)
+                  total[g][i][t][e] = fmaf(cur.scale[u][c][g][i].at(e),
+                                           fmaf(-off(g, i, e), sum[t][e], acc[g][i][t][e]),
+                                           total[g][i][t][e]);
+        };
+        if (zeros)
+          add([&](int g, int i, int e) { return kBase<T> + cur.zero[u][c][g][i].at(e); });
+        else
+          add([&](int, int, int) { return kBase<T> + 8.0f; });
       }
     }
     cur = next;
@@ -268,23 +266,24 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
 
   if constexpr (STAGED) __syncthreads();  // the inputs have been read
   f32x4* sums = reinterpret_cast<f32x4*>(lds);
+  constexpr int kSums = G * R * MT;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (i > 0) __syncthreads();
+  for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) sums[((wave * G + g) * MT + t) * kWave + lane] = total[g][i][t];
-    __syncthreads();
-    for (int t = wave; t < MT; t += W) {
-      f32x4 v[G];
+      for (int t = 0; t < MT; ++t)
+        sums[(wave * kSums + (g * R + i) * MT + t) * kWave + lane] = total[g][i][t];
+  __syncthreads();
+  for (int j = wave; j < R * MT; j += W) {
+    if (first + j / MT < nt0) continue;
+    f32x4 v[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        v[g] = sums[(g * MT + t) * kWave + lane];
-        for (int w = 1; w < W; ++w) v[g] += sums[((w * G + g) * MT + t) * kWave + lane];
-      }
-      finish<T, G>(p, m0 + 16 * t + r, 16 * (nt0 + i) + 4 * quad, v);
+    for (int g = 0; g < G; ++g) {
+      v[g] = sums[(g * R * MT + j) * kWave + lane];
+      for (int w = 1; w < W; ++w) v[g] += sums[(w * kSums + g * R * MT + j) * kWave + lane];
     }
+    finish<T, G>(p, m0 + 16 * (j % MT) + r, 16 * (first + j / MT) + 4 * quad, v);
   }
 }
 
@@ -296,7 +295,7 @@ hipError_t launch(const LinearParams& p, hipStream_t stream) {
   const dim3 grid((p.NT + R - 1) / R, (p.M + 16 * MT - 1) / (16 * MT));
   RLM_REQUIRE(grid.y < 65536u, "%s: too many tokens for one call", name);
   RLM_TRY(check_launch(name, static_cast<int64_t>(grid.x) * grid.y, kWave * waves));
-  size_t bytes = static_cast<size_t>(waves) * G * MT * kWave * 16;
+  size_t bytes = static_cast<size_t>(waves) * G * R * MT * kWave * 16;
   if (STAGED) bytes = std::max<size_t>(bytes, std::min(p.M, 16) * staged_pitch<T>(p.KT));
   if (bytes > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
@@ -310,24 +309,26 @@ hipError_t launch(const LinearParams& p, hipStream_t stream) {
   return launch_status(name);
 }
 
+// Measured (us, bf16 or fp16, groups of 128; 8 waves):
+//   staged, 1 token: tiles in flight 2 x 1 / 2 x 2 / 2 x 4    4096 to 11008 gated 13.3 / 15.3 / 22.9
+//                    8192 to 8192, rows tiles 2 / 1           10.1 / 11.6    to 28672 28.4 / 31.4
+//   8 tokens of 8192 to 8192: inputs with the codes 12.9 (one row tile 17.2), staged (131 KB of LDS) 15.8
+// Sixteen waves to a workgroup: 1 token gated 16.3, 8192 to 28672 32.9.
 template <typename T, typename S, int G, int CH>
 hipError_t launch_tokens(const LinearParams& p, hipStream_t stream) {
-  constexpr int U = CH == 1 ? 2 : 4;
-  if (p.M <= 16 && p.M * staged_pitch<T>(p.KT) <= kMaxStaged) {
+  if (p.M <= 16 && p.M * staged_pitch<T>(p.KT) <= (p.wide_x ? kMaxStaged : kMostStaged)) {
     if (!p.wide_s) return launch<T, S, 1, 1, G, CH, 1, false, true>(p, stream);
     if constexpr (G == 1)
-      if (p.NT >= 512) return launch<T, S, 1, 2, G, CH, U / 2, true, true>(p, stream);
-    return launch<T, S, 1, 1, G, CH, G == 2 ? U / 2 : U, true, true>(p, stream);
+      if (p.NT >= kManyTiles) return launch<T, S, 1, 2, G, CH, 1, true, true>(p, stream);
+    return launch<T, S, 1, 1, G, CH, G == 2 || CH == 1 ? 1 : 2, true, true>(p, stream);
   }
   if (!p.wide_s || !p.wide_x) return launch<T, S, 2, 1, G, CH, 1, false, false>(p, stream);
   if (p.M <= 16) {
-    constexpr int V = sizeof(T) == 4 || CH == 1 ? 1 : 2;
     if constexpr (G == 1)
-      if (p.NT >= 512) return launch<T, S, 1, 2, G, CH, V, true, false>(p, stream);
-    return launch<T, S, 1, 1, G, CH, V, true, false>(p, stream);
+      if (p.NT >= kManyTiles) return launch<T, S, 1, 2, G, CH, 1, true, false>(p, stream);
+    return launch<T, S, 1, 1, G, CH, 1, true, false>(p, stream);
   }
-  if (p.M <= 32 || sizeof(T) == 4) return launch<T, S, 2, 1, G, CH, 1, true, false>(p, stream);
-  return launch<T, S, 4, 1, G, CH, 1, true, false>(p, stream);
+  return launch<T, S, 2, 1, G, CH, 1, true, false>(p, stream);
 }
 
 template <typename T, typename S, int G>
@@ -345,6 +346,26 @@ hipError_t launch_types(const LinearParams& p, int dtype, int scale_dtype, hipSt
                                   : launch_group<bf16, bf16, G>(p, stream);
   return scale_dtype == RLM_F32 ? launch_group<f16, float, G>(p, stream)
                                 : launch_group<f16, f16, G>(p, stream);
+}
+
+// Whether many tokens share tiles, and how.
+bool tile_shape(const LinearParams& p, int dtype, int products, TileShape* shape) {
+  // 16-bit inputs; a workgroup's tokens, the codes and the scales below 2 GiB each.
+  if (dtype == RLM_F32 || p.M <= 32 || p.x_s >= (int64_t(1) << 22) ||
+      static_cast<int64_t>(p.NT) * p.KT >= (int64_t(1) << 20) ||
+      static_cast<int64_t>((p.K + p.group - 1) / p.group) * p.N >= (int64_t(1) << 28))
+    return false;
+  // Modelled times (us): rounds of workgroups, steps of 128 inputs, a step's time.
+  const int64_t rows = static_cast<int64_t>(p.NT) * products;
+  auto rounds = [&](int tiles, int tokens, int resident) {
+    const int64_t groups = (rows + tiles - 1) / tiles * ((p.M + tokens - 1) / tokens);
+    return static_cast<double>((groups + resident - 1) / resident);
+  };
+  const double wide = rounds(16, 128, 256) * p.KT * 2.45;
+  const double middle = std::min(rounds(8, 64, 256) * 3.9, rounds(8, 64, 512) * 4.5) * ((p.KT + 1) / 2);
+  const double small = rounds(4, 64, 256) * ((p.KT + 3) / 4) * 2.65;
+  *shape = wide <= middle && wide <= small ? kWide : middle <= small ? kMiddle : kSmall;
+  return true;
 }
 
 struct Weight {
@@ -372,6 +393,8 @@ hipError_t linear(const rlm_tensor* input, const Weight (&weights)[2], int count
   RLM_REQUIRE(N >= 1 && N <= (int64_t(1) << 24), "%s: outputs must be in [1, 2^24], got %lld",
               weights[0].scales_name, (long long)N);
   const int64_t NT = (N + 15) / 16;
+  RLM_REQUIRE(groups * N < (int64_t(1) << 29), "%s: fewer than 2^29 elements, got %lld",
+              weights[0].scales_name, (long long)(groups * N));
   const int64_t per_scale = 4 * dtype_size(weights[0].scales->dtype);
   p.wide_s = N % 4 == 0;
   for (int g = 0; g < count; ++g) {
@@ -428,8 +451,11 @@ hipError_t linear(const rlm_tensor* input, const Weight (&weights)[2], int count
   p.group = static_cast<int>(group_size);
   p.by_group_tiles = FastDiv(static_cast<uint32_t>(std::max<int64_t>(group_size / kDeep, 1)));
   p.activation = activation;
-  if (p.M > 64 && tile_fits(p, input->dtype))
-    return tile_launch(p, count, input->dtype, weights[0].scales->dtype, stream);
+  TileShape shape;
+  if (tile_shape(p, input->dtype, count, &shape))
+    return input->dtype == RLM_BF16
+               ? tile_launch_bf16(p, shape, count, weights[0].scales->dtype, stream)
+               : tile_launch_f16(p, shape, count, weights[0].scales->dtype, stream);
   return count == 2 ? launch_types<2>(p, input->dtype, weights[0].scales->dtype, stream)
                     : launch_types<1>(p, input->dtype, weights[0].scales->dtype, stream);
 }

@@ -79,6 +79,38 @@ __device__ __forceinline__ s16x8 ones() {
   return __builtin_bit_cast(s16x8, make_uint4(kOnes, kOnes, kOnes, kOnes));
 }
 
+// Raw values of four neighbouring scales or zero points (WIDE: one access), and one of them.
+template <typename S, bool WIDE>
+struct Four {
+  typedef typename std::conditional<sizeof(S) == 4, uint32_t, uint16_t>::type one_t;
+  struct Each {
+    one_t e[4];
+  };
+  typename std::conditional<sizeof(S) == 4, uint4, uint2>::type v;
+  // lane_off: this lane's byte offsets in a row, row_off: the row's.
+  __device__ __forceinline__ void load(rsrc_t r, const uint32_t (&lane_off)[WIDE ? 1 : 4],
+                                       uint32_t row_off) {
+    if constexpr (WIDE && sizeof(S) == 4) {
+      v = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_off[0], row_off, 0));
+    } else if constexpr (WIDE) {
+      v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_off[0], row_off, 0));
+    } else {
+      Each x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(S) == 4)
+          x.e[i] = __builtin_amdgcn_raw_buffer_load_b32(r, lane_off[i], row_off, 0);
+        else
+          x.e[i] = __builtin_amdgcn_raw_buffer_load_b16(r, lane_off[i], row_off, 0);
+      }
+      v = __builtin_bit_cast(decltype(v), x);
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    return to_f32(__builtin_bit_cast(S, __builtin_bit_cast(Each, v).e[i]));
+  }
+};
+
 __device__ __forceinline__ uint32_t word_of(const uint4& w, int i) {
   return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
 }
@@ -110,10 +142,13 @@ __device__ __forceinline__ void finish(const LinearParams& p, int token, int n,
 }
 
 // Many tokens: tiles of tokens in LDS shared by the weight rows of a workgroup
-// (rlm_linear_4bit_tile.hip).
-bool tile_fits(const LinearParams& p, int dtype);
-hipError_t tile_launch(const LinearParams& p, int products, int dtype, int scale_dtype,
-                       hipStream_t stream);
+// (rlm_linear_4bit_tile.hpp), which has 256 rows and 128 tokens, 128 and 64 in two parts of the inputs,
+// or 64 and 64 in four parts.
+enum TileShape { kWide, kMiddle, kSmall };
+hipError_t tile_launch_bf16(const LinearParams& p, TileShape shape, int products, int scale_dtype,
+                            hipStream_t stream);
+hipError_t tile_launch_f16(const LinearParams& p, TileShape shape, int products, int scale_dtype,
+                           hipStream_t stream);
 
 }  // namespace linear4
 }  // namespace rlm

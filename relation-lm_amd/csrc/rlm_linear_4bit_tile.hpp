@@ -1,0 +1,382 @@
+// Products with 4-bit weights for many tokens: x tiles in LDS shared by the weight rows of a workgroup.
+// (Instances: rlm_linear_4bit_bf16.hip, rlm_linear_4bit_f16.hip.)
+//
+// A wave has 64 weight rows (gated: 32 of each weight) and 64 tokens, a workgroup WR by WT waves of them
+// for each of WK parts of the inputs.  Inputs come by DMA into LDS, 128 of each token at a time, the
+// next 128 on their way while these are worked on; codes come from memory straight into registers in
+// operand order.  Per group, total += s acc with acc = sum (16 + c) x; what the 16 and the zero point
+// add,
+//   sum_g (16 + z_g) s_g X_g,   X_g = the group's sum of inputs,
+// is itself a product over groups: the waves that share tokens each sum some of them, with ones as the
+// other operand, and every 32 (or 16) groups (16 + z) s and X meet as sums of three bf16 parts (six
+// products, to 2^-24 of their size).  The parts of the inputs are added in LDS at the end, in order.
+#pragma once
+
+#include "rlm_linear_4bit.hpp"
+
+namespace rlm {
+namespace linear4 {
+
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+typedef const __attribute__((address_space(3))) s16x8* lds_frag;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) u32x4* lds_piece;
+typedef const __attribute__((address_space(3))) f32x4* lds_f32x4;
+typedef __attribute__((address_space(3))) float* lds_float;
+
+// Groups whose sums are kept, and the floats between two tokens' sums.
+template <int WK>
+constexpr int kChunks = WK == 1 ? 32 : 16;
+template <int WK>
+constexpr int kSumPitch = kChunks<WK> + 4;
+template <int WT, int WK>
+constexpr int kTileLds = WK * 64 * WT * (2 * 2 * kDeep + 4 * kSumPitch<WK>);
+
+// Eight 16-bit inputs at any address: those below K.
+template <typename T>
+__device__ __forceinline__ u32x4 eight_inputs(const T* row, int k, int K) {
+  u32x4 v = {0, 0, 0, 0};
+  if (k + 8 <= K) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else {
+    struct Raw {
+      T e[8];
+    } raw;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw.e[i] = k + i < K ? row[k + i] : T{};
+    v = __builtin_bit_cast(u32x4, raw);
+  }
+  return v;
+}
+
+// G products; CH matrix instructions to a group (four also where a group is several tiles).  ALIGNED:
+// inputs by DMA, four scales at a time.
+template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED>
+__global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bit_tile_kernel(LinearParams p,
+                                                                                FastDiv by_rows) {
+  constexpr int R = 4 / G;                       // 16-row tiles of a wave, of each weight
+  constexpr int C = 4 / CH;                      // groups of a tile of codes
+  constexpr int kTokens = 64 * WT;               // of a workgroup
+  constexpr int kStage = kTokens * kDeep * 2;    // bytes of inputs
+  constexpr int NC = kChunks<WK>, kPitch = kSumPitch<WK>;
+  extern __shared__ __align__(1024) char lds[];  // [WK][2] stages, [WK] sums
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 15, quad = lane >> 4;
+  // Neighbouring workgroups of an XCD share tokens and, a row of workgroups later, weights.
+  uint32_t row_block;
+  const uint32_t token_block =
+      by_rows.div(static_cast<uint32_t>(xcd_tile(blockIdx.x, gridDim.x)), row_block);
+  const int m0 = static_cast<int>(token_block) * kTokens;
+  const int rq = wave % WR, half = wave / WR % WT, kq = wave / (WR * WT);
+  const int nt0 = static_cast<int>(row_block) * WR * R + rq * R;
+  const int mate = wave % (WR * WT);             // of the waves that share a part of the inputs
+  // This part's tiles of codes.
+  const int per = (p.KT + WK - 1) / WK;
+  const int kt0 = kq * per, tiles = min(per, p.KT - kt0);  // (none or fewer for the last parts)
+
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const uint32_t stages = lds0 + kq * 2 * kStage;
+  // Rows of 16 pieces, swizzled so that a piece column spreads over all banks.  A wave brings four
+  // rows at a time: rows 4 j .. 4 j + 3 for j = mate, mate + WR WT, ...
+  constexpr int kBring = kTokens / 4 / (WR * WT);
+  const T* base = static_cast<const T*>(p.x) + static_cast<int64_t>(m0) * p.x_s;
+  const int rows = min(kTokens, p.M - m0);
+  const uint32_t row_bytes = static_cast<uint32_t>(p.x_s) * 2;
+  // (Rows past the last are out of range and come as zeros.)
+  const rsrc_t x_rows = make_rsrc(base, static_cast<uint32_t>(rows - 1) * row_bytes + 2u * p.K);
+  auto issue = [&](int i) {
+    const int kt = kt0 + i;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(stages + (i & 1) * kStage);
+#pragma unroll
+    for (int n = 0; n < kBring; ++n) {
+      const int j = mate + n * WR * WT;
+      const int k = kDeep * kt + 8 * ((lane & 15) ^ (lane >> 4) ^ (4 * (j & 3)));
+      if constexpr (ALIGNED) {
+        const uint32_t off = static_cast<uint32_t>(4 * j + (lane >> 4)) * row_bytes + 2u * k;
+        lds_dma16(x_rows, to + 1024u * j, kDeep * (kt + 1) <= p.K || k < p.K ? off : kNoOffset);
+      } else {
+        const int row = min(4 * j + (lane >> 4), rows - 1);
+        *(lds_piece)static_cast<uintptr_t>(to + 1024u * j + 16 * lane) =
+            eight_inputs(base + static_cast<int64_t>(row) * p.x_s, k, p.K);
+      }
+    }
+  };
+  // Tiles of codes and scales by uniform offsets; rows past the last read others', and nobody keeps
+  // their outputs.
+  auto tile_of = [&](int i) { return min(nt0 + i, p.NT - 1); };
+  rsrc_t codes[G], scales[G];
+  const int groups = (p.K + p.group - 1) / p.group;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    codes[g] = make_rsrc(p.codes[g], static_cast<uint32_t>(p.NT) * p.KT * 1024u);
+    scales[g] = make_rsrc(p.scales[g], static_cast<uint32_t>(groups) * p.N * sizeof(S));
+  }
+  auto load_words = [&](int kt, uint4 (&w)[G][R]) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        w[g][i] = __builtin_bit_cast(
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                       codes[g], 16u * lane, (static_cast<uint32_t>(tile_of(i)) * p.KT + kt) * 1024u, 0));
+  };
+
+  float total[G][R][4][4];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[g][i][t][e] = 0.0f;
+
+  uint4 words[G][R];
+  load_words(min(kt0, p.KT - 1), words);
+  if (tiles > 0) issue(0);
+
+  // Sums kept, NC chunks of each token of this part.
+  const uint32_t sums0 = lds0 + WK * 2 * kStage + (kq * kTokens + 64 * half) * kPitch * 4;
+  auto group_of = [&](int chunk) {  // a chunk's group; past the last input, the last one
+    const int at = CH < 4 ? chunk : static_cast<int>(p.by_group_tiles.div(static_cast<uint32_t>(chunk)));
+    return min(at, groups - 1);
+  };
+  const uint32_t x_row = (64 * half + r) * 256 + ((quad ^ r) << 4);
+
+  for (int n = 0; n < per; ++n) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    barrier();  // these inputs are in LDS for every wave, the other stage has been read
+    if (n + 1 < tiles) issue(n + 1);
+    if (n < tiles) {
+      const int kt = kt0 + n;
+      uint4 next[G][R];
+      load_words(min(kt + 1, p.KT - 1), next);
+      const uint32_t x_at = stages + (n & 1) * kStage + x_row;
+      auto inputs = [&](int s, s16x8 (&x)[4]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          x[t] = *(lds_frag)static_cast<uintptr_t>((x_at ^ (64u * s)) + 4096u * t);
+      };
+      s16x8 x[4];
+      inputs(0, x);
+      // (A loop where it has several rounds: unrolled, it spills.)
+#pragma unroll 1
+      for (int c = 0; c < C; ++c) {
+        const int chunk = C * kt + c;
+        const uint32_t line = static_cast<uint32_t>(group_of(chunk)) * p.N;
+        Four<S, ALIGNED> scale[G][R];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            uint32_t lane_off[ALIGNED ? 1 : 4];
+#pragma unroll
+            for (int e = 0; e < (ALIGNED ? 1 : 4); ++e)
+              lane_off[e] = min(4 * quad + e, p.N - (ALIGNED ? 4 : 1) - 16 * tile_of(i)) * sizeof(S);
+            scale[g][i].load(scales[g], lane_off, (line + 16 * tile_of(i)) * sizeof(S));
+          }
+        f32x4 acc[G][R][4], sum[4 / WR];
+#pragma unroll
+        for (int t = 0; t < 4 / WR; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[g][i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < CH; ++s) {
+          s16x8 x_next[4];
+          inputs((c * CH + s + 1) & 3, x_next);
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+              const s16x8 a = decode<T>(word_of(words[g][i], s));
+#pragma unroll
+              for (int t = 0; t < 4; ++t) acc[g][i][t] = product(a, x[t], acc[g][i][t], T{});
+            }
+          __builtin_amdgcn_sched_barrier(0);  // operands of one step and the next live at once
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (WR == 1 || rq == t % WR) sum[t / WR] = product(ones<T>(), x[t], sum[t / WR], T{});
+#pragma unroll
+          for (int t = 0; t < 4; ++t) x[t] = x_next[t];
+        }
+        if (quad == 0) {
+#pragma unroll
+          for (int t = 0; t < 4 / WR; ++t)
+            *(lds_float)static_cast<uintptr_t>(sums0 + ((16 * (t * WR + rq) + r) * kPitch +
+                                                        (C * n + c) % NC) * 4) = sum[t][0];
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                total[g][i][t][e] = fmaf(scale[g][i].at(e), acc[g][i][t][e], total[g][i][t][e]);
+        if constexpr (CH < 4) {  // the next chunk's words to the front
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+              const uint4 w = words[g][i];
+              words[g][i] = CH == 1 ? make_uint4(w.y, w.z, w.w, w.x) : make_uint4(w.z, w.w, w.x, w.y);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < R; ++i) words[g][i] = next[g][i];
+    }
+
+    // total -= ((16 + z) s) X over the kept chunks.
+    const int done = C * (n + 1);
+    if (done % NC != 0 && n + 1 != per) continue;
+    barrier();
+    const int kept = (done - 1) / NC * NC;                     // the first one, of this part's,
+    const int end = min(done, C * tiles);                      // and behind the last
+    if (kept >= end) continue;
+    s16x8 xs[4][3];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t at = sums0 + (16 * t + r) * kPitch * 4 + 32 * min(quad, NC / 8 - 1);
+      const f32x4 lo = *(lds_f32x4)static_cast<uintptr_t>(at);
+      const f32x4 hi = *(lds_f32x4)static_cast<uintptr_t>(at + 16);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = e < 4 ? lo[e] : hi[e - 4];
+        v[e] = kept + 8 * quad + e < end ? v[e] : 0.0f;
+      }
+      attention::split<3>(v, xs[t]);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int row = min(16 * (nt0 + i) + r, p.N - 1);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int chunk = min(kept + 8 * quad + e, end - 1);
+          const int64_t at = static_cast<int64_t>(group_of(C * kt0 + chunk)) * p.N + row;
+          float z = 8.0f;
+          if (p.zeros[g] != nullptr) z = to_f32(static_cast<const S*>(p.zeros[g])[at]);
+          v[e] = kept + 8 * quad + e < end
+                     ? (kBase<T> + z) * to_f32(static_cast<const S*>(p.scales[g])[at]) : 0.0f;
+        }
+        s16x8 cs[3];
+        attention::split<3>(v, cs);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+          a = product(cs[2], xs[t][0], a, bf16{});
+          a = product(cs[0], xs[t][2], a, bf16{});
+          a = product(cs[1], xs[t][1], a, bf16{});
+          a = product(cs[1], xs[t][0], a, bf16{});
+          a = product(cs[0], xs[t][1], a, bf16{});
+          a = product(cs[0], xs[t][0], a, bf16{});
+#pragma unroll
+          for (int e = 0; e < 4; ++e) total[g][i][t][e] -= a[e];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+
+  const int token0 = m0 + 64 * half + r, out0 = 16 * nt0 + 4 * quad;
+  if constexpr (WK == 1) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        f32x4 v[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[g][e] = total[g][i][t][e];
+        finish<T, G>(p, token0 + 16 * t, out0 + 16 * i, v);
+      }
+  } else {
+    // Part kq finishes the token tiles kq, kq + WK, ...
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    barrier();
+    f32x4* parts = reinterpret_cast<f32x4*>(lds);  // [wave][G][R][4][64]
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          parts[(((wave * G + g) * R + i) * 4 + t) * kWave + lane] =
+              f32x4{total[g][i][t][0], total[g][i][t][1], total[g][i][t][2], total[g][i][t][3]};
+    barrier();
+    for (int t = kq; t < 4; t += WK)
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        f32x4 v[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          v[g] = parts[(((mate * G + g) * R + i) * 4 + t) * kWave + lane];
+#pragma unroll
+          for (int w = 1; w < WK; ++w)
+            v[g] += parts[((((w * WR * WT + mate) * G + g) * R + i) * 4 + t) * kWave + lane];
+        }
+        finish<T, G>(p, token0 + 16 * t, out0 + 16 * i, v);
+      }
+  }
+}
+
+template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED>
+hipError_t launch_tile(const LinearParams& p, hipStream_t stream) {
+  const char* name = G == 2 ? "gated_linear_4bit" : "linear_4bit";
+  constexpr int kThreads = WR * WT * WK * kWave, kLds = kTileLds<WT, WK>;
+  static_assert(WK == 1 || kThreads * 256 <= WK * 2 * 64 * WT * kDeep * 2, "parts in the stages");
+  const int64_t row_blocks = (p.NT + WR * 4 / G - 1) / (WR * 4 / G);
+  const int64_t token_blocks = (p.M + 64 * WT - 1) / (64 * WT);
+  RLM_TRY(check_launch(name, row_blocks * token_blocks, kThreads));
+  const auto kernel = &linear_4bit_tile_kernel<T, S, G, CH, WR, WT, WK, ALIGNED>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  RLM_REQUIRE(e == hipSuccess, "%s: %d bytes of LDS refused: %s", name, kLds, hipGetErrorString(e));
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(row_blocks * token_blocks)), dim3(kThreads),
+                     kLds, stream, p, FastDiv(static_cast<uint32_t>(row_blocks)));
+  return launch_status(name);
+}
+
+template <typename T, typename S, int G, int CH>
+hipError_t launch_shape(const LinearParams& p, TileShape shape, hipStream_t stream) {
+  if (!p.wide_x || !p.wide_s) return launch_tile<T, S, G, CH, 2, 1, 2, false>(p, stream);
+  if (shape == kWide) return launch_tile<T, S, G, CH, 4, 2, 1, true>(p, stream);
+  if (shape == kMiddle) return launch_tile<T, S, G, CH, 2, 1, 2, true>(p, stream);
+  return launch_tile<T, S, G, CH, 1, 1, 4, true>(p, stream);
+}
+template <typename T, typename S, int G>
+hipError_t launch_group_tile(const LinearParams& p, TileShape shape, hipStream_t stream) {
+  if (p.group == 32) return launch_shape<T, S, G, 1>(p, shape, stream);
+  if (p.group == 64) return launch_shape<T, S, G, 2>(p, shape, stream);
+  return launch_shape<T, S, G, 4>(p, shape, stream);
+}
+template <typename T>
+hipError_t launch_tile_type(const LinearParams& p, TileShape shape, int products, int scale_dtype,
+                            hipStream_t stream) {
+  if (products == 2)
+    return scale_dtype == RLM_F32 ? launch_group_tile<T, float, 2>(p, shape, stream)
+                                  : launch_group_tile<T, T, 2>(p, shape, stream);
+  return scale_dtype == RLM_F32 ? launch_group_tile<T, float, 1>(p, shape, stream)
+                                : launch_group_tile<T, T, 1>(p, shape, stream);
+}
+
+}  // namespace linear4
+}  // namespace rlm
