@@ -151,9 +151,13 @@ __device__ __forceinline__ void buf_store_f32(float v, rsrc_t r, uint32_t off) {
 // vmcnt(0) before the next LDS access; the caller waits (s_waitcnt vmcnt +
 // barrier) before the data is read.  The LDS base travels in M0, passed as an
 // operand bound to that register ("{m0}"), so the compiler writes M0 itself
-// and knows it holds this value.
+// and knows it holds this value.  The five wait states before the load are those
+// that a vector instruction's scalar result (v_readlane, v_readfirstlane) has to
+// age before a vector-memory instruction reads it: the compiler inserts them for
+// its own instructions only, and where it has spilled the descriptor to lanes of a
+// register it reads it back right before the load.
 __device__ __forceinline__ void lds_dma16(rsrc_t r, uint32_t lds_addr, uint32_t voff) {
-  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds"
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                :
                : "v"(voff), "s"(r), "{m0}"(lds_addr)
                : "memory");
@@ -161,7 +165,7 @@ __device__ __forceinline__ void lds_dma16(rsrc_t r, uint32_t lds_addr, uint32_t 
 // The same with a wave-uniform byte offset added to every lane's (soff, an SGPR).
 __device__ __forceinline__ void lds_dma16(rsrc_t r, uint32_t lds_addr, uint32_t voff,
                                           uint32_t soff) {
-  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds"
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                :
                : "v"(voff), "s"(r), "s"(soff), "{m0}"(lds_addr)
                : "memory");
