@@ -158,5 +158,7 @@ extern "C" hipError_t rlm_routed_attention_quantized(
       fill(query, key_cache, value_cache, key_scale, value_scale, true, blocks, positions,
            block_size, local_window, scale, ring, out, out_lse, p);
   if (e != hipSuccess || p.items == 0) return e;
-  return quantized_launch(p, query->dtype, stream);
+  const int waves = quantized_tile_waves(p, query->dtype);
+  return waves != 0 ? quantized_tile_launch(p, query->dtype, waves, stream)
+                    : quantized_launch(p, query->dtype, stream);
 }

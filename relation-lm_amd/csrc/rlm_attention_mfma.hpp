@@ -83,5 +83,74 @@ __device__ __forceinline__ s16x8 read_values(uint32_t at, uint32_t apart) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// ---- Caches of 8 bits: e4m3 codes, exact in bf16, met by operands that are sums of bf16 parts.
+
+struct code8 {
+  uint8_t bits;
+};
+__device__ __forceinline__ float code_to_f32(code8 c) {
+  return __builtin_amdgcn_cvt_f32_fp8(c.bits, 0);
+}
+
+// Parts of a query, and of the weights that meet the values.
+template <typename T>
+constexpr int kParts = sizeof(T) == 4 ? 3 : __is_same(T, f16) ? 2 : 1;
+template <typename T>
+constexpr int kWeightParts = sizeof(T) == 4 ? 3 : 2;
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
+typedef const __attribute__((address_space(3))) f32x4* lds_f32x4;
+
+// 16-byte pieces of an LDS row of at most 16 PIECES codes, and where a row's pieces stand: 32 rows
+// of one piece column, as a transposing read takes them, spread over all banks.
+constexpr int code_pitch(int pieces) {
+  return pieces <= 2 ? 2 : pieces <= 4 ? 4 : pieces <= 8 ? 8 : 16;
+}
+template <int PITCH>
+__device__ __forceinline__ int code_swizzle(int row) {
+  return PITCH == 2 ? (row >> 3) & 1 : swizzle<PITCH>(row);
+}
+
+// Eight codes as bf16.
+__device__ __forceinline__ s16x8 decode8(uint32_t lo, uint32_t hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true)};
+  return __builtin_bit_cast(s16x8, x);
+}
+
+// Eight elements of a query as bf16 parts.
+template <typename T>
+__device__ __forceinline__ void load_parts(const T* src, bool there, s16x8 (&part)[kParts<T>]) {
+  if constexpr (__is_same(T, bf16)) {
+    uint4 x = *reinterpret_cast<const uint4*>(src);
+    if (!there) x = make_uint4(0, 0, 0, 0);
+    part[0] = __builtin_bit_cast(s16x8, x);
+  } else {
+    float x[8];
+    const float4 lo = load4(src), hi = load4(src + 4);
+    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
+    x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = there ? x[e] : 0.0f;
+    split<kParts<T>>(x, part);
+  }
+}
+
+// The first of the eight features of a row of codes that lane group `quad` has for product j (an order
+// that gives a lane 16 neighbouring codes where it can).
+template <int DC>
+__device__ __forceinline__ int code_feature(int j, int quad) {
+  return j < DC / 2 * 2 ? 64 * (j / 2) + 16 * quad + 8 * (j & 1) : 32 * j + 8 * quad;
+}
+// The key of 32 whose codes lane (r, quad) reads for a transposing read: the keys of a lane group's
+// weights, 4 quad .. + 3 and 16 + 4 quad .. + 3.
+__device__ __forceinline__ int code_row(int r, int quad) {
+  return 4 * quad + ((r >> 1) & 3) + 16 * (r >> 3);
+}
+
 }  // namespace attention
 }  // namespace rlm

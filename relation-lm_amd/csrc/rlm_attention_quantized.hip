@@ -24,53 +24,6 @@ using namespace attention;
 
 constexpr int kKeys = 32;  // keys of a wave's tile
 
-template <typename T>  // of a query
-constexpr int kParts = sizeof(T) == 4 ? 3 : __is_same(T, f16) ? 2 : 1;
-template <typename T>
-constexpr int kWeightParts = sizeof(T) == 4 ? 3 : 2;
-
-typedef int i32x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
-typedef const __attribute__((address_space(3))) f32x4* lds_f32x4;
-
-// 16-byte pieces of an LDS row of at most 16 PIECES codes, and where a row's pieces stand: 32 rows
-// of one piece column, as a transposing read takes them, spread over all banks.
-constexpr int code_pitch(int pieces) {
-  return pieces <= 2 ? 2 : pieces <= 4 ? 4 : pieces <= 8 ? 8 : 16;
-}
-template <int PITCH>
-__device__ __forceinline__ int code_swizzle(int row) {
-  return PITCH == 2 ? (row >> 3) & 1 : swizzle<PITCH>(row);
-}
-
-// Eight codes as bf16.
-__device__ __forceinline__ s16x8 decode(uint32_t lo, uint32_t hi) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false),
-                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true),
-                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false),
-                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true)};
-  return __builtin_bit_cast(s16x8, x);
-}
-
-// Eight elements of a query as bf16 parts.
-template <typename T>
-__device__ __forceinline__ void load_parts(const T* src, bool there, s16x8 (&part)[kParts<T>]) {
-  if constexpr (__is_same(T, bf16)) {
-    uint4 x = *reinterpret_cast<const uint4*>(src);
-    if (!there) x = make_uint4(0, 0, 0, 0);
-    part[0] = __builtin_bit_cast(s16x8, x);
-  } else {
-    float x[8];
-    const float4 lo = load4(src), hi = load4(src + 4);
-    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
-    x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = there ? x[e] : 0.0f;
-    split<kParts<T>>(x, part);
-  }
-}
-
 // DC: head dim in 32s; SHARES workgroups have a share of the value features each.
 template <typename T, int DC, int MAXW, int SHARES>
 __global__ __launch_bounds__(MAXW* kWave) void attend_codes_kernel(Params p) {
@@ -101,10 +54,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_codes_kernel(Params p) {
   const int32_t* picks = p.blocks + b * p.blk_sb + step * p.blk_st + hk * p.blk_sh;
   int32_t pick = lane < p.TOP ? picks[lane] : -1;
 
-  // The first of the eight features that lane group `quad` has of piece j.
-  auto feature = [&](int j) {
-    return j < DC / 2 * 2 ? 64 * (j / 2) + 16 * quad + 8 * (j & 1) : 32 * j + 8 * quad;
-  };
+  auto feature = [&](int j) { return code_feature<DC>(j, quad); };
   s16x8 qf[DC][NP];
   {
     const T* src = static_cast<const T*>(p.q) + b * p.q_sb + step * p.q_st + head * p.q_sh;
@@ -206,7 +156,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_codes_kernel(Params p) {
 #pragma unroll
       for (int j = 0; j < DC; ++j) {
         const uint4 w = kw[kt][j / 2];
-        const s16x8 kf = j & 1 ? decode(w.z, w.w) : decode(w.x, w.y);
+        const s16x8 kf = j & 1 ? decode8(w.z, w.w) : decode8(w.x, w.y);
 #pragma unroll
         for (int n = 0; n < NP; ++n) s = product(kf, qf[j][n], s, bf16{});
       }
@@ -240,8 +190,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_codes_kernel(Params p) {
     for (int j = 0; j < DT; ++j) acc[j] *= fade;
     s16x8 weights[NW];
     split<NW>(x, weights);
-    // Keys in the order of the weights: 4 quad .. + 3, then 16 + 4 quad .. + 3.
-    const int vrow = 4 * quad + ((r >> 1) & 3) + 16 * (r >> 3);
+    const int vrow = code_row(r, quad);
     const uint32_t value0 = mine + vrow * kRow + (code_swizzle<kPitch>(vrow) << 4) + (r & 1) * 8;
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     wave_sync();
@@ -249,7 +198,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_codes_kernel(Params p) {
     for (int j = 0; j < DT; ++j) {
       const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
           (lds_i32x2)static_cast<uintptr_t>(value0 ^ (16u * j)));
-      const s16x8 vf = decode(static_cast<uint32_t>(c[0]), static_cast<uint32_t>(c[1]));
+      const s16x8 vf = decode8(static_cast<uint32_t>(c[0]), static_cast<uint32_t>(c[1]));
 #pragma unroll
       for (int n = 0; n < NW; ++n) acc[j] = product(vf, weights[n], acc[j], bf16{});
     }

@@ -1,0 +1,105 @@
+// Key tiles shared by the rows of a workgroup (rlm_attention_tile.hpp) over caches of 8 bits.
+//
+// Tiles of codes come by DMA as they are, with their rows' scales, a wave's keys' and another's values';
+// keys are decoded as they are read from LDS, values by transposing 8-bit reads.  A query is a sum of bf16
+// parts, the weights times their values' scales likewise (rlm_attention_quantized.hip says which).
+//
+// Bound: instructions.  A wave spends about 400 on 64 keys of 64 features, 64 of them on decoding and 48 on
+// splitting the weights, for 24 products; a third of the weights are of keys that a row did not pick.
+// 2 x 999 queries of 12 heads on 4 of 64 features (a window of 128, eight of up to 128 blocks of 64)
+// take 65 us, a query to a workgroup 79; 4 x 4096 take 167 us and 8000 of 16 on 2 of 128 (256, eight)
+// 189, where caches of 16 bits, with nothing to decode, take 110 and 124.
+#include "rlm_attention_tile.hpp"
+
+namespace rlm {
+namespace {
+
+// Tiles of 64 keys up to 64 features, of 32 above.  Measured with 32 and one wave where 64 are taken: 76
+// against 63 us, and with 64 where 32 are: 189 against 64 (2 x 999 queries of 12 heads on 4 of 64 and of
+// 16 on 2 of 128 features).  A third and fourth tile under way bring nothing: what a wave does with a
+// tile, about 400 instructions to 64 keys, hides the loads of the next.
+template <typename T, bool WHOLE, int kWaves>
+hipError_t launch_waves(TileParams& tp, hipStream_t stream) {
+  const int dc = (tp.p.D + 31) / 32;
+  if (dc <= 1) return launch_tiles<T, code8, 1, WHOLE, 64, kWaves>(tp, stream);
+  if (dc <= 2) return launch_tiles<T, code8, 2, WHOLE, 64, kWaves>(tp, stream);
+  if (dc <= 3) return launch_tiles<T, code8, 3, WHOLE, 32, kWaves>(tp, stream);
+  if (dc <= 4) return launch_tiles<T, code8, 4, WHOLE, 32, kWaves>(tp, stream);
+  return launch_tiles<T, code8, 8, WHOLE, 32, kWaves>(tp, stream);
+}
+
+template <typename T, bool WHOLE>
+hipError_t launch_type(TileParams& tp, int waves, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2)
+    if (waves == 4) return launch_waves<T, WHOLE, 4>(tp, stream);
+  return launch_waves<T, WHOLE, 1>(tp, stream);
+}
+
+bool fits(const Params& p) {
+  const int64_t limit = (int64_t(1) << 31) / kMostKeys - 1;  // a tile, and its scales, below 2 GiB
+  return !p.ring && p.Tq > 1 && p.T >= 1 && p.BS % 4 == 0 && p.k_st < limit && p.v_st < limit &&
+         4 * p.ks_st < limit && 4 * p.vs_st < limit &&
+         static_cast<int64_t>(p.B) * p.Hk * ((p.G + 15) / 16) * p.Tq < (int64_t(1) << 31);
+}
+
+}  // namespace
+
+namespace attention {
+
+// Shared tiles for workgroups of 4 waves (16-bit queries), of one, or (0) a query to a workgroup: the
+// fastest of these by modelled times (us).  Measured, with picks half of which 64 neighbouring queries share (batch, key
+// heads, group, dim, rows, block, window, picks; then queries: one query / 4 waves / one wave):
+//   bf16  2,4,3,64,8192,64,128,8    256: 28 / 78 / 49    999: 79 / 90 / 63   2000: 149 / 112 / 110
+//                                  4000: 276 / 168 / 173
+//         1,2,8,128,8192,64,256,8   512: 25 / 100 / 53  2000: 74 / 110 / 65  4000: 132 / 126 / 135
+//         4,4,3,64,4096,64,128,8   4096: 504 / 166 / 211
+//         2,8,1,32,1024,16,32,8    1000: 39 / 27 / 25
+//         2,4,2,96,4096,16,100,8   1000: 53 / 79 / 63
+//         2,4,3,64,8192,8,64,8     1500: 30 / 137 / 124
+//   fp32  2,4,3,64,8192,64,128,8    999: 108 / 113 / 76  4000: 337 / 239 / 206
+//         1,2,8,128,8192,64,256,8   512: 35 / 104 / 56   4000: 172 / 206 / 150
+// One query: its keys' products.  Tiles: a chain of the union of a workgroup's keys, which grows with
+// about the root of its queries, while the workgroups find room on the chip.
+int quantized_tile_waves(const Params& p, int dtype) {
+  if (!fits(p)) return 0;
+  const bool is32 = dtype == RLM_F32;
+  const double keys = static_cast<double>(std::min<int64_t>(p.T, p.local_window + p.TOP * p.BS));
+  const double query = 8.0 + p.items * keys * (6e-6 + 1.2e-7 * p.D) * (is32 ? 1.4 : 1.0);
+  const int chunks = (p.G + kRows - 1) / kRows, heads = (p.G + chunks - 1) / chunks;
+  const double tile_keys = p.D <= 64 ? 64.0 : 32.0;
+  const double alone = std::min(p.T / tile_keys + 1.0,
+                                p.local_window / tile_keys + 1.0 + p.TOP * std::max(1.0, p.BS / tile_keys));
+  const double step = tile_keys * (0.009 + 2.3e-4 * p.D) * (is32 ? 1.2 : 1.0) *
+                      (p.BS % kMostKeys == 0 ? 1.0 : 1.5);
+  auto tiles = [&](int waves, double cost, double room) {
+    const int queries = waves * (kRows / heads);  // of a workgroup
+    const double steps =
+        std::min(p.T / tile_keys + 1.0, alone * (1.0 + 0.45 * std::sqrt(static_cast<double>(queries))));
+    const double groups =
+        static_cast<double>(p.B) * p.Hk * chunks * ((p.Tq + queries - 1) / queries);
+    return 5.0 + steps * step * cost * std::max(1.0, groups / room);
+  };
+  const double one = tiles(1, 1.0, 1400.0), four = is32 ? one : tiles(4, 1.35, 820.0);
+  if (query <= std::min(one, four)) return 0;
+  return one <= four ? 1 : 4;
+}
+
+hipError_t quantized_tile_launch(Params& p, int dtype, int waves, hipStream_t stream) {
+  TileParams tp{};
+  tp.p = p;
+  tp.negate = p.scale_log2 < 0.0f;
+  tp.far = p.T * std::max(p.k_st, p.v_st) >= (int64_t(1) << 31) - 4096;
+  // A scale of 0 as the smallest number: scores of 0 for the keys, -inf for the masked.
+  tp.c = std::max(std::fabs(p.scale_log2), 1e-37f);
+  const bool whole = p.BS % kMostKeys == 0;
+#define RLM_TILE_TYPE(T)                                \
+  return whole ? launch_type<T, true>(tp, waves, stream) \
+               : launch_type<T, false>(tp, waves, stream);
+  if (dtype == RLM_F32) RLM_TILE_TYPE(float)
+  if (dtype == RLM_BF16) RLM_TILE_TYPE(bf16)
+  RLM_TILE_TYPE(f16)
+#undef RLM_TILE_TYPE
+}
+
+}  // namespace attention
+}  // namespace rlm

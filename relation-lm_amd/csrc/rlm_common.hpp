@@ -170,6 +170,13 @@ __device__ __forceinline__ void lds_dma16(rsrc_t r, uint32_t lds_addr, uint32_t 
                : "v"(voff), "s"(r), "s"(soff), "{m0}"(lds_addr)
                : "memory");
 }
+// Four bytes per lane likewise: lane i's land at lds_addr + 4*i.
+__device__ __forceinline__ void lds_dma4(rsrc_t r, uint32_t lds_addr, uint32_t voff) {
+  asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds"
+               :
+               : "v"(voff), "s"(r), "{m0}"(lds_addr)
+               : "memory");
+}
 // s_waitcnt immediate that waits until at most n vector-memory operations of
 // this wave are outstanding (gfx9 encoding: vmcnt in bits 3:0 and 15:14),
 // leaving the export and LDS counters untouched.
