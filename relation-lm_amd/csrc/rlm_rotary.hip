@@ -21,6 +21,8 @@
 // Accesses are of 16 bytes where pairs, head dim, strides and addresses allow, else of one element: the
 // 4 x 4096 tokens with every token real, into caches, take 15.5 us in bf16 (26.5 in fp32), 37.2 (35.4) with
 // 31 pairs in place of 32 and 29.5 (28.5) from rows one element off; 8 single tokens 6.0 either way.
+#include <type_traits>
+
 #include "rlm_common.hpp"
 #include "rlm_fastdiv.hpp"
 
@@ -236,6 +238,37 @@ __device__ __forceinline__ void load8(const T* src, int count, float (&x)[8]) {
   }
 }
 
+// Eight features of a row whose L lanes each have eight: its scale, and these features' codes.
+template <int L>
+__device__ __forceinline__ float quantize8(const float (&x)[8], uint32_t (&codes)[2]) {
+  // The largest magnitude as bits: NaN above infinity above every number.
+  uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+  for (int off = 1; off < L; off <<= 1)
+    most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), off, kWave)));
+  const bool finite = most < 0x7f800000u;
+  // Not below the smallest normal number, whose reciprocal is finite.
+  const float least = fmaxf(__uint_as_float(most) / 448.0f, 1.17549435e-38f);
+  const float inv = 1.0f / least;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // x / s as the correctly rounded reciprocal and one correction give it: values that are
+      // few-bit fractions of the largest fall on or beside the codes' ties.
+      const float q = x[4 * w + e] * inv;
+      y[e] = fmaf(fmaf(-q, least, x[4 * w + e]), inv, q);
+    }
+    const int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    codes[w] = finite ? static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true))
+                      : 0u;
+  }
+  return !finite ? __uint_as_float(0x7fc00000u) : most == 0 ? 0.0f : least;
+}
+
 // Rotation with the key and value rows written as e4m3 codes and a scale each.  L lanes have a
 // row, eight features each, so that its largest magnitude is a few lane exchanges; a pair's
 // other half is read a second time (from L1) by the lane that has it not.
@@ -317,32 +350,8 @@ __global__ __launch_bounds__(kThreads) void rotary_quantize_kernel(RotaryParams 
       }
       continue;
     }
-    // The largest magnitude as bits: NaN above infinity above every number.
-    uint32_t most = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-    for (int off = 1; off < L; off <<= 1)
-      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), off, kWave)));
-    const bool finite = most < 0x7f800000u;
-    // Not below the smallest normal number, whose reciprocal is finite.
-    const float least = fmaxf(__uint_as_float(most) / 448.0f, 1.17549435e-38f);
-    const float inv = finite ? 1.0f / least : 0.0f;
-    const float scale = !finite ? __uint_as_float(0x7fc00000u) : most == 0 ? 0.0f : least;
     uint32_t codes[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // x / s as the correctly rounded reciprocal and one correction give it: values that are
-        // few-bit fractions of the largest fall on or beside the codes' ties.
-        const float q = x[4 * w + e] * inv;
-        y[e] = finite ? fmaf(fmaf(-q, least, x[4 * w + e]), inv, q) : 0.0f;
-      }
-      int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-      codes[w] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true));
-    }
+    const float scale = quantize8<L>(x, codes);
     uint8_t* dst = is_v ? static_cast<uint8_t*>(p.ov) + b * p.ov_sb + row * p.ov_st + h * p.ov_sh
                         : static_cast<uint8_t*>(p.ok) + b * p.ok_sb + row * p.ok_st + h * p.ok_sh;
     if constexpr (WIDE) {
@@ -360,10 +369,137 @@ __global__ __launch_bounds__(kThreads) void rotary_quantize_kernel(RotaryParams 
   }
 }
 
+// The same for workgroups of several tokens: a wave has one head of 64 / L tokens at a time, the next one's
+// rows on their way, so that what depends on the head is scalar and what depends on the token comes
+// from LDS.  A lane has both halves of four pairs (interleaved: four pairs), or eight features that do not
+// turn.  With every address from 64-bit products per row, as above, instructions bound it: 4 x 4096 tokens
+// of 12 + 4 + 4 heads of 64 take 16.1 us (84 MB, 5.2 TB/s) where they took 22.0.
+template <typename T, int L, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void rotary_quantize_tokens_kernel(RotaryParams p) {
+  __shared__ float2 turn[kMaxAngles];
+  __shared__ int64_t dest[kMaxTokens];
+  __shared__ int64_t from[3][kMaxTokens], to[2][kMaxTokens], scale_to[2][kMaxTokens];
+  const uint32_t first = blockIdx.x * static_cast<uint32_t>(p.per_group);
+  const uint32_t count = min(static_cast<uint32_t>(p.per_group), p.tokens - first);
+  if (threadIdx.x < count) {
+    uint32_t step;
+    const uint32_t b = p.by_queries.div(first + threadIdx.x, step);
+    from[0][threadIdx.x] = b * p.q_sb + step * p.q_st;
+    from[1][threadIdx.x] = b * p.k_sb + step * p.k_st;
+    from[2][threadIdx.x] = b * p.v_sb + step * p.v_st;
+  }
+  set_up(p, first, count, turn, dest);
+  if (threadIdx.x < count) {
+    const int64_t b = p.by_queries.div(first + threadIdx.x), row = dest[threadIdx.x];
+    to[0][threadIdx.x] = b * p.ok_sb + row * p.ok_st;
+    to[1][threadIdx.x] = b * p.ov_sb + row * p.ov_st;
+    scale_to[0][threadIdx.x] = b * p.ks_sb + row * p.ks_st;
+    scale_to[1][threadIdx.x] = b * p.vs_sb + row * p.vs_st;
+  }
+  __syncthreads();
+
+  constexpr int kTokens = kWave / L, kWaves = kThreads / kWave;
+  typedef typename std::conditional<sizeof(T) == 4, uint4, uint2>::type raw_t;  // four features
+  struct Four {
+    T e[4];
+  };
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x & (kWave - 1), part = lane % L;
+  const int D = p.D, F = p.F;
+  const bool inside = 8 * part < D;
+  const bool turns = INTERLEAVED ? 8 * part < 2 * F : 4 * part < F;
+  // A lane's first and second four features.
+  const int one = !INTERLEAVED && turns ? 4 * part : inside ? 8 * part : 0;
+  const int two = !INTERLEAVED && turns ? F + 4 * part : one + 4;
+  const int chunks = (count + kTokens - 1) / kTokens;
+  const int total = p.heads * chunks;  // (head, chunk of tokens), the waves' in turn
+  auto kind_of = [&](int head) { return head < p.Hq ? 0 : head < p.Hq + p.Hk ? 1 : 2; };
+  auto token_of = [&](int chunk) {
+    return min(chunk * kTokens + lane / L, static_cast<int>(count) - 1);
+  };
+  raw_t next[2];
+  auto fetch = [&](int head, int chunk) {
+    const int kind = kind_of(head);
+    const T* base = kind == 0   ? static_cast<const T*>(p.q) + head * p.q_sh
+                    : kind == 1 ? static_cast<const T*>(p.k) + (head - p.Hq) * p.k_sh
+                                : static_cast<const T*>(p.v) + (head - p.Hq - p.Hk) * p.v_sh;
+    const T* src = base + from[kind][token_of(chunk)];
+    next[0] = *reinterpret_cast<const raw_t*>(src + one);
+    next[1] = *reinterpret_cast<const raw_t*>(src + two);
+  };
+  int head = wave % p.heads, chunk = wave / p.heads;
+  auto advance = [&](int& h, int& c) {
+    h += kWaves;
+    while (h >= p.heads) {
+      h -= p.heads;
+      ++c;
+    }
+  };
+  if (wave < total) fetch(head, chunk);
+  for (int i = wave; i < total; i += kWaves) {
+    const Four low = __builtin_bit_cast(Four, next[0]), high = __builtin_bit_cast(Four, next[1]);
+    int next_head = head, next_chunk = chunk;
+    advance(next_head, next_chunk);
+    if (i + kWaves < total) fetch(next_head, next_chunk);
+    const int kind = kind_of(head);
+    const int token = token_of(chunk);
+    const bool here = inside && chunk * kTokens + lane / L < static_cast<int>(count);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = inside ? to_f32(low.e[e]) : 0.0f;
+      x[4 + e] = inside ? to_f32(high.e[e]) : 0.0f;
+    }
+    if (kind != 2 && turns) {
+      const float2* tr = turn + token * F + 4 * part;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 cs = tr[e];
+        float &a = INTERLEAVED ? x[2 * e] : x[e], &b = INTERLEAVED ? x[2 * e + 1] : x[4 + e];
+        const float a0 = a;
+        a = fmaf(a0, cs.x, -(b * cs.y));
+        b = fmaf(a0, cs.y, b * cs.x);
+      }
+    }
+    if (kind == 0) {
+      T* dst = static_cast<T*>(p.oq) + (static_cast<int64_t>(first + token) * p.Hq + head) * D;
+      if (here) {
+        put4<T>(dst + one, x[0], x[1], x[2], x[3]);
+        put4<T>(dst + two, x[4], x[5], x[6], x[7]);
+      }
+    } else {
+      uint32_t codes[2];
+      const float scale = quantize8<L>(x, codes);
+      const int h = kind == 1 ? head - p.Hq : head - p.Hq - p.Hk;
+      uint8_t* dst = (kind == 1 ? static_cast<uint8_t*>(p.ok) + h * p.ok_sh
+                                : static_cast<uint8_t*>(p.ov) + h * p.ov_sh) + to[kind - 1][token];
+      float* sc = (kind == 1 ? p.ks + h * p.ks_sh : p.vs + h * p.vs_sh) + scale_to[kind - 1][token];
+      if (here && dest[token] >= 0) {
+        *reinterpret_cast<uint32_t*>(dst + one) = codes[0];
+        *reinterpret_cast<uint32_t*>(dst + two) = codes[1];
+        if (part == 0) *sc = scale;
+      }
+    }
+    head = next_head;
+    chunk = next_chunk;
+  }
+}
+
 template <typename T, int L, bool WIDE>
 hipError_t launch_quantize(const RotaryParams& p, bool interleaved, hipStream_t stream) {
   const dim3 grid((p.tokens + p.per_group - 1) / p.per_group);
   RLM_TRY(check_launch("rotary_to_quantized_caches", grid.x, kThreads));
+  if constexpr (WIDE) {
+    if (p.per_group * L >= kWave) {
+      if (interleaved)
+        hipLaunchKernelGGL((rotary_quantize_tokens_kernel<T, L, true>), grid, dim3(kThreads), 0,
+                           stream, p);
+      else
+        hipLaunchKernelGGL((rotary_quantize_tokens_kernel<T, L, false>), grid, dim3(kThreads), 0,
+                           stream, p);
+      return launch_status("rotary_to_quantized_caches");
+    }
+  }
   if (interleaved)
     hipLaunchKernelGGL((rotary_quantize_kernel<T, L, WIDE, true>), grid, dim3(kThreads), 0, stream,
                        p);
@@ -539,6 +675,12 @@ hipError_t rotary_common(const rlm_tensor* query, const rlm_tensor* key, const r
                       wide_access(query, per_vec) && wide_access(key, per_vec) &&
                       wide_access(value, per_vec) && wide_access(out_query, per_vec) &&
                       wide_access(out_key, 8, 8) && wide_access(out_value, 8, 8);
+    const int row_lanes = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
+    const int together = kWave / row_lanes;
+    // Many tokens: as many to a workgroup as a wave has at a time.  Measured, the rule above / these (us,
+    // bf16; tokens of 12 + 4 + 4 heads of 64): 4096 8.6 / 8.7, 8192 14.9 / 10.6, 16384 20.1 / 16.1; of 32 + 8 + 8
+    // of 128: 2048 13.2 / 14.7, 4096 22.4 / 19.4, 8000 45.3 / 35.8.
+    if (wide && p.tokens / together >= 1024 && together * F <= kMaxAngles) p.per_group = together;
 #define RLM_QUANTIZE(T)                                                          \
   return wide ? launch_quantize_lanes<T, true>(p, lanes, interleaved != 0, stream) \
               : launch_quantize_lanes<T, false>(p, lanes, interleaved != 0, stream);
