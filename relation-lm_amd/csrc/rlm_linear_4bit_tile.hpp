@@ -25,6 +25,7 @@ __device__ __forceinline__ void barrier() {
 
 typedef const __attribute__((address_space(3))) s16x8* lds_frag;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) u32x4* lds_piece;
 typedef const __attribute__((address_space(3))) f32x4* lds_f32x4;
 typedef __attribute__((address_space(3))) float* lds_float;
@@ -34,8 +35,12 @@ template <int WK>
 constexpr int kChunks = WK == 1 ? 32 : 16;
 template <int WK>
 constexpr int kSumPitch = kChunks<WK> + 4;
-template <int WT, int WK>
-constexpr int kTileLds = WK * 64 * WT * (2 * 2 * kDeep + 4 * kSumPitch<WK>);
+// Bytes of a step's scales of one weight: C groups of ROWS rows, in whole loads of a wave.
+template <typename S, int C, int ROWS>
+constexpr int kScaleBytes = (C * ROWS * static_cast<int>(sizeof(S)) + 255) / 256 * 256;
+template <typename S, int G, int CH, int WR, int WT, int WK>
+constexpr int kTileLds = WK * (64 * WT * (2 * 2 * kDeep + 4 * kSumPitch<WK>) +
+                               2 * G * kScaleBytes<S, 4 / CH, WR * 64 / G>);
 
 // Eight 16-bit inputs at any address: those below K.
 template <typename T>
@@ -64,7 +69,11 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
   constexpr int kTokens = 64 * WT;               // of a workgroup
   constexpr int kStage = kTokens * kDeep * 2;    // bytes of inputs
   constexpr int NC = kChunks<WK>, kPitch = kSumPitch<WK>;
-  extern __shared__ __align__(1024) char lds[];  // [WK][2] stages, [WK] sums
+  constexpr int kRows = WR * 16 * R;              // of each weight
+  constexpr int kScales = kScaleBytes<S, C, kRows>;
+  typedef const __attribute__((address_space(3)))
+      typename std::conditional<sizeof(S) == 4, u32x4, u32x2>::type* lds_scales;
+  extern __shared__ __align__(1024) char lds[];  // [WK][2] stages, [WK] sums, [WK][2][G] scales
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, quad = lane >> 4;
@@ -90,9 +99,44 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
   const uint32_t row_bytes = static_cast<uint32_t>(p.x_s) * 2;
   // (Rows past the last are out of range and come as zeros.)
   const rsrc_t x_rows = make_rsrc(base, static_cast<uint32_t>(rows - 1) * row_bytes + 2u * p.K);
+  const int groups = (p.K + p.group - 1) / p.group;
+  auto group_of = [&](int chunk) {  // a chunk's group; past the last input, the last one
+    const int at = CH < 4 ? chunk : static_cast<int>(p.by_group_tiles.div(static_cast<uint32_t>(chunk)));
+    return min(at, groups - 1);
+  };
+  // Tiles of codes and scales by uniform offsets; rows past the last read others', and nobody keeps
+  // their outputs.
+  auto tile_of = [&](int i) { return min(nt0 + i, p.NT - 1); };
+  rsrc_t codes[G], scales[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    codes[g] = make_rsrc(p.codes[g], static_cast<uint32_t>(p.NT) * p.KT * 1024u);
+    scales[g] = make_rsrc(p.scales[g], static_cast<uint32_t>(groups) * p.N * sizeof(S));
+  }
+  // A step's scales: four bytes to a lane, groups after each other (rows past the last read others').
+  const uint32_t scales0 = lds0 + WK * (2 * kStage + kTokens * kPitch * 4) + kq * 2 * G * kScales;
+  auto issue_scales = [&](int i) {
+    constexpr int kEach = 4 / static_cast<int>(sizeof(S)), kUnits = kRows / kEach;  // of a group
+    constexpr int kLoads = kScales / 256;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int n = 0; n < (kLoads + WR * WT - 1) / (WR * WT); ++n) {
+        const int j = mate + n * WR * WT;
+        if (kLoads % (WR * WT) != 0 && j >= kLoads) break;
+        const int unit = j * kWave + lane, c = unit / kUnits;
+        const uint32_t at =
+            static_cast<uint32_t>(group_of(C * (kt0 + i) + (CH < 4 ? min(c, C - 1) : 0))) * p.N +
+            row_block * kRows + unit % kUnits * kEach;
+        lds_dma4(scales[g],
+                 __builtin_amdgcn_readfirstlane(scales0 + ((i & 1) * G + g) * kScales + j * 256),
+                 at * static_cast<uint32_t>(sizeof(S)));
+      }
+  };
   auto issue = [&](int i) {
     const int kt = kt0 + i;
     const uint32_t to = __builtin_amdgcn_readfirstlane(stages + (i & 1) * kStage);
+    if constexpr (ALIGNED) issue_scales(i);
 #pragma unroll
     for (int n = 0; n < kBring; ++n) {
       const int j = mate + n * WR * WT;
@@ -107,16 +151,6 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
       }
     }
   };
-  // Tiles of codes and scales by uniform offsets; rows past the last read others', and nobody keeps
-  // their outputs.
-  auto tile_of = [&](int i) { return min(nt0 + i, p.NT - 1); };
-  rsrc_t codes[G], scales[G];
-  const int groups = (p.K + p.group - 1) / p.group;
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    codes[g] = make_rsrc(p.codes[g], static_cast<uint32_t>(p.NT) * p.KT * 1024u);
-    scales[g] = make_rsrc(p.scales[g], static_cast<uint32_t>(groups) * p.N * sizeof(S));
-  }
   auto load_words = [&](int kt, uint4 (&w)[G][R]) {
 #pragma unroll
     for (int g = 0; g < G; ++g)
@@ -143,10 +177,6 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 
   // Sums kept, NC chunks of each token of this part.
   const uint32_t sums0 = lds0 + WK * 2 * kStage + (kq * kTokens + 64 * half) * kPitch * 4;
-  auto group_of = [&](int chunk) {  // a chunk's group; past the last input, the last one
-    const int at = CH < 4 ? chunk : static_cast<int>(p.by_group_tiles.div(static_cast<uint32_t>(chunk)));
-    return min(at, groups - 1);
-  };
   const uint32_t x_row = (64 * half + r) * 256 + ((quad ^ r) << 4);
 
   for (int n = 0; n < per; ++n) {
@@ -169,18 +199,20 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 #pragma unroll 1
       for (int c = 0; c < C; ++c) {
         const int chunk = C * kt + c;
-        const uint32_t line = static_cast<uint32_t>(group_of(chunk)) * p.N;
         Four<S, ALIGNED> scale[G][R];
+        if constexpr (!ALIGNED) {
+          const uint32_t line = static_cast<uint32_t>(group_of(chunk)) * p.N;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+          for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int i = 0; i < R; ++i) {
-            uint32_t lane_off[ALIGNED ? 1 : 4];
+            for (int i = 0; i < R; ++i) {
+              uint32_t lane_off[4];
 #pragma unroll
-            for (int e = 0; e < (ALIGNED ? 1 : 4); ++e)
-              lane_off[e] = min(4 * quad + e, p.N - (ALIGNED ? 4 : 1) - 16 * tile_of(i)) * sizeof(S);
-            scale[g][i].load(scales[g], lane_off, (line + 16 * tile_of(i)) * sizeof(S));
-          }
+              for (int e = 0; e < 4; ++e)
+                lane_off[e] = min(4 * quad + e, p.N - 1 - 16 * tile_of(i)) * sizeof(S);
+              scale[g][i].load(scales[g], lane_off, (line + 16 * tile_of(i)) * sizeof(S));
+            }
+        }
         f32x4 acc[G][R][4], sum[4 / WR];
 #pragma unroll
         for (int t = 0; t < 4 / WR; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -194,6 +226,13 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
         for (int s = 0; s < CH; ++s) {
           s16x8 x_next[4];
           inputs((c * CH + s + 1) & 3, x_next);
+          // The token tiles that this wave sums.
+          s16x8 mine[4 / WR];
+#pragma unroll
+          for (int t = 0; t < 4 / WR; ++t)
+            mine[t] = WR == 1 ? x[t]
+                              : *(lds_frag)static_cast<uintptr_t>((x_at ^ (64u * ((c * CH + s) & 3))) +
+                                                                  4096u * (t * WR + rq));
 #pragma unroll
           for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -202,10 +241,9 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 #pragma unroll
               for (int t = 0; t < 4; ++t) acc[g][i][t] = product(a, x[t], acc[g][i][t], T{});
             }
-          __builtin_amdgcn_sched_barrier(0);  // operands of one step and the next live at once
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (WR == 1 || rq == t % WR) sum[t / WR] = product(ones<T>(), x[t], sum[t / WR], T{});
+          for (int t = 0; t < 4 / WR; ++t) sum[t] = product(ones<T>(), mine[t], sum[t], T{});
+          __builtin_amdgcn_sched_barrier(0);  // operands of one step and the next live at once
 #pragma unroll
           for (int t = 0; t < 4; ++t) x[t] = x_next[t];
         }
@@ -214,6 +252,15 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
           for (int t = 0; t < 4 / WR; ++t)
             *(lds_float)static_cast<uintptr_t>(sums0 + ((16 * (t * WR + rq) + r) * kPitch +
                                                         (C * n + c) % NC) * 4) = sum[t][0];
+        }
+        if constexpr (ALIGNED) {
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+              scale[g][i].v = __builtin_bit_cast(decltype(scale[g][i].v), *(lds_scales)static_cast<uintptr_t>(
+                  scales0 + (n & 1) * G * kScales + g * kScales +
+                  (c * kRows + 16 * (rq * R + i) + 4 * quad) * static_cast<uint32_t>(sizeof(S))));
         }
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -341,7 +388,7 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED>
 hipError_t launch_tile(const LinearParams& p, hipStream_t stream) {
   const char* name = G == 2 ? "gated_linear_4bit" : "linear_4bit";
-  constexpr int kThreads = WR * WT * WK * kWave, kLds = kTileLds<WT, WK>;
+  constexpr int kThreads = WR * WT * WK * kWave, kLds = kTileLds<S, G, CH, WR, WT, WK>;
   static_assert(WK == 1 || kThreads * 256 <= WK * 2 * 64 * WT * kDeep * 2, "parts in the stages");
   const int64_t row_blocks = (p.NT + WR * 4 / G - 1) / (WR * 4 / G);
   const int64_t token_blocks = (p.M + 64 * WT - 1) / (64 * WT);
