@@ -363,27 +363,26 @@ bool tile_shape(const LinearParams& p, int dtype, int products, TileShape* shape
   // Modelled times (us).  Few tokens: the weights once for every 32.  Tiles: rounds of workgroups, steps of 128
   // inputs (two or four parts of them at once), a step's time by the group's size.  Measured (tokens, outputs,
   // width, group; few tokens / wide / middle / small):
-  //   plain  64,4096,4096,128: 20 / 76 / 62 / 23     333,2304,768,32: 20 / 30 / 17 / 15    ,128: 14 / 23 / 15 / 11
-  //          333,4096,4096,32: 110 / 132 / 66 / 83   ,64: 85 / 134 / 92 / 53               ,128: 82 / 79 / 64 / 45
-  //          1024,4096,4096,32: 324 / 132 / 86 / 166 ,64: 247 / 137 / 102 / 106            ,128: 241 / 80 / 72 / 88
-  //   gated  64,4096,4096,128: 24 / 79 / 43 / 25     333,2304,768,32: 33 / 32 / 19 / 31    ,128: 19 / 25 / 16 / 21
-  //          333,4096,4096,32: 153 / 133 / 88 / 128  ,64: 116 / 134 / 103 / 84             ,128: 105 / 82 / 55 / 70
-  //          1024,4096,4096,32: 445 / 141 / 174 / 337                                      ,128: 310 / 85 / 108 / 180
+  //   plain  64,4096,4096,128: 20 / 65 / 31 / 23     333,2304,768,32: 20 / 30 / 16 / 15    ,128: 14 / 22 / 12 / 11
+  //          333,4096,4096,32: 110 / 126 / 62 / 77   ,64: 85 / 88 / 45 / 53                ,128: 82 / 68 / 35 / 45
+  //          1024,4096,4096,32: 324 / 127 / 83 / 153 ,64: 247 / 90 / 60 / 106              ,128: 241 / 69 / 45 / 89
+  //          4096,4096,4096,32: 1288 / 258 / 316 / 610  ,64: 978 / 183 / 220 / 416         ,128:  - / 139 / 165 / 348
+  //   gated  64,4096,4096,128: 24 / 70 / 33 / 24     333,2304,768,32: 33 / 32 / 18 / 30    ,128: 19 / 24 / 14 / 21
+  //          333,4096,4096,32: 153 / 128 / 88 / 119  ,64: 116 / 92 / 63 / 84               ,128: 105 / 73 / 48 / 71
+  //          1024,4096,4096,32: 445 / 139 / 175 / 312   ,64:  - / 98 / 120 / 220           ,128: 310 / 76 / 92 / 181
   const int ch = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;
-  constexpr double kWideStep[] = {4.05, 4.1, 2.35}, kSmallStep[] = {4.8, 2.9, 2.5},
-                   kMiddleStep[] = {4.0, 5.5, 3.7}, kMiddleTwo[] = {5.15, 6.15, 4.3};
+  constexpr double kWideStep[] = {3.65, 2.43, 1.83}, kSmallStep[] = {4.0, 2.43, 2.05},
+                   kMiddleStep[] = {3.35, 2.25, 1.6}, kMiddleTwo[] = {4.85, 3.35, 2.4};
   auto rounds = [&](int tiles, int tokens, int resident) {
     const int64_t groups = (rows + tiles - 1) / tiles * ((p.M + tokens - 1) / tokens);
     return static_cast<double>((groups + resident - 1) / resident);
   };
-  const bool light = products == 2 && ch == 2;  // gated, whole tiles to a group
   const double few = 5.0 + (p.M + 31) / 32 * (static_cast<double>(rows) * p.KT * 2048.0) /
                                (products == 2 ? (ch == 0 ? 2.5e6 : 3.3e6) : (ch == 0 ? 1.75e6 : 2.35e6));
-  const double wide = 4.5 + rounds(16, 128, 256) * p.KT * kWideStep[ch];
-  const double middle = 4.5 + (p.KT + 1) / 2 *
-                                  std::min(rounds(8, 64, 256) * (light ? 3.3 : kMiddleStep[ch]),
-                                           rounds(8, 64, 512) * (light ? 3.3 : kMiddleTwo[ch]));
-  const double small = rounds(4, 64, 256) * (4.5 + (p.KT + 3) / 4 * kSmallStep[ch]);
+  const double wide = 9.0 + rounds(16, 128, 256) * p.KT * kWideStep[ch];
+  const double middle = 7.0 + (p.KT + 1) / 2 * std::min(rounds(8, 64, 256) * kMiddleStep[ch],
+                                                        rounds(8, 64, 512) * kMiddleTwo[ch]);
+  const double small = rounds(4, 64, 256) * (6.8 + (p.KT + 3) / 4 * kSmallStep[ch]);
   *shape = wide <= middle && wide <= small ? kWide : middle <= small ? kMiddle : kSmall;
   return few > std::min(wide, std::min(middle, small));
 }

@@ -243,7 +243,6 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
             }
 #pragma unroll
           for (int t = 0; t < 4 / WR; ++t) sum[t] = product(ones<T>(), mine[t], sum[t], T{});
-          __builtin_amdgcn_sched_barrier(0);  // operands of one step and the next live at once
 #pragma unroll
           for (int t = 0; t < 4; ++t) x[t] = x_next[t];
         }

@@ -14,12 +14,15 @@ from test_linear_4bit_gpu import U, check, host, on, product, weight
 
 pytestmark = pytest.mark.gpu
 
-SHAPES = {"wide": (4, 2, 1), "middle": (2, 1, 2), "small": (1, 1, 4)}   # waves: rows, tokens, parts
+# Waves along rows, tokens and parts of the inputs; whether inputs come by DMA.
+SHAPES = {"wide": (4, 2, 1, True), "middle": (2, 1, 2, True), "small": (1, 1, 4, True)}
 
 
 def instance(call):
-    """(waves' rows, tokens, parts, aligned) of the tile kernel that the call takes."""
+    """(waves' rows, tokens, parts, aligned) of the tile kernel that the call takes, or None."""
     names = launched(call)
+    if "linear_4bit_kernel" in names:
+        return None
     plain = re.search(r"linear_4bit_tile_kernel<.*, \d+, \d+, (\d+), (\d+), (\d+), (\w+)>", names)
     if plain:
         return int(plain[1]), int(plain[2]), int(plain[3]), plain[4] == "true"
@@ -30,12 +33,14 @@ def instance(call):
 
 PLAIN = [
     # tile, group, tokens, outputs, width
-    ("wide", 32, 2099, 2000, 304), ("wide", 64, 2099, 2000, 1104), ("wide", 128, 2099, 1000, 1104),
-    ("wide", 128, 2099, 2000, 2104), ("wide", 256, 701, 2000, 304), ("wide", 32, 2099, 2000, 1104),
+    ("wide", 32, 2099, 2000, 304), ("wide", 64, 2099, 2000, 1104), ("wide", 128, 2099, 2000, 1104),
+    ("wide", 128, 2099, 2000, 2104), ("wide", 256, 2099, 2000, 304), ("wide", 32, 2099, 2000, 1104),
     ("middle", 32, 701, 2000, 304), ("middle", 32, 2099, 504, 2104), ("middle", 64, 2099, 1000, 1104),
     ("middle", 128, 701, 2000, 1104), ("middle", 256, 2099, 1000, 2104),
-    ("small", 32, 299, 2000, 304), ("small", 32, 701, 1000, 1104), ("small", 64, 499, 1000, 2104),
-    ("small", 128, 201, 2000, 304), ("small", 256, 499, 1000, 1104), ("small", 64, 299, 2000, 1104),
+    ("middle", 128, 2099, 1000, 1104), ("middle", 256, 701, 2000, 304),
+    ("small", 32, 499, 2000, 304), ("small", 32, 701, 1000, 1104), ("small", 64, 499, 1000, 2104),
+    ("small", 128, 499, 2000, 304), ("small", 256, 701, 1000, 1104), ("small", 64, 299, 2000, 1104),
+    ("few", 32, 299, 2000, 304), ("few", 128, 201, 2000, 304), ("few", 256, 499, 1000, 1104),
 ]
 
 
@@ -55,14 +60,15 @@ def test_linear(device, shape, dtype):
         want, d = product(x, w, group)
         want = want + host(bias)
         check(got, want, d + U * (np.abs(want) + d), dtype)
-        assert instance(lambda: linear_4bit(*args)) == SHAPES[tile] + (True,)
+        assert instance(lambda: linear_4bit(*args)) == SHAPES.get(tile)
 
 
 GATED = [
     ("wide", 32, 2099, 1000, 304), ("wide", 64, 2099, 1000, 1104), ("wide", 128, 2099, 1000, 1104),
     ("middle", 32, 701, 1000, 1104), ("middle", 64, 701, 2000, 1104),
     ("middle", 128, 1499, 504, 1104), ("middle", 256, 499, 2000, 304),
-    ("small", 32, 201, 2000, 304), ("small", 64, 201, 2000, 1104), ("small", 128, 299, 1000, 2104),
+    ("small", 32, 499, 1000, 1104), ("small", 64, 201, 2000, 1104), ("small", 128, 299, 1000, 2104),
+    ("few", 32, 201, 2000, 304),
 ]
 
 
@@ -84,7 +90,7 @@ def test_gated_linear(device, shape, dtype):
         d_act = 1.13 * da + 8 * U * np.abs(act)
         d = d_act * (np.abs(b) + db) + np.abs(act) * db
         check(got, act * b, d + U * np.abs(act * b), dtype)
-        assert instance(lambda: gated_linear_4bit(*args)) == SHAPES[tile] + (True,)
+        assert instance(lambda: gated_linear_4bit(*args)) == SHAPES.get(tile)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -104,7 +110,7 @@ def test_any_alignment(device, group, dtype):
 def test_inputs_that_are_not_finite(device):
     """An infinity or NaN reaches its own token's outputs and no other's."""
     g = torch.Generator().manual_seed(9)
-    for tile, group, tokens, outputs, width in (PLAIN[0], PLAIN[6], PLAIN[11]):
+    for tile, group, tokens, outputs, width in (PLAIN[0], PLAIN[6], PLAIN[13]):
         x = torch.randn(tokens, width, generator=g).to(torch.bfloat16)
         w = on(device, weight(g, outputs, width, group, True, torch.bfloat16))
         plain = linear_4bit(x.to(device), *w, group)
