@@ -3,13 +3,20 @@
 //
 // A wave has 64 weight rows (gated: 32 of each weight) and 64 tokens, a workgroup WR by WT waves of them
 // for each of WK parts of the inputs.  Inputs come by DMA into LDS, 128 of each token at a time, the
-// next 128 on their way while these are worked on; codes come from memory straight into registers in
-// operand order.  Per group, total += s acc with acc = sum (16 + c) x; what the 16 and the zero point
+// next 128 on their way while these are worked on, and so do the step's scales; codes come from memory
+// straight into registers in operand order.  Per group, total += s acc with acc = sum (16 + c) x; what the 16 and the zero point
 // add,
 //   sum_g (16 + z_g) s_g X_g,   X_g = the group's sum of inputs,
 // is itself a product over groups: the waves that share tokens each sum some of them, with ones as the
 // other operand, and every 32 (or 16) groups (16 + z) s and X meet as sums of three bf16 parts (six
 // products, to 2^-24 of their size).  The parts of the inputs are added in LDS at the end, in order.
+//
+// Bound: instructions, and what a barrier a step leaves idle.  A wave's step of 64 rows, 64 tokens and 128
+// inputs has 67 products and about 220 other vector instructions (128 decode, 64 scale); each keeps its
+// unit busy 45% of the time and waits take 30%.  4096 tokens of 4096 -> 4096 take 140 us in groups of 128
+// (980 TFLOP/s; the vendor's bf16 product of 8192 reaches 1560), 183 of 64 and 257 of 32, whose sums
+// are scaled two and four times as often.  With the scales loaded in the step that uses them 161 / 276 /
+// 267.  Rows that are no whole accesses: 184 with 4095 outputs, 320 with 4095 inputs too.
 #pragma once
 
 #include "rlm_linear_4bit.hpp"
@@ -60,8 +67,8 @@ __device__ __forceinline__ u32x4 eight_inputs(const T* row, int k, int K) {
 }
 
 // G products; CH matrix instructions to a group (four also where a group is several tiles).  ALIGNED:
-// inputs by DMA, four scales at a time.
-template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED>
+// inputs by DMA; EVEN: scales by DMA.
+template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED, bool EVEN>
 __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bit_tile_kernel(LinearParams p,
                                                                                 FastDiv by_rows) {
   constexpr int R = 4 / G;                       // 16-row tiles of a wave, of each weight
@@ -133,10 +140,43 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
                  at * static_cast<uint32_t>(sizeof(S)));
       }
   };
+  // The same through registers, an element to a lane: loaded with the step's inputs, written behind the
+  // products of the step before.
+  constexpr int kMates = WR * WT * kWave, kOwn = EVEN ? 1 : (C * kRows + kMates - 1) / kMates;
+  typedef typename std::conditional<sizeof(S) == 4, uint32_t, uint16_t>::type one_t;
+  one_t own[G][kOwn];
+  auto load_scales = [&](int i) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int n = 0; n < kOwn; ++n) {
+        const int unit = mate * kWave + n * kMates + lane, c = min(unit / kRows, C - 1);
+        const uint32_t at = (static_cast<uint32_t>(group_of(C * (kt0 + i) + c)) * p.N +
+                             row_block * kRows + unit % kRows) * static_cast<uint32_t>(sizeof(S));
+        if constexpr (sizeof(S) == 4)
+          own[g][n] = __builtin_amdgcn_raw_buffer_load_b32(scales[g], at, 0, 0);
+        else
+          own[g][n] = __builtin_amdgcn_raw_buffer_load_b16(scales[g], at, 0, 0);
+      }
+  };
+  auto write_scales = [&](int i) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int n = 0; n < kOwn; ++n) {
+        const int unit = mate * kWave + n * kMates + lane;
+        if (C * kRows % kMates == 0 || unit < C * kRows)
+          *(__attribute__((address_space(3))) one_t*)static_cast<uintptr_t>(
+              scales0 + ((i & 1) * G + g) * kScales + unit * static_cast<uint32_t>(sizeof(S))) = own[g][n];
+      }
+  };
   auto issue = [&](int i) {
     const int kt = kt0 + i;
     const uint32_t to = __builtin_amdgcn_readfirstlane(stages + (i & 1) * kStage);
-    if constexpr (ALIGNED) issue_scales(i);
+    if constexpr (EVEN)
+      issue_scales(i);
+    else
+      load_scales(i);
 #pragma unroll
     for (int n = 0; n < kBring; ++n) {
       const int j = mate + n * WR * WT;
@@ -173,7 +213,10 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 
   uint4 words[G][R];
   load_words(min(kt0, p.KT - 1), words);
-  if (tiles > 0) issue(0);
+  if (tiles > 0) {
+    issue(0);
+    if (!EVEN) write_scales(0);
+  }
 
   // Sums kept, NC chunks of each token of this part.
   const uint32_t sums0 = lds0 + WK * 2 * kStage + (kq * kTokens + 64 * half) * kPitch * 4;
@@ -199,20 +242,7 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 #pragma unroll 1
       for (int c = 0; c < C; ++c) {
         const int chunk = C * kt + c;
-        Four<S, ALIGNED> scale[G][R];
-        if constexpr (!ALIGNED) {
-          const uint32_t line = static_cast<uint32_t>(group_of(chunk)) * p.N;
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-              uint32_t lane_off[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                lane_off[e] = min(4 * quad + e, p.N - 1 - 16 * tile_of(i)) * sizeof(S);
-              scale[g][i].load(scales[g], lane_off, (line + 16 * tile_of(i)) * sizeof(S));
-            }
-        }
+        Four<S, true> scale[G][R];
         f32x4 acc[G][R][4], sum[4 / WR];
 #pragma unroll
         for (int t = 0; t < 4 / WR; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -252,15 +282,15 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
             *(lds_float)static_cast<uintptr_t>(sums0 + ((16 * (t * WR + rq) + r) * kPitch +
                                                         (C * n + c) % NC) * 4) = sum[t][0];
         }
-        if constexpr (ALIGNED) {
 #pragma unroll
-          for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int i = 0; i < R; ++i)
-              scale[g][i].v = __builtin_bit_cast(decltype(scale[g][i].v), *(lds_scales)static_cast<uintptr_t>(
-                  scales0 + (n & 1) * G * kScales + g * kScales +
-                  (c * kRows + 16 * (rq * R + i) + 4 * quad) * static_cast<uint32_t>(sizeof(S))));
-        }
+          for (int i = 0; i < R; ++i)
+            scale[g][i].v = __builtin_bit_cast(
+                decltype(scale[g][i].v),
+                *(lds_scales)static_cast<uintptr_t>(
+                    scales0 + ((n & 1) * G + g) * kScales +
+                    (c * kRows + 16 * (rq * R + i) + 4 * quad) * static_cast<uint32_t>(sizeof(S))));
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -285,6 +315,7 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
       for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int i = 0; i < R; ++i) words[g][i] = next[g][i];
+      if (!EVEN && n + 1 < tiles) write_scales(n + 1);
     }
 
     // total -= ((16 + z) s) X over the kept chunks.
@@ -384,7 +415,7 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
   }
 }
 
-template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED>
+template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED, bool EVEN>
 hipError_t launch_tile(const LinearParams& p, hipStream_t stream) {
   const char* name = G == 2 ? "gated_linear_4bit" : "linear_4bit";
   constexpr int kThreads = WR * WT * WK * kWave, kLds = kTileLds<S, G, CH, WR, WT, WK>;
@@ -392,7 +423,7 @@ hipError_t launch_tile(const LinearParams& p, hipStream_t stream) {
   const int64_t row_blocks = (p.NT + WR * 4 / G - 1) / (WR * 4 / G);
   const int64_t token_blocks = (p.M + 64 * WT - 1) / (64 * WT);
   RLM_TRY(check_launch(name, row_blocks * token_blocks, kThreads));
-  const auto kernel = &linear_4bit_tile_kernel<T, S, G, CH, WR, WT, WK, ALIGNED>;
+  const auto kernel = &linear_4bit_tile_kernel<T, S, G, CH, WR, WT, WK, ALIGNED, EVEN>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   RLM_REQUIRE(e == hipSuccess, "%s: %d bytes of LDS refused: %s", name, kLds, hipGetErrorString(e));
@@ -403,10 +434,11 @@ hipError_t launch_tile(const LinearParams& p, hipStream_t stream) {
 
 template <typename T, typename S, int G, int CH>
 hipError_t launch_shape(const LinearParams& p, TileShape shape, hipStream_t stream) {
-  if (!p.wide_x || !p.wide_s) return launch_tile<T, S, G, CH, 2, 1, 2, false>(p, stream);
-  if (shape == kWide) return launch_tile<T, S, G, CH, 4, 2, 1, true>(p, stream);
-  if (shape == kMiddle) return launch_tile<T, S, G, CH, 2, 1, 2, true>(p, stream);
-  return launch_tile<T, S, G, CH, 1, 1, 4, true>(p, stream);
+  if (!p.wide_x) return launch_tile<T, S, G, CH, 2, 1, 2, false, false>(p, stream);
+  if (!p.wide_s) return launch_tile<T, S, G, CH, 2, 1, 2, true, false>(p, stream);
+  if (shape == kWide) return launch_tile<T, S, G, CH, 4, 2, 1, true, true>(p, stream);
+  if (shape == kMiddle) return launch_tile<T, S, G, CH, 2, 1, 2, true, true>(p, stream);
+  return launch_tile<T, S, G, CH, 1, 1, 4, true, true>(p, stream);
 }
 template <typename T, typename S, int G>
 hipError_t launch_group_tile(const LinearParams& p, TileShape shape, hipStream_t stream) {

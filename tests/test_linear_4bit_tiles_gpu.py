@@ -23,10 +23,10 @@ def instance(call):
     names = launched(call)
     if "linear_4bit_kernel" in names:
         return None
-    plain = re.search(r"linear_4bit_tile_kernel<.*, \d+, \d+, (\d+), (\d+), (\d+), (\w+)>", names)
+    plain = re.search(r"linear_4bit_tile_kernel<.*, \d+, \d+, (\d+), (\d+), (\d+), (\w+), \w+>", names)
     if plain:
         return int(plain[1]), int(plain[2]), int(plain[3]), plain[4] == "true"
-    mangled = re.search(r"linear_4bit_tile_kernel.*Li\d+ELi\d+ELi(\d+)ELi(\d+)ELi(\d+)ELb(\d)E", names)
+    mangled = re.search(r"linear_4bit_tile_kernel.*Li\d+ELi\d+ELi(\d+)ELi(\d+)ELi(\d+)ELb(\d)ELb\dE", names)
     assert mangled, names
     return tuple(int(mangled[i]) for i in (1, 2, 3)) + (mangled[4] == "1",)
 
@@ -120,3 +120,27 @@ def test_inputs_that_are_not_finite(device):
         others = torch.ones(tokens, dtype=torch.bool)
         others[17] = others[90] = False
         assert torch.equal(got[others.to(device)], plain[others.to(device)])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("scale_dtype", ["same", "fp32"])
+def test_odd_outputs(device, group, scale_dtype, dtype):
+    """Whole accesses of inputs, none of scales; plain and gated."""
+    print(f"odd outputs {group} {scale_dtype} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(group)
+    kind = torch.float32 if scale_dtype == "fp32" else dtype
+    x = torch.randn(301, 1104, generator=g).to(dtype)
+    gate, up = [weight(g, 777, 1104, group, True, kind) for _ in range(2)]
+    args = (x.to(device), *on(device, gate), group)
+    got = linear_4bit(*args)
+    torch.cuda.synchronize()
+    (a, da), (b, db) = product(x, gate, group), product(x, up, group)
+    check(got, a, da, dtype)
+    assert instance(lambda: linear_4bit(*args)) == (2, 1, 2, True)
+    (gc, gs, gz), (uc, us, uz) = on(device, gate), on(device, up)
+    got = gated_linear_4bit(x.to(device), gc, gs, uc, us, gz, uz, group, "silu")
+    torch.cuda.synchronize()
+    act = torch.nn.functional.silu(torch.from_numpy(a)).numpy()
+    d_act = 1.13 * da + 8 * U * np.abs(act)
+    check(got, act * b, d_act * (np.abs(b) + db) + np.abs(act) * db + U * np.abs(act * b), dtype)
