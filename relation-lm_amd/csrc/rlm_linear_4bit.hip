@@ -350,8 +350,8 @@ hipError_t launch_types(const LinearParams& p, int dtype, int scale_dtype, hipSt
 
 // Whether many tokens share tiles, and how.
 bool tile_shape(const LinearParams& p, int dtype, int products, TileShape* shape) {
-  // 16-bit inputs; a workgroup's tokens, the codes and the scales below 2 GiB each.
-  if (dtype == RLM_F32 || p.M <= 32 || p.x_s >= (int64_t(1) << 22) ||
+  // A workgroup's tokens, the codes and the scales below 2 GiB each.
+  if (p.M <= 32 || p.x_s >= (int64_t(1) << 21) ||
       static_cast<int64_t>(p.NT) * p.KT >= (int64_t(1) << 20) ||
       static_cast<int64_t>((p.K + p.group - 1) / p.group) * p.N >= (int64_t(1) << 28))
     return false;
@@ -370,6 +370,12 @@ bool tile_shape(const LinearParams& p, int dtype, int products, TileShape* shape
   //   gated  64,4096,4096,128: 24 / 70 / 33 / 24     333,2304,768,32: 33 / 32 / 18 / 30    ,128: 19 / 24 / 14 / 21
   //          333,4096,4096,32: 153 / 128 / 88 / 119  ,64: 116 / 92 / 63 / 84               ,128: 105 / 73 / 48 / 71
   //          1024,4096,4096,32: 445 / 139 / 175 / 312   ,64:  - / 98 / 120 / 220           ,128: 310 / 76 / 92 / 181
+  //   fp32   64,4096,4096,64: 45 / 211 / 89          333,2304,768,32: 43 / 57 / 28
+  //          333,4096,4096,32: 242 / 258 / 117       ,128: 226 / 207 / 80
+  //          1024,4096,4096,32: 712 / 265 / 232      ,64: 676 / 226 / 184                  ,128: 666 / 211 / 158
+  //          4096,4096,4096,32: 2840 / 540 / 954     ,64: 2720 / 466 / 754                 ,128: 2670 / 424 / 638
+  //          gated 333,2304,768,128: 48 / 48 / 24    1024,4096,4096,128: 775 / 210 / 313
+  const bool is32 = dtype == RLM_F32;
   const int ch = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;
   constexpr double kWideStep[] = {3.65, 2.43, 1.83}, kSmallStep[] = {4.0, 2.43, 2.05},
                    kMiddleStep[] = {3.35, 2.25, 1.6}, kMiddleTwo[] = {4.85, 3.35, 2.4};
@@ -377,12 +383,17 @@ bool tile_shape(const LinearParams& p, int dtype, int products, TileShape* shape
     const int64_t groups = (rows + tiles - 1) / tiles * ((p.M + tokens - 1) / tokens);
     return static_cast<double>((groups + resident - 1) / resident);
   };
-  const double few = 5.0 + (p.M + 31) / 32 * (static_cast<double>(rows) * p.KT * 2048.0) /
-                               (products == 2 ? (ch == 0 ? 2.5e6 : 3.3e6) : (ch == 0 ? 1.75e6 : 2.35e6));
-  const double wide = 9.0 + rounds(16, 128, 256) * p.KT * kWideStep[ch];
-  const double middle = 7.0 + (p.KT + 1) / 2 * std::min(rounds(8, 64, 256) * kMiddleStep[ch],
-                                                        rounds(8, 64, 512) * kMiddleTwo[ch]);
-  const double small = rounds(4, 64, 256) * (6.8 + (p.KT + 3) / 4 * kSmallStep[ch]);
+  const double rate = is32            ? (products == 2 ? 1.1e6 : 0.8e6)
+                      : products == 2 ? (ch == 0 ? 2.5e6 : 3.3e6)
+                                      : (ch == 0 ? 1.75e6 : 2.35e6);
+  const double few = 5.0 + (p.M + 31) / 32 * (static_cast<double>(rows) * p.KT * 2048.0) / rate;
+  constexpr double kWide32[] = {8.0, 6.9, 6.4}, kMiddle32[] = {7.0, 5.5, 4.7};
+  const double wide = 9.0 + rounds(16, 128, 256) * p.KT * (is32 ? kWide32 : kWideStep)[ch];
+  const double one = rounds(8, 64, 256) * (is32 ? kMiddle32 : kMiddleStep)[ch];
+  const double two = is32 ? one : rounds(8, 64, 512) * kMiddleTwo[ch];
+  const double middle = 7.0 + (p.KT + 1) / 2 * std::min(one, two);
+  const double small =
+      is32 ? middle : rounds(4, 64, 256) * (6.8 + (p.KT + 3) / 4 * kSmallStep[ch]);
   *shape = wide <= middle && wide <= small ? kWide : middle <= small ? kMiddle : kSmall;
   return few > std::min(wide, std::min(middle, small));
 }
@@ -472,9 +483,10 @@ hipError_t linear(const rlm_tensor* input, const Weight (&weights)[2], int count
   p.activation = activation;
   TileShape shape;
   if (tile_shape(p, input->dtype, count, &shape))
-    return input->dtype == RLM_BF16
-               ? tile_launch_bf16(p, shape, count, weights[0].scales->dtype, stream)
-               : tile_launch_f16(p, shape, count, weights[0].scales->dtype, stream);
+    return (input->dtype == RLM_BF16  ? tile_launch_bf16
+            : input->dtype == RLM_F16 ? tile_launch_f16
+                                      : tile_launch_f32)(p, shape, count, weights[0].scales->dtype,
+                                                         stream);
   return count == 2 ? launch_types<2>(p, input->dtype, weights[0].scales->dtype, stream)
                     : launch_types<1>(p, input->dtype, weights[0].scales->dtype, stream);
 }

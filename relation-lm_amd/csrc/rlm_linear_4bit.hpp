@@ -143,11 +143,13 @@ __device__ __forceinline__ void finish(const LinearParams& p, int token, int n,
 
 // Many tokens: tiles of tokens in LDS shared by the weight rows of a workgroup
 // (rlm_linear_4bit_tile.hpp), which has 256 rows and 128 tokens, 128 and 64 in two parts of the inputs,
-// or 64 and 64 in four parts.
+// or 64 and 64 in four parts (16-bit inputs).
 enum TileShape { kWide, kMiddle, kSmall };
 hipError_t tile_launch_bf16(const LinearParams& p, TileShape shape, int products, int scale_dtype,
                             hipStream_t stream);
 hipError_t tile_launch_f16(const LinearParams& p, TileShape shape, int products, int scale_dtype,
+                           hipStream_t stream);
+hipError_t tile_launch_f32(const LinearParams& p, TileShape shape, int products, int scale_dtype,
                            hipStream_t stream);
 
 }  // namespace linear4

@@ -1,5 +1,5 @@
 // Products with 4-bit weights for many tokens: x tiles in LDS shared by the weight rows of a workgroup.
-// (Instances: rlm_linear_4bit_bf16.hip, rlm_linear_4bit_f16.hip.)
+// (Instances: rlm_linear_4bit_bf16.hip, rlm_linear_4bit_f16.hip, rlm_linear_4bit_f32.hip.)
 //
 // A wave has 64 weight rows (gated: 32 of each weight) and 64 tokens, a workgroup WR by WT waves of them
 // for each of WK parts of the inputs.  Inputs come by DMA into LDS, 128 of each token at a time, the
@@ -17,6 +17,9 @@
 // (980 TFLOP/s; the vendor's bf16 product of 8192 reaches 1560), 183 of 64 and 257 of 32, whose sums
 // are scaled two and four times as often.  With the scales loaded in the step that uses them 161 / 276 /
 // 267.  Rows that are no whole accesses: 184 with 4095 outputs, 320 with 4095 inputs too.
+//
+// fp32 inputs are staged as they are and split into three bf16 parts as they are read (24 bits; three
+// products a part of codes): 420 us in groups of 128, 330 TFLOP/s, where the vendor's fp32 product does 150.
 #pragma once
 
 #include "rlm_linear_4bit.hpp"
@@ -45,22 +48,23 @@ constexpr int kSumPitch = kChunks<WK> + 4;
 // Bytes of a step's scales of one weight: C groups of ROWS rows, in whole loads of a wave.
 template <typename S, int C, int ROWS>
 constexpr int kScaleBytes = (C * ROWS * static_cast<int>(sizeof(S)) + 255) / 256 * 256;
-template <typename S, int G, int CH, int WR, int WT, int WK>
-constexpr int kTileLds = WK * (64 * WT * (2 * 2 * kDeep + 4 * kSumPitch<WK>) +
+template <typename T, typename S, int G, int CH, int WR, int WT, int WK>
+constexpr int kTileLds = WK * (64 * WT * (2 * static_cast<int>(sizeof(T)) * kDeep + 4 * kSumPitch<WK>) +
                                2 * G * kScaleBytes<S, 4 / CH, WR * 64 / G>);
 
-// Eight 16-bit inputs at any address: those below K.
+// Sixteen bytes of inputs at any address: those below K.
 template <typename T>
-__device__ __forceinline__ u32x4 eight_inputs(const T* row, int k, int K) {
+__device__ __forceinline__ u32x4 piece_of_inputs(const T* row, int k, int K) {
+  constexpr int kEach = 16 / static_cast<int>(sizeof(T));
   u32x4 v = {0, 0, 0, 0};
-  if (k + 8 <= K) {
+  if (k + kEach <= K) {
     __builtin_memcpy(&v, row + k, 16);
   } else {
     struct Raw {
-      T e[8];
+      T e[kEach];
     } raw;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw.e[i] = k + i < K ? row[k + i] : T{};
+    for (int i = 0; i < kEach; ++i) raw.e[i] = k + i < K ? row[k + i] : T{};
     v = __builtin_bit_cast(u32x4, raw);
   }
   return v;
@@ -69,12 +73,16 @@ __device__ __forceinline__ u32x4 eight_inputs(const T* row, int k, int K) {
 // G products; CH matrix instructions to a group (four also where a group is several tiles).  ALIGNED:
 // inputs by DMA; EVEN: scales by DMA.
 template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED, bool EVEN>
-__global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bit_tile_kernel(LinearParams p,
+__global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 || (sizeof(T) == 4 && WK == 2) ? 1 : 2) void linear_4bit_tile_kernel(LinearParams p,
                                                                                 FastDiv by_rows) {
   constexpr int R = 4 / G;                       // 16-row tiles of a wave, of each weight
   constexpr int C = 4 / CH;                      // groups of a tile of codes
   constexpr int kTokens = 64 * WT;               // of a workgroup
-  constexpr int kStage = kTokens * kDeep * 2;    // bytes of inputs
+  constexpr bool k32 = sizeof(T) == 4;
+  typedef matrix_t<T> M;                          // what the matrix unit multiplies
+  constexpr int kBytes = static_cast<int>(sizeof(T)) * kDeep;  // of a token's inputs
+  constexpr int kPieces = kBytes / 16;
+  constexpr int kStage = kTokens * kBytes;
   constexpr int NC = kChunks<WK>, kPitch = kSumPitch<WK>;
   constexpr int kRows = WR * 16 * R;              // of each weight
   constexpr int kScales = kScaleBytes<S, C, kRows>;
@@ -98,14 +106,15 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   const uint32_t stages = lds0 + kq * 2 * kStage;
-  // Rows of 16 pieces, swizzled so that a piece column spreads over all banks.  A wave brings four
-  // rows at a time: rows 4 j .. 4 j + 3 for j = mate, mate + WR WT, ...
-  constexpr int kBring = kTokens / 4 / (WR * WT);
+  // Rows of pieces of 16 bytes, swizzled so that a piece column spreads over all banks.  A wave brings four
+  // rows at a time (fp32: two): those of load j for j = mate, mate + WR WT, ...
+  constexpr int kTogether = kWave / kPieces;
+  constexpr int kBring = kTokens / kTogether / (WR * WT);
   const T* base = static_cast<const T*>(p.x) + static_cast<int64_t>(m0) * p.x_s;
   const int rows = min(kTokens, p.M - m0);
-  const uint32_t row_bytes = static_cast<uint32_t>(p.x_s) * 2;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.x_s) * sizeof(T);
   // (Rows past the last are out of range and come as zeros.)
-  const rsrc_t x_rows = make_rsrc(base, static_cast<uint32_t>(rows - 1) * row_bytes + 2u * p.K);
+  const rsrc_t x_rows = make_rsrc(base, static_cast<uint32_t>(rows - 1) * row_bytes + sizeof(T) * p.K);
   const int groups = (p.K + p.group - 1) / p.group;
   auto group_of = [&](int chunk) {  // a chunk's group; past the last input, the last one
     const int at = CH < 4 ? chunk : static_cast<int>(p.by_group_tiles.div(static_cast<uint32_t>(chunk)));
@@ -180,14 +189,14 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 #pragma unroll
     for (int n = 0; n < kBring; ++n) {
       const int j = mate + n * WR * WT;
-      const int k = kDeep * kt + 8 * ((lane & 15) ^ (lane >> 4) ^ (4 * (j & 3)));
+      const int at = kTogether * j + lane / kPieces;  // row
+      const int k = kDeep * kt + 16 / static_cast<int>(sizeof(T)) * (lane % kPieces ^ (at & 15));
       if constexpr (ALIGNED) {
-        const uint32_t off = static_cast<uint32_t>(4 * j + (lane >> 4)) * row_bytes + 2u * k;
+        const uint32_t off = static_cast<uint32_t>(at) * row_bytes + sizeof(T) * k;
         lds_dma16(x_rows, to + 1024u * j, kDeep * (kt + 1) <= p.K || k < p.K ? off : kNoOffset);
       } else {
-        const int row = min(4 * j + (lane >> 4), rows - 1);
         *(lds_piece)static_cast<uintptr_t>(to + 1024u * j + 16 * lane) =
-            eight_inputs(base + static_cast<int64_t>(row) * p.x_s, k, p.K);
+            piece_of_inputs(base + static_cast<int64_t>(min(at, rows - 1)) * p.x_s, k, p.K);
       }
     }
   };
@@ -220,7 +229,7 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 
   // Sums kept, NC chunks of each token of this part.
   const uint32_t sums0 = lds0 + WK * 2 * kStage + (kq * kTokens + 64 * half) * kPitch * 4;
-  const uint32_t x_row = (64 * half + r) * 256 + ((quad ^ r) << 4);
+  const uint32_t x_row = (64 * half + r) * kBytes + (((k32 ? 2 * quad : quad) ^ r) << 4);
 
   for (int n = 0; n < per; ++n) {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
@@ -236,8 +245,16 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
         for (int t = 0; t < 4; ++t)
           x[t] = *(lds_frag)static_cast<uintptr_t>((x_at ^ (64u * s)) + 4096u * t);
       };
+      // Eight fp32 inputs of token tile t.
+      auto eight = [&](int s, int t, float (&v)[8]) {
+        const uint32_t at = (x_at ^ (128u * s)) + 8192u * t;
+        const f32x4 lo = *(lds_f32x4)static_cast<uintptr_t>(at);
+        const f32x4 hi = *(lds_f32x4)static_cast<uintptr_t>(at ^ 16u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < 4 ? lo[e] : hi[e - 4];
+      };
       s16x8 x[4];
-      inputs(0, x);
+      if constexpr (!k32) inputs(0, x);
       // (A loop where it has several rounds: unrolled, it spills.)
 #pragma unroll 1
       for (int c = 0; c < C; ++c) {
@@ -252,29 +269,64 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
           for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int t = 0; t < 4; ++t) acc[g][i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (k32) {
+          float alone[4 / WR] = {};
 #pragma unroll
-        for (int s = 0; s < CH; ++s) {
-          s16x8 x_next[4];
-          inputs((c * CH + s + 1) & 3, x_next);
-          // The token tiles that this wave sums.
-          s16x8 mine[4 / WR];
+          for (int s = 0; s < CH; ++s) {
+            const int at = (c * CH + s) & 3;
+            s16x8 a[G][R];
 #pragma unroll
-          for (int t = 0; t < 4 / WR; ++t)
-            mine[t] = WR == 1 ? x[t]
-                              : *(lds_frag)static_cast<uintptr_t>((x_at ^ (64u * ((c * CH + s) & 3))) +
-                                                                  4096u * (t * WR + rq));
+            for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int g = 0; g < G; ++g)
+              for (int i = 0; i < R; ++i) a[g][i] = decode<M>(word_of(words[g][i], s));
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-              const s16x8 a = decode<T>(word_of(words[g][i], s));
+            for (int t = 0; t < 4; ++t) {
+              float v[8];
+              eight(at, t, v);
+              s16x8 parts[3];
+              attention::split<3>(v, parts);
 #pragma unroll
-              for (int t = 0; t < 4; ++t) acc[g][i][t] = product(a, x[t], acc[g][i][t], T{});
+              for (int n = 2; n >= 0; --n)
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                  for (int i = 0; i < R; ++i) acc[g][i][t] = product(a[g][i], parts[n], acc[g][i][t], M{});
             }
+            // The token tiles that this wave sums.
 #pragma unroll
-          for (int t = 0; t < 4 / WR; ++t) sum[t] = product(ones<T>(), mine[t], sum[t], T{});
+            for (int t = 0; t < 4 / WR; ++t) {
+              float v[8];
+              eight(at, t * WR + (WR == 1 ? 0 : rq), v);
+              alone[t] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            }
+          }
 #pragma unroll
-          for (int t = 0; t < 4; ++t) x[t] = x_next[t];
+          for (int t = 0; t < 4 / WR; ++t) sum[t][0] = attention::rows_sum(alone[t]);
+        } else {
+#pragma unroll
+          for (int s = 0; s < CH; ++s) {
+            s16x8 x_next[4];
+            inputs((c * CH + s + 1) & 3, x_next);
+            // The token tiles that this wave sums.
+            s16x8 mine[4 / WR];
+#pragma unroll
+            for (int t = 0; t < 4 / WR; ++t)
+              mine[t] = WR == 1 ? x[t]
+                                : *(lds_frag)static_cast<uintptr_t>((x_at ^ (64u * ((c * CH + s) & 3))) +
+                                                                    4096u * (t * WR + rq));
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+              for (int i = 0; i < R; ++i) {
+                const s16x8 a = decode<M>(word_of(words[g][i], s));
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[g][i][t] = product(a, x[t], acc[g][i][t], T{});
+              }
+#pragma unroll
+            for (int t = 0; t < 4 / WR; ++t) sum[t] = product(ones<T>(), mine[t], sum[t], T{});
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[t] = x_next[t];
+          }
         }
         if (quad == 0) {
 #pragma unroll
@@ -352,7 +404,7 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
           float z = 8.0f;
           if (p.zeros[g] != nullptr) z = to_f32(static_cast<const S*>(p.zeros[g])[at]);
           v[e] = kept + 8 * quad + e < end
-                     ? (kBase<T> + z) * to_f32(static_cast<const S*>(p.scales[g])[at]) : 0.0f;
+                     ? (kBase<M> + z) * to_f32(static_cast<const S*>(p.scales[g])[at]) : 0.0f;
         }
         s16x8 cs[3];
         attention::split<3>(v, cs);
@@ -418,8 +470,8 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 ? 1 : 2) void linear_4bi
 template <typename T, typename S, int G, int CH, int WR, int WT, int WK, bool ALIGNED, bool EVEN>
 hipError_t launch_tile(const LinearParams& p, hipStream_t stream) {
   const char* name = G == 2 ? "gated_linear_4bit" : "linear_4bit";
-  constexpr int kThreads = WR * WT * WK * kWave, kLds = kTileLds<S, G, CH, WR, WT, WK>;
-  static_assert(WK == 1 || kThreads * 256 <= WK * 2 * 64 * WT * kDeep * 2, "parts in the stages");
+  constexpr int kThreads = WR * WT * WK * kWave, kLds = kTileLds<T, S, G, CH, WR, WT, WK>;
+  static_assert(WK == 1 || kThreads * 256 <= WK * 2 * 64 * WT * kDeep * static_cast<int>(sizeof(T)), "parts in the stages");
   const int64_t row_blocks = (p.NT + WR * 4 / G - 1) / (WR * 4 / G);
   const int64_t token_blocks = (p.M + 64 * WT - 1) / (64 * WT);
   RLM_TRY(check_launch(name, row_blocks * token_blocks, kThreads));
@@ -437,8 +489,9 @@ hipError_t launch_shape(const LinearParams& p, TileShape shape, hipStream_t stre
   if (!p.wide_x) return launch_tile<T, S, G, CH, 2, 1, 2, false, false>(p, stream);
   if (!p.wide_s) return launch_tile<T, S, G, CH, 2, 1, 2, true, false>(p, stream);
   if (shape == kWide) return launch_tile<T, S, G, CH, 4, 2, 1, true, true>(p, stream);
-  if (shape == kMiddle) return launch_tile<T, S, G, CH, 2, 1, 2, true, true>(p, stream);
-  return launch_tile<T, S, G, CH, 1, 1, 4, true, true>(p, stream);
+  if constexpr (sizeof(T) == 2)  // (four parts of fp32 inputs do not fit)
+    if (shape == kSmall) return launch_tile<T, S, G, CH, 1, 1, 4, true, true>(p, stream);
+  return launch_tile<T, S, G, CH, 2, 1, 2, true, true>(p, stream);
 }
 template <typename T, typename S, int G>
 hipError_t launch_group_tile(const LinearParams& p, TileShape shape, hipStream_t stream) {
@@ -449,11 +502,12 @@ hipError_t launch_group_tile(const LinearParams& p, TileShape shape, hipStream_t
 template <typename T>
 hipError_t launch_tile_type(const LinearParams& p, TileShape shape, int products, int scale_dtype,
                             hipStream_t stream) {
-  if (products == 2)
-    return scale_dtype == RLM_F32 ? launch_group_tile<T, float, 2>(p, shape, stream)
-                                  : launch_group_tile<T, T, 2>(p, shape, stream);
-  return scale_dtype == RLM_F32 ? launch_group_tile<T, float, 1>(p, shape, stream)
-                                : launch_group_tile<T, T, 1>(p, shape, stream);
+  if constexpr (sizeof(T) == 2)
+    if (scale_dtype != RLM_F32)
+      return products == 2 ? launch_group_tile<T, T, 2>(p, shape, stream)
+                           : launch_group_tile<T, T, 1>(p, shape, stream);
+  return products == 2 ? launch_group_tile<T, float, 2>(p, shape, stream)
+                       : launch_group_tile<T, float, 1>(p, shape, stream);
 }
 
 }  // namespace linear4

@@ -144,3 +144,38 @@ def test_odd_outputs(device, group, scale_dtype, dtype):
     act = torch.nn.functional.silu(torch.from_numpy(a)).numpy()
     d_act = 1.13 * da + 8 * U * np.abs(act)
     check(got, act * b, d_act * (np.abs(b) + db) + np.abs(act) * db + U * np.abs(act * b), dtype)
+
+
+FP32 = [
+    # tile, group, tokens, outputs, width
+    ("wide", 32, 2099, 2000, 304), ("wide", 64, 2099, 2000, 1104), ("wide", 256, 2099, 2000, 304),
+    ("middle", 32, 1299, 1000, 1104), ("middle", 64, 1299, 1000, 304), ("middle", 128, 701, 1000, 1104),
+    ("middle", 384, 299, 2000, 1104), ("odd outputs", 32, 301, 777, 1104),
+    ("odd outputs", 64, 301, 1777, 1104), ("odd outputs", 128, 301, 777, 1104),
+    ("odd", 32, 301, 777, 1001), ("odd", 64, 301, 777, 1001), ("odd", 128, 301, 777, 1001),
+    ("few", 64, 65, 1000, 304),
+]
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("shape", FP32, ids=str)
+def test_fp32(device, shape, zeros):
+    tile, group, tokens, outputs, width = shape
+    print(f"fp32 tiles {shape} {zeros}", flush=True)
+    g = torch.Generator().manual_seed(sum(shape[1:]))
+    x = torch.randn(tokens, width, generator=g)
+    gate, up = [weight(g, outputs, width, group, zeros, torch.float32) for _ in range(2)]
+    args = (x.to(device), *on(device, gate), group)
+    got = linear_4bit(*args)
+    torch.cuda.synchronize()
+    (a, da), (b, db) = product(x, gate, group), product(x, up, group)
+    check(got, a, da, torch.float32)
+    expected = {"odd outputs": (2, 1, 2, True), "odd": (2, 1, 2, False), **SHAPES}.get(tile)
+    assert instance(lambda: linear_4bit(*args)) == expected
+    (gc, gs, gz), (uc, us, uz) = on(device, gate), on(device, up)
+    got = gated_linear_4bit(x.to(device), gc, gs, uc, us, gz, uz, group, "silu")
+    torch.cuda.synchronize()
+    act = torch.nn.functional.silu(torch.from_numpy(a)).numpy()
+    d_act = 1.13 * da + 8 * U * np.abs(act)
+    check(got, act * b, d_act * (np.abs(b) + db) + np.abs(act) * db + U * np.abs(act * b),
+          torch.float32)
