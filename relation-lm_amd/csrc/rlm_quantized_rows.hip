@@ -1,7 +1,9 @@
 // Rows of an 8-bit cache read back in a float type: out[b, i, h] = cache[b, row, h] * scale[b, row, h],
 // row = rows[b, i] or i.
 //
-// Bound: memory, 1 + 4 / D bytes read and the type's written for each feature.
+// Bound: memory, 1 + 4 / D bytes read and the type's written for each feature: 4 x 16384 rows of 4 heads
+// of 128 features in bf16 (102 MB, which the MALL holds) take 16.4 us, 6.2 TB/s; 8 x 640 named rows of 3
+// of 64 take 4.1, a launch and two round trips.
 #include "rlm_common.hpp"
 #include "rlm_fastdiv.hpp"
 
