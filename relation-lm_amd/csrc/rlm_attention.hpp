@@ -55,8 +55,8 @@ __device__ __forceinline__ float rows_sum(float v) { return swap32_sum(swap16_su
 hipError_t query_launch(const Params& p, int dtype, hipStream_t stream);
 // The same over caches of 8 bits (rlm_attention_quantized.hip).
 hipError_t quantized_launch(const Params& p, int dtype, hipStream_t stream);
-// And shared tiles over them (rlm_attention_quantized_tile.hip), for workgroups of so many waves (0: the
-// kernel above is the faster one).
+// And shared tiles over them (rlm_attention_quantized_tile.hip), for workgroups of so many waves (two:
+// of one's rows; 0: the kernel above is the faster one).
 int quantized_tile_waves(const Params& p, int dtype);
 hipError_t quantized_tile_launch(Params& p, int dtype, int waves, hipStream_t stream);
 // Key tiles shared by the rows of a workgroup (rlm_attention_tile.hip).

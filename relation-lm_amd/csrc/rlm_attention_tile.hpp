@@ -160,13 +160,18 @@ constexpr int tile_bytes() {
 }
 
 // KV: the caches' elements, T or 8-bit codes.  DC: head dim in 32s, WHOLE: a tile lies within one
-// block; tiles of kKeys keys for kWaves waves, two of them in LDS.
-template <typename T, typename KV, int DC, bool WHOLE, int kKeys, int kWaves>
-__global__ __launch_bounds__(kWaves* kWave,
-                             DC <= 4 && !(__is_same(KV, code8) && sizeof(T) == 4 && DC > 1) ? 4 : 2) void
+// block; tiles of kKeys keys for kWaves waves, two of them in LDS.  kShares: waves that share out the
+// tiles of one wave's rows, two tiles of each in LDS, and add up at the end.
+template <typename T, typename KV, int DC, bool WHOLE, int kKeys, int kWaves, int kShares>
+__global__ __launch_bounds__(kWaves* kShares* kWave,
+                             kShares > 1 ? (DC <= 4 ? 3 : 2)
+                             : DC <= 4 && !(__is_same(KV, code8) && sizeof(T) == 4 && DC > 1) ? 4
+                                                                                            : 2) void
 attend_tile_kernel(TileParams tp) {
   constexpr bool kCodes = __is_same(KV, code8);
-  constexpr int kThreads = kWaves * kWave;
+  static_assert(kShares == 1 || kWaves == 1, "shares of one wave's tiles");
+  constexpr int kThreads = kWaves * kShares * kWave;       // of which as many bring a tile:
+  constexpr int kBringers = kWaves * kWave;
   constexpr int KT = kKeys / 16;                           // 16-key groups of a tile
   constexpr bool k32 = sizeof(T) == 4 && !kCodes;
   constexpr int kPitch = tile_pitch<T, KV, DC>();          // 16-byte pieces of an LDS row
@@ -174,7 +179,7 @@ attend_tile_kernel(TileParams tp) {
   constexpr int kTile = kKeys * kRow;                      // bytes of a key (or value) tile
   constexpr int kBuffer = tile_bytes<T, KV, DC, kKeys>();  // of both, codes: and 2 x 64 scales
   constexpr int kPieces = kPitch * kKeys;
-  constexpr int kDma = (kPieces + kThreads - 1) / kThreads;  // DMA instructions of a wave per tile
+  constexpr int kDma = (kPieces + kBringers - 1) / kBringers;  // DMA instructions of a wave per tile
   constexpr int DT = 2 * DC;                               // head dim in 16s
   constexpr int NP = kCodes ? kParts<T> : 1, NW = kCodes ? kWeightParts<T> : 1;
   typedef typename std::conditional<kCodes, bf16, T>::type M;  // what the matrix unit multiplies
@@ -188,7 +193,8 @@ attend_tile_kernel(TileParams tp) {
 
   const Params& p = tp.p;
   const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wave = kWaves == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int share = kShares == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, quad = lane >> 4;
   // The longest sequences' ends first; a (batch row, key head)'s workgroups stay on one XCD
   // (or a few) where their number and the XCDs' divide each other.
@@ -286,7 +292,8 @@ attend_tile_kernel(TileParams tp) {
 
   // This lane's pieces of a tile: row and byte in the row, which the swizzle permutes; pieces
   // past the head dim come as zeros.
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const uint32_t lds0 =
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + share * 2 * kBuffer;
   const uint32_t k_bytes = static_cast<uint32_t>(p.k_st * sizeof(KV));
   const uint32_t v_bytes = static_cast<uint32_t>(p.v_st * sizeof(KV));
   uint32_t k_off[kDma], v_off[kDma];
@@ -316,7 +323,7 @@ attend_tile_kernel(TileParams tp) {
                    __builtin_amdgcn_readfirstlane(at + 256),
                    static_cast<uint32_t>(key) * static_cast<uint32_t>(4 * p.vs_st));
       }
-      if (kPieces < kThreads && wave * kWave >= kPieces) return;  // a tile of fewer pieces than threads
+      if (kPieces < kBringers && wave * kWave >= kPieces) return;  // a tile of fewer pieces than threads
     }
     // Rows past the last that a query of the workgroup sees (their keys are masked, and they may
     // hold anything) read that one.
@@ -379,7 +386,7 @@ attend_tile_kernel(TileParams tp) {
       }
     }
     __syncthreads();
-    if (wave == 0) {
+    if (wave == 0 && share == 0) {
       int count = 0;
       for (int i = 0; i < window_tiles; i += kWave) {
         const int t = i + lane;
@@ -397,16 +404,19 @@ attend_tile_kernel(TileParams tp) {
       if (lane == 0) s_count = count;
     }
     __syncthreads();
-    const int count = __builtin_amdgcn_readfirstlane(s_count);
-    if (count == 0) continue;
+    const int listed = __builtin_amdgcn_readfirstlane(s_count);
+    if (listed == 0) continue;
+    // This share's entries: share, share + kShares, ...
+    const int count = (listed - share + kShares - 1) / kShares;
+    auto entry_of = [&](int i) { return list[min(share + kShares * i, listed - 1)]; };
     // Lane i holds the list's entry i of the current 64, and what the wave's queries see of it.
     const int word = wave / 2;
     const uint32_t own = 0xffffu << (16 * (wave & 1));
-    int entry = list[min(lane, count - 1)];
+    int entry = entry_of(lane);
     uint32_t seen = act[entry * kWords + word] & own;
     auto tile_of = [&](int i) {
       if ((i & (kWave - 1)) == 0 && i != 0) {
-        entry = list[min(i + lane, count - 1)];
+        entry = entry_of(i + lane);
         seen = act[entry * kWords + word] & own;
       }
       return __builtin_amdgcn_readlane(entry, i & (kWave - 1));
@@ -414,12 +424,16 @@ attend_tile_kernel(TileParams tp) {
     // Tile n of the list is in LDS half n mod 2; the next one is on its way while it is worked on.
     int next = tile_of(0);
     uint32_t next_see = __builtin_amdgcn_readlane(seen, 0);
-    issue(0, w0 + kKeys * next);
+    if (count > 0) issue(0, w0 + kKeys * next);
     for (int n = 0; n < count; ++n) {
       const int t = next;
       const uint32_t see = next_see;
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-      barrier();  // tile n is in LDS for every wave, tile n - 1 has been read by every wave
+      // Tile n is in LDS for every wave that reads it, tile n - 1 has been read by them.
+      if constexpr (kWaves == 1)
+        wave_sync();
+      else
+        barrier();
       if (n + 1 < count) {
         next = tile_of(n + 1);
         next_see = __builtin_amdgcn_readlane(seen, (n + 1) & (kWave - 1));
@@ -610,7 +624,29 @@ attend_tile_kernel(TileParams tp) {
     __syncthreads();  // the lists and tiles have been read
   }
 
-  const float total = rows_sum(l);
+  float total = rows_sum(l);
+  if constexpr (kShares > 1) {
+    // The shares' sums, in the shares' order (the tiles have been read).
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);                                    // [share][DT][64]
+    float2* stats = reinterpret_cast<float2*>(sums + (kShares - 1) * DT * kWave);  // [share][64]
+    if (share > 0) {
+#pragma unroll
+      for (int j = 0; j < DT; ++j) sums[((share - 1) * DT + j) * kWave + lane] = acc[j];
+      stats[(share - 1) * kWave + lane] = make_float2(m, total);
+    }
+    __syncthreads();
+    if (share > 0) return;
+    for (int other = 0; other + 1 < kShares; ++other) {
+      const float2 of = stats[other * kWave + lane];
+      const float top = fmaxf(m, of.x), base = top == -INFINITY ? 0.0f : top;
+      const float mine = __builtin_amdgcn_exp2f(m - base), theirs = __builtin_amdgcn_exp2f(of.x - base);
+      m = top;
+      total = total * mine + of.y * theirs;
+#pragma unroll
+      for (int j = 0; j < DT; ++j)
+        acc[j] = acc[j] * mine + sums[(other * DT + j) * kWave + lane] * theirs;
+    }
+  }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   bool fine = fabsf(total) < INFINITY;
 #pragma unroll
@@ -642,7 +678,7 @@ attend_tile_kernel(TileParams tp) {
   }
 }
 
-template <typename T, typename KV, int DC, bool WHOLE, int kKeys, int kWaves>
+template <typename T, typename KV, int DC, bool WHOLE, int kKeys, int kWaves, int kShares = 1>
 hipError_t launch_tiles(TileParams& tp, hipStream_t stream) {
   const char* name = __is_same(KV, code8) ? "routed_attention_quantized" : "routed_attention";
   const Params& p = tp.p;
@@ -653,7 +689,7 @@ hipError_t launch_tiles(TileParams& tp, hipStream_t stream) {
   tp.pairs = static_cast<uint32_t>(p.B * p.Hk * tp.chunks);
   tp.tiles = (static_cast<uint32_t>(p.Tq) + kWaves * tp.nqw - 1) / (kWaves * tp.nqw);
   RLM_TRY(check_launch(name, static_cast<int64_t>(tp.pairs) * tp.tiles,
-                       kWaves * kWave));
+                       kWaves * kShares * kWave));
   tp.by_pairs = FastDiv(tp.pairs);
   tp.by_chunks = FastDiv(static_cast<uint32_t>(tp.chunks));
   tp.by_kv = FastDiv(static_cast<uint32_t>(p.Hk));
@@ -661,15 +697,15 @@ hipError_t launch_tiles(TileParams& tp, hipStream_t stream) {
   tp.by_picks = FastDiv(static_cast<uint32_t>(p.TOP + 1));
   tp.by_wave_queries = FastDiv(static_cast<uint32_t>(tp.nqw));
   tp.by_block = FastDiv(static_cast<uint32_t>(p.BS));
-  const size_t lds = 2 * tile_bytes<T, KV, DC, kKeys>();  // two tiles of keys and values
+  const size_t lds = 2 * kShares * tile_bytes<T, KV, DC, kKeys>();  // two tiles of a share
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(&attend_tile_kernel<T, KV, DC, WHOLE, kKeys, kWaves>),
+        reinterpret_cast<const void*>(&attend_tile_kernel<T, KV, DC, WHOLE, kKeys, kWaves, kShares>),
         hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     RLM_REQUIRE(e == hipSuccess, "%s: %zu bytes of LDS refused: %s", name, lds, hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((attend_tile_kernel<T, KV, DC, WHOLE, kKeys, kWaves>),
-                     dim3(tp.pairs * tp.tiles), dim3(kWaves * kWave), lds, stream, tp);
+  hipLaunchKernelGGL((attend_tile_kernel<T, KV, DC, WHOLE, kKeys, kWaves, kShares>),
+                     dim3(tp.pairs * tp.tiles), dim3(kWaves * kShares * kWave), lds, stream, tp);
   return launch_status(name);
 }
 

@@ -19,20 +19,20 @@ DIMS = [32, 48, 64, 80, 96, 128, 256, 16, 112, 160]
 
 
 def instance(device, parts, block, window=WINDOW):
-    """(head dim in 32s, whole, keys of a tile, waves) of the kernel that the call takes."""
+    """(head dim in 32s, whole, keys of a tile, waves, shares) of the tile kernel that the call takes."""
     names = launched(lambda: raw_seq(device, parts, block, window))
-    plain = re.search(r"attend_tile_kernel<.*code8, (\d+), (\w+), (\d+), (\d+)>", names)
+    plain = re.search(r"attend_tile_kernel<.*code8, (\d+), (\w+), (\d+), (\d+), (\d+)>", names)
     if plain:
-        return int(plain[1]), plain[2] == "true", int(plain[3]), int(plain[4])
-    mangled = re.search(r"attend_tile_kernel.*code8ELi(\d+)ELb(\d)ELi(\d+)ELi(\d+)E", names)
+        return int(plain[1]), plain[2] == "true", int(plain[3]), int(plain[4]), int(plain[5])
+    mangled = re.search(r"attend_tile_kernel.*code8ELi(\d+)ELb(\d)ELi(\d+)ELi(\d+)ELi(\d+)E", names)
     assert mangled, names
-    return int(mangled[1]), mangled[2] == "1", int(mangled[3]), int(mangled[4])
+    return int(mangled[1]), mangled[2] == "1", int(mangled[3]), int(mangled[4]), int(mangled[5])
 
 
-def expected_instance(dim, block, waves):
+def expected_instance(dim, block, waves, shares):
     dc = -(-dim // 32)
     dc = dc if dc <= 4 else 8
-    return dc, block % 64 == 0, 64 if dc <= 2 else 32, waves
+    return dc, block % 64 == 0, 64 if dc <= 2 else 32, waves, shares
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -43,8 +43,11 @@ def test_many_queries(device, dim, block, dtype):
     g = torch.Generator().manual_seed(dim + block)
     parts = case(g, 2, 700, 32, 4, dim, ROWS, block, 2, 1, dtype)
     run_seq(device, parts, block, WINDOW)
-    waves = 1 if dtype == torch.float32 else 4
-    assert instance(device, parts, block) == expected_instance(dim, block, waves)
+    if dtype != torch.float32:
+        assert instance(device, parts, block) == expected_instance(dim, block, 4, 1)
+    elif (dim, block) != (64, 4):        # (a query to a workgroup)
+        shares = 2 if dim <= 64 else 1
+        assert instance(device, parts, block) == expected_instance(dim, block, 1, shares)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -54,10 +57,23 @@ def test_fewer_queries(device, dim, block, dtype):
     g = torch.Generator().manual_seed(dim + block)
     parts = case(g, 2, 301, 32, 4, dim, ROWS, block, 2, 1, dtype)
     run_seq(device, parts, block, WINDOW)
-    assert instance(device, parts, block) == expected_instance(dim, block, 1)
+    shares = 2 if dim <= 64 else 1
+    assert instance(device, parts, block) == expected_instance(dim, block, 1, shares)
 
 
-SHARED = [(301, 64), (700, 64), (700, 20)]    # queries, block: one wave, four, four in parts
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim, block", [(d, 64) for d in DIMS] + [(32, 4), (64, 48), (96, 12), (128, 48),
+                                                                  (160, 20)])
+def test_few_queries(device, dim, block, dtype):
+    print(f"few queries dim {dim} block {block} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(dim + block)
+    parts = case(g, 2, 199, 32, 4, dim, ROWS, block, 2, 1, dtype)
+    run_seq(device, parts, block, WINDOW)
+    assert dim == 160 or instance(device, parts, block) == expected_instance(dim, block, 1, 2)
+
+
+# queries, block: two waves that share out tiles, four waves of 16-bit queries
+SHARED = [(301, 64), (301, 20), (700, 64), (700, 20)]
 
 
 @pytest.mark.parametrize("what", ["codes", "scale nan", "scale inf"])
