@@ -72,6 +72,24 @@ __device__ __forceinline__ s16x8 decode(uint32_t w) {
   return __builtin_bit_cast(s16x8, make_uint4(o[0], o[1], o[2], o[3]));
 }
 
+// Eight codes as c - 8 in bf16, in the order 0 4 1 5 2 6 3 7.  e4m3 below 2^-5 is n 2^-9 for its low four bits
+// n: a code's byte 0x80 + (8 - c) or c - 8 is the difference in sign and magnitude, which one conversion a
+// pair makes bf16.  17 instructions; through fp32, as above, 28.
+__device__ __forceinline__ s16x8 decode_less_8(uint32_t w) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  bf16x2 o[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t c = (h == 0 ? w : w >> 4) & 0x0f0f0f0fu;
+    const uint32_t low = 0x88888888u - c;  // of c <= 8, which its bytes' signs say
+    const uint32_t is_low = __builtin_amdgcn_perm(low << 8, low, 0x090b080au);
+    const uint32_t code = (low & is_low) | (c & 0x07070707u & ~is_low);
+    o[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code, 512.0f, false);
+    o[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code, 512.0f, true);
+  }
+  return __builtin_bit_cast(s16x8, o);
+}
+
 // Ones as an operand.
 template <typename T>
 __device__ __forceinline__ s16x8 ones() {

@@ -19,7 +19,9 @@
 // 267.  Rows that are no whole accesses: 184 with 4095 outputs, 320 with 4095 inputs too.
 //
 // fp32 inputs are staged as they are and split into three bf16 parts as they are read (24 bits; three
-// products a part of codes): 420 us in groups of 128, 330 TFLOP/s, where the vendor's fp32 product does 150.
+// products a part of codes), and codes meet them as c - 8, so that only z - 8 is taken back: 438 us in groups of
+// 128, 314 TFLOP/s, where the vendor's fp32 product does 150.  (Codes as 16 + c: 419, and errors 50 times
+// those of the vendor's product; decoding is 36 instructions a 32 inputs more.)
 #pragma once
 
 #include "rlm_linear_4bit.hpp"
@@ -278,13 +280,14 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 || (sizeof(T) == 4 && WK
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
-              for (int i = 0; i < R; ++i) a[g][i] = decode<M>(word_of(words[g][i], s));
+              for (int i = 0; i < R; ++i) a[g][i] = decode_less_8(word_of(words[g][i], s));
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
               float v[8];
               eight(at, t, v);
+              float paired[8] = {v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};  // as the codes
               s16x8 parts[3];
-              attention::split<3>(v, parts);
+              attention::split<3>(paired, parts);
 #pragma unroll
               for (int n = 2; n >= 0; --n)
 #pragma unroll
@@ -404,7 +407,7 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 || (sizeof(T) == 4 && WK
           float z = 8.0f;
           if (p.zeros[g] != nullptr) z = to_f32(static_cast<const S*>(p.zeros[g])[at]);
           v[e] = kept + 8 * quad + e < end
-                     ? (kBase<M> + z) * to_f32(static_cast<const S*>(p.scales[g])[at]) : 0.0f;
+                     ? (kBase<T> + z) * to_f32(static_cast<const S*>(p.scales[g])[at]) : 0.0f;
         }
         s16x8 cs[3];
         attention::split<3>(v, cs);
