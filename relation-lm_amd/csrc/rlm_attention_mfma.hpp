@@ -92,6 +92,12 @@ __device__ __forceinline__ float code_to_f32(code8 c) {
   return __builtin_amdgcn_cvt_f32_fp8(c.bits, 0);
 }
 
+// A row's scale, NaN where it is not finite: an infinite one would give a score of -inf or +inf by the sign of
+// the codes' product, and so drop its row or not.
+__device__ __forceinline__ float scale_or_nan(float s) {
+  return __builtin_fabsf(s) < INFINITY ? s : __builtin_nanf("");
+}
+
 // Parts of a query, and of the weights that meet the values.
 template <typename T>
 constexpr int kParts = sizeof(T) == 4 ? 3 : __is_same(T, f16) ? 2 : 1;

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(MAXW* kWave) void attend_codes_kernel(Params p) {
           0, 0);
     }
     *(__attribute__((address_space(3))) float*)static_cast<uintptr_t>(mine + kValues + 4 * lane) =
-        scale;
+        scale_or_nan(scale);
     wave_sync();
 
     float x[8], top = -INFINITY;

@@ -121,8 +121,9 @@ __device__ void attend_row_alone(const Params& p, int64_t b, int64_t step, int64
         if (d < p.D) s = fmaf(qf[i], feature_of(kbase + at * p.k_st, d), s);
       }
       if constexpr (__is_same(KV, code8)) {
-        s = wave_sum_f32(s) * (p.ks[b * p.ks_sb + at * p.ks_st + hk * p.ks_sh] * scale_log2);
-        const float vs = p.vs[b * p.vs_sb + at * p.vs_st + hk * p.vs_sh];
+        s = wave_sum_f32(s) *
+            (scale_or_nan(p.ks[b * p.ks_sb + at * p.ks_st + hk * p.ks_sh]) * scale_log2);
+        const float vs = scale_or_nan(p.vs[b * p.vs_sb + at * p.vs_st + hk * p.vs_sh]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] *= vs;
       } else {
@@ -287,6 +288,7 @@ attend_tile_kernel(TileParams tp) {
 
   f32x4 acc[DT];
   float m = -INFINITY, l = 0.0f;
+  uint64_t odd = 0;  // codes: whether a key's scale was not finite (a score of -inf leaves no trace in the sums)
 #pragma unroll
   for (int j = 0; j < DT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
@@ -458,6 +460,11 @@ attend_tile_kernel(TileParams tp) {
         pick[kt] = row_ok & (((who >> bit) & 1) != 0);
       }
 
+      if constexpr (kCodes) {  // a lane a key
+        const float ks = *(lds_f32)static_cast<uintptr_t>(tile0 + 2 * kTile + 4 * lane);
+        odd |= __builtin_amdgcn_ballot_w64(!(fabsf(ks) < INFINITY));
+      }
+
       // S^T = K Q^T.
       f32x4 s[KT];
 #pragma unroll
@@ -625,6 +632,7 @@ attend_tile_kernel(TileParams tp) {
   }
 
   float total = rows_sum(l);
+  if (odd != 0) total = __builtin_nanf("");
   if constexpr (kShares > 1) {
     // The shares' sums, in the shares' order (the tiles have been read).
     f32x4* sums = reinterpret_cast<f32x4*>(lds);                                    // [share][DT][64]

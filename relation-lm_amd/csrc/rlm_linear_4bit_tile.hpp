@@ -20,8 +20,8 @@
 //
 // fp32 inputs are staged as they are and split into three bf16 parts as they are read (24 bits; three
 // products a part of codes), and codes meet them as c - 8, so that only z - 8 is taken back: 438 us in groups of
-// 128, 314 TFLOP/s, where the vendor's fp32 product does 150.  (Codes as 16 + c: 419, and errors 50 times
-// those of the vendor's product; decoding is 36 instructions a 32 inputs more.)
+// 128, 314 TFLOP/s, where the vendor's fp32 product does 150.  (Codes as 16 + c: 419, and errors 42 times as
+// large with 304 inputs of one sign; decoding takes 36 instructions more to 32 inputs.)
 #pragma once
 
 #include "rlm_linear_4bit.hpp"
