@@ -85,14 +85,17 @@ constexpr int64_t staged_pitch(int KT) {
 // while these are worked on.  STAGED: the tokens' inputs are put into LDS first (one token tile),
 // else they come with the codes.  WIDE: whole accesses (of inputs: where they are not staged).
 template <typename T, typename S, int MT, int R, int G, int CH, int U, bool WIDE, bool STAGED>
-__global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearParams p) {
+__global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearParams p,
+                                                                         FastDiv by_rows) {
   constexpr int NP = kParts<T>, C = 4 / CH;
   extern __shared__ __align__(16) char lds[];  // inputs; later [wave][G][R][MT][64] f32x4
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int W = blockDim.x / kWave;
   const int r = lane & 15, quad = lane >> 4;
-  const int m0 = blockIdx.y * 16 * MT;
+  // (Token blocks in a grid's y would end at 65535.)
+  uint32_t row_block;
+  const int m0 = static_cast<int>(by_rows.div(blockIdx.x, row_block)) * 16 * MT;
 
   struct Batch {
     uint4 words[U][G][R];
@@ -106,7 +109,7 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void linear_4bit_kernel(LinearPar
   const bool zeros = p.zeros[0] != nullptr;
   // Codes and scales by uniform offsets.  Rows past the last read others', and nobody keeps their
   // outputs.
-  const int nt0 = static_cast<int>(blockIdx.x) * R;
+  const int nt0 = static_cast<int>(row_block) * R;
   const int first = min(nt0, p.NT - R);  // R <= NT; the last workgroup may begin in the one before
   rsrc_t codes[G], scales[G], zero_points[G];
   const int groups = (p.K + p.group - 1) / p.group;
@@ -299,9 +302,8 @@ hipError_t launch(const LinearParams& p, hipStream_t stream) {
   const char* name = G == 2 ? "gated_linear_4bit" : "linear_4bit";
   int waves = 1;
   while (waves < kMaxWaves && waves < p.KT) waves *= 2;
-  const dim3 grid((p.NT + R - 1) / R, (p.M + 16 * MT - 1) / (16 * MT));
-  RLM_REQUIRE(grid.y < 65536u, "%s: too many tokens for one call", name);
-  RLM_TRY(check_launch(name, static_cast<int64_t>(grid.x) * grid.y, kWave * waves));
+  const int64_t row_blocks = (p.NT + R - 1) / R, token_blocks = (p.M + 16 * MT - 1) / (16 * MT);
+  RLM_TRY(check_launch(name, row_blocks * token_blocks, kWave * waves));
   size_t bytes = static_cast<size_t>(waves) * G * R * MT * kWave * 16;
   if (STAGED) bytes = std::max<size_t>(bytes, std::min(p.M, 16) * staged_pitch<T>(p.KT));
   if (bytes > 48 * 1024) {
@@ -311,8 +313,9 @@ hipError_t launch(const LinearParams& p, hipStream_t stream) {
     RLM_REQUIRE(e == hipSuccess, "%s: %zu bytes of LDS refused: %s", name, bytes,
                 hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((linear_4bit_kernel<T, S, MT, R, G, CH, U, WIDE, STAGED>), grid,
-                     dim3(kWave * waves), bytes, stream, p);
+  hipLaunchKernelGGL((linear_4bit_kernel<T, S, MT, R, G, CH, U, WIDE, STAGED>),
+                     dim3(static_cast<unsigned>(row_blocks * token_blocks)), dim3(kWave * waves),
+                     bytes, stream, p, FastDiv(static_cast<uint32_t>(row_blocks)));
   return launch_status(name);
 }
 
