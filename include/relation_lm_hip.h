@@ -827,7 +827,7 @@ hipError_t rlm_rotary_to_quantized_caches(
     const rlm_tensor* out_query, hipStream_t stream);
 
 /*
- * Rows of an 8-bit cache in a float type: out [B,N,Hk,D] = cache * scale, rounded once.
+ * Rows of an 8-bit cache in a float type: out [B,N,Hk,D] = cache * scale, an fp32 product rounded to it.
  * cache [B,T,Hk,D] RLM_F8E4M3 and scale [B,T,Hk] f32 of any strides; rows [B,N] int32/int64
  * names cache rows in any order (those outside [0, T) give zeros), or NULL for all of them
  * (N == T).
@@ -907,7 +907,9 @@ hipError_t rlm_routed_attention_quantized(
  * hold anything.  scales and zeros [ceil(K/group_size), N] share a float dtype; zeros NULL
  * means 8; bias [N] of any float dtype or NULL.  group_size 32, 64 or a multiple of 128.
  * input row-strided, of any float dtype, as out (dense).  Products are summed in fp32:
- * codes are exact in 16 bits, fp32 inputs enter as three bf16 parts.
+ * codes are exact in 16 bits, fp32 inputs enter as three bf16 parts.  With inputs of 16 bits a
+ * group's sums hold up to 31 times its inputs (fp32 inputs: 8 times), and inputs of which these pass
+ * fp32 give NaN, as those that are not finite do.
  */
 hipError_t rlm_linear_4bit(const rlm_tensor* input, const rlm_tensor* codes,
                            const rlm_tensor* scales, const rlm_tensor* zeros,

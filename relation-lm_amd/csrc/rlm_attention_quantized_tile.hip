@@ -4,11 +4,16 @@
 // keys are decoded as they are read from LDS, values by transposing 8-bit reads.  A query is a sum of bf16
 // parts, the weights times their values' scales likewise (rlm_attention_quantized.hip says which).
 //
-// Bound: instructions.  A wave spends about 400 on 64 keys of 64 features, 64 of them on decoding and 48 on
+// A wave spends about 400 vector instructions on 64 keys of 64 features, 64 of them on decoding and 48 on
 // splitting the weights, for 24 products; a third of the weights are of keys that a row did not pick.
-// 2 x 999 queries of 12 heads on 4 of 64 features (a window of 128, eight of up to 128 blocks of 64)
-// take 58 to 60 us, a query to a workgroup 79; 4 x 4096 take 167 us and 8000 of 16 on 2 of 128 (256, eight)
-// 189, where caches of 16 bits, with nothing to decode, take 110 and 124.
+//
+// Bound, many queries: these instructions.  4 x 4096 queries of 12 heads on 4 of 64 features (a window of
+// 128, eight blocks of 64) take 167 to 172 us, in 69% of whose clocks vector instructions issue (matrix cores busy
+// 20%), and 8000 of 16 on 2 of 128 (256, eight) 189 to 195; caches of 16 bits, with nothing to decode, take 110
+// and 124.  Fewer: rounds of workgroups.  2 x 999 of the first kind, late in 8192 rows, are 1600 workgroups of
+// two waves with 38 KB of LDS each, four to a CU: 6.25 to a CU are two rounds of about 26 us, 62 to 64 us with what
+// surrounds them (a query to a workgroup 79).  Vector instructions issue in 35% of the clocks and matrix cores are
+// busy in 10; 37% of the waves' life is waits for tiles and lists, 17% for their turn to issue.
 #include "rlm_attention_tile.hpp"
 
 namespace rlm {
@@ -18,7 +23,8 @@ namespace {
 // against 63 us, and with 64 where 32 are: 189 against 64 (2 x 999 queries of 12 heads on 4 of 64 and of
 // 16 on 2 of 128 features).  A third and fourth tile under way bring nothing: what a wave does with a
 // tile, about 400 instructions to 64 keys, hides the loads of the next.
-// Two waves: the rows of one, whose tiles they share out.
+// Two waves: the rows of one, whose tiles they share out.  One wave is never asked for up to 64 features
+// (quantized_tile_waves), which is why it has no tiles of 64 keys.
 template <typename T, bool WHOLE, int kWaves>
 hipError_t launch_waves(TileParams& tp, hipStream_t stream) {
   constexpr int kRowWaves = kWaves == 2 ? 1 : kWaves, kShares = kWaves == 2 ? 2 : 1;
@@ -101,6 +107,7 @@ hipError_t quantized_tile_launch(Params& p, int dtype, int waves, hipStream_t st
   tp.far = p.T * std::max(p.k_st, p.v_st) >= (int64_t(1) << 31) - 4096;
   // A scale of 0 as the smallest number: scores of 0 for the keys, -inf for the masked.
   tp.c = std::max(std::fabs(p.scale_log2), 1e-37f);
+  // (Instances of 32-key tiles would hold blocks that are multiples of 32 as whole ones.)
   const bool whole = p.BS % kMostKeys == 0;
 #define RLM_TILE_TYPE(T)                                \
   return whole ? launch_type<T, true>(tp, waves, stream) \

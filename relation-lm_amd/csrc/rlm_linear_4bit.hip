@@ -360,7 +360,8 @@ hipError_t launch_types(const LinearParams& p, int dtype, int scale_dtype, hipSt
 
 // Whether many tokens share tiles, and how.
 bool tile_shape(const LinearParams& p, int dtype, int products, TileShape* shape) {
-  // A workgroup's tokens, the codes and the scales below 2 GiB each.
+  // 32-bit offsets: a workgroup's tokens, the codes and the scales below 1 GiB each.  (Larger weights take the
+  // kernel for few tokens, which reads them once for every 32.)
   if (p.M <= 32 || p.x_s >= (int64_t(1) << 21) ||
       static_cast<int64_t>(p.NT) * p.KT >= (int64_t(1) << 20) ||
       static_cast<int64_t>((p.K + p.group - 1) / p.group) * p.N >= (int64_t(1) << 28))
@@ -385,6 +386,8 @@ bool tile_shape(const LinearParams& p, int dtype, int products, TileShape* shape
   //          1024,4096,4096,32: 712 / 265 / 232      ,64: 676 / 226 / 184                  ,128: 666 / 211 / 158
   //          4096,4096,4096,32: 2840 / 540 / 954     ,64: 2720 / 466 / 754                 ,128: 2670 / 424 / 638
   //          gated 333,2304,768,128: 48 / 48 / 24    1024,4096,4096,128: 775 / 210 / 313
+  // (fp32 tiles with codes as 16 + c.  As c - 8 both shapes take 2 to 10% longer -- wide, 4096 tokens: 552, 493,
+  // 437; middle, 1024: 237, 192, 168 -- which leaves the choice as it is.)
   const bool is32 = dtype == RLM_F32;
   const int ch = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;
   constexpr double kWideStep[] = {3.65, 2.43, 1.83}, kSmallStep[] = {4.0, 2.43, 2.05},

@@ -12,8 +12,8 @@
 // products, to 2^-24 of their size).  The parts of the inputs are added in LDS at the end, in order.
 //
 // Bound: instructions, and what a barrier a step leaves idle.  A wave's step of 64 rows, 64 tokens and 128
-// inputs has 67 products and about 220 other vector instructions (128 decode, 64 scale); each keeps its
-// unit busy 45% of the time and waits take 30%.  4096 tokens of 4096 -> 4096 take 140 us in groups of 128
+// inputs has 71 products (64 of weights, 4 of input sums, 3 of what is taken back) and about 220 other vector
+// instructions (128 decode, 64 scale); each keeps its unit busy 45% of the time and waits take 30%.  4096 tokens of 4096 -> 4096 take 140 us in groups of 128
 // (980 TFLOP/s; the vendor's bf16 product of 8192 reaches 1560), 183 of 64 and 257 of 32, whose sums
 // are scaled two and four times as often.  With the scales loaded in the step that uses them 161 / 276 /
 // 267.  Rows that are no whole accesses: 184 with 4095 outputs, 320 with 4095 inputs too.
@@ -260,7 +260,6 @@ __global__ __launch_bounds__(WR* WT* WK* kWave, WK == 4 || (sizeof(T) == 4 && WK
       // (A loop where it has several rounds: unrolled, it spills.)
 #pragma unroll 1
       for (int c = 0; c < C; ++c) {
-        const int chunk = C * kt + c;
         Four<S, true> scale[G][R];
         f32x4 acc[G][R][4], sum[4 / WR];
 #pragma unroll

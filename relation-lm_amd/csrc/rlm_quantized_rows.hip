@@ -1,5 +1,6 @@
 // Rows of an 8-bit cache read back in a float type: out[b, i, h] = cache[b, row, h] * scale[b, row, h],
-// row = rows[b, i] or i.
+// row = rows[b, i] or i.  The product is rounded to fp32 and then to the type: a code of 4 bits times a scale
+// of 24 may pass fp32, and where that first rounding lands on a 16-bit tie (1 of 2^16) it may be the other neighbour.
 //
 // Bound: memory, 1 + 4 / D bytes read and the type's written for each feature: 4 x 16384 rows of 4 heads
 // of 128 features in bf16 (102 MB, which the MALL holds) take 16.4 us, 6.2 TB/s; 8 x 640 named rows of 3

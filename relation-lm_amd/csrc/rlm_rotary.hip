@@ -375,7 +375,8 @@ __global__ __launch_bounds__(kThreads) void rotary_quantize_kernel(RotaryParams 
 // rows on their way, so that what depends on the head is scalar and what depends on the token comes
 // from LDS.  A lane has both halves of four pairs (interleaved: four pairs), or eight features that do not
 // turn.  With every address from 64-bit products per row, as above, instructions bound it: 4 x 4096 tokens
-// of 12 + 4 + 4 heads of 64 take 16.1 us (84 MB, 5.2 TB/s) where they took 22.0.
+// of 12 + 4 + 4 heads of 64 take 16.1 us (84 MB, 5.2 TB/s) where they took 22.0.  (Rows of tokens that are not
+// real are read with the others, and not written.)
 template <typename T, int L, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotary_quantize_tokens_kernel(RotaryParams p) {
   __shared__ float2 turn[kMaxAngles];

@@ -83,7 +83,8 @@ def linear_4bit(input: Tensor, codes: Tensor, scales: Tensor, zeros: Tensor | No
     ``zeros`` the same or None (8 everywhere); ``group_size`` 32, 64 or a multiple of 128 (the
     last group may be short).  N and K are arbitrary.  Codes meet the input exactly, sums are
     fp32, and each group's sum is scaled in fp32.  An input that is not finite makes its
-    token's outputs NaN.
+    token's outputs NaN, and so may inputs whose sums, of up to 31 times 128 of them, pass fp32
+    (from about 2^115; 2^117 in fp32).
     """
     return torch.ops.rlm_quantized.linear_4bit(input, codes, scales, zeros, group_size, bias)
 
