@@ -32,7 +32,8 @@ def quantize_4bit(weight: Tensor, group_size: int = 128, symmetric: bool = False
 
     Each group's range, widened to hold 0, is cut into 15 steps of one scale with a whole zero
     point, and values rounded to the nearest; ``symmetric``: the scale is the largest magnitude
-    / 7, the zero point 8 (no zeros).  A group of zeros has scale 1.
+    / 7, the zero point 8 (no zeros).  A group of zeros has scale 1; one with an infinity or NaN
+    stands for no finite values.
     """
     _check_group(group_size)
     if weight.dim() != 2 or not weight.is_floating_point():
@@ -47,11 +48,11 @@ def quantize_4bit(weight: Tensor, group_size: int = 128, symmetric: bool = False
     else:
         low, high = w.amin(-1).clamp_max(0), w.amax(-1).clamp_min(0)
         scales = (high - low) / 15
-    scales = torch.where(scales > 0, scales, torch.ones_like(scales))
+    scales = torch.where(scales == 0, torch.ones_like(scales), scales)
     if not symmetric:
         zeros = (-low / scales).round().clamp(0, 15)
     codes = (w / scales[..., None]).round() + (8 if symmetric else zeros[..., None])
-    codes = codes.clamp(0, 15).to(torch.uint8).view(n, -1)[:, :k].contiguous()
+    codes = codes.nan_to_num(0).clamp(0, 15).to(torch.uint8).view(n, -1)[:, :k].contiguous()
     return (codes, scales.T.contiguous(),
             None if zeros is None else zeros.T.contiguous())
 
