@@ -827,7 +827,8 @@ hipError_t rlm_rotary_to_quantized_caches(
     const rlm_tensor* out_query, hipStream_t stream);
 
 /*
- * Rows of an 8-bit cache in a float type: out [B,N,Hk,D] = cache * scale, an fp32 product rounded to it.
+ * Rows of an 8-bit cache in a float type: out [B,N,Hk,D] = cache * scale, an fp32 product
+ * rounded to it.
  * cache [B,T,Hk,D] RLM_F8E4M3 and scale [B,T,Hk] f32 of any strides; rows [B,N] int32/int64
  * names cache rows in any order (those outside [0, T) give zeros), or NULL for all of them
  * (N == T).

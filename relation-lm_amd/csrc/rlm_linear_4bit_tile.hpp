@@ -13,10 +13,10 @@
 //
 // Bound: instructions, and what a barrier a step leaves idle.  A wave's step of 64 rows, 64 tokens and 128
 // inputs has 71 products (64 of weights, 4 of input sums, 3 of what is taken back) and about 220 other vector
-// instructions (128 decode, 64 scale); each keeps its unit busy 45% of the time and waits take 30%.  4096 tokens of 4096 -> 4096 take 140 us in groups of 128
-// (980 TFLOP/s; the vendor's bf16 product of 8192 reaches 1560), 183 of 64 and 257 of 32, whose sums
-// are scaled two and four times as often.  With the scales loaded in the step that uses them 161 / 276 /
-// 267.  Rows that are no whole accesses: 184 with 4095 outputs, 320 with 4095 inputs too.
+// instructions (128 decode, 64 scale); each keeps its unit busy 45% of the time and waits take 30%.
+// 4096 tokens of 4096 -> 4096 take 140 us in groups of 128 (980 TFLOP/s; the vendor's bf16 product of 8192
+// reaches 1560), 183 of 64 and 257 of 32, whose sums are scaled two and four times as often.  With the scales
+// loaded in the step that uses them 161 / 276 / 267.  Rows that are no whole accesses: 184 with 4095 outputs, 320 with 4095 inputs too.
 //
 // fp32 inputs are staged as they are and split into three bf16 parts as they are read (24 bits; three
 // products a part of codes), and codes meet them as c - 8, so that only z - 8 is taken back: 438 us in groups of

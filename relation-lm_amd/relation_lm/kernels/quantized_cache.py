@@ -41,7 +41,7 @@ def rotary_to_quantized_caches(query: Tensor, key: Tensor, value: Tensor, positi
 def quantized_rows(cache: Tensor, scale: Tensor, rows: Tensor | None = None,
                    dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """Rows of an 8-bit cache in ``dtype`` (bfloat16, float16 or float32), each code times its
-    row's scale as an fp32 product, rounded to it: all of them, [B,T,Hk,D], or the ``rows`` [B,N] named (int32 or
-    int64 cache rows in any order, repeats allowed), [B,N,Hk,D] with zeros where a row is
-    outside [0, T)."""
+    row's scale as an fp32 product, rounded to it: all of them, [B,T,Hk,D], or the ``rows``
+    [B,N] named (int32 or int64 cache rows in any order, repeats allowed), [B,N,Hk,D] with zeros
+    where a row is outside [0, T)."""
     return torch.ops.rlm_quantized.quantized_rows(cache, scale, rows, dtype)
